@@ -342,6 +342,111 @@ int sed_resampler_get_filter(const sed_resampler* r, int32_t* up, int32_t* down,
 int sed_resampler_forward(const sed_resampler* r, const void* pcm, int32_t pcm_kind, float pcm_divisor, int64_t B,
                           int64_t L, int64_t pcm_stride, float* out, int64_t out_stride, void* stream);
 
+/* ---- sequence operators between the front-end and the decoders --------------------------------------------- */
+
+/* The operators of the networks this library's features feed and its decoders read that are no matrix product: a gated linear
+ * recurrence along the frames (the sequence mixer of the Audio-Mamba classifier, external/audio_mamba, whose native extension
+ * is not in the reference's tree), the short causal convolution in front of it, and a group norm with an activation on
+ * channels-last maps.  Element types are fp32, bf16 or fp16 (SED_F32 ..); arithmetic, states and sums are fp32, every output is
+ * rounded once.  Parameters (A, skip, dt_bias, weight, bias) and their gradients are fp32.
+ *
+ * frames: int32 DEVICE array [B] or NULL: clip b has frames[b] rows of its own (clamped to the row count).  Rows behind them are
+ * never read; outputs and gradients there are zero.  Strides are in elements, the last axis is contiguous; outputs and gradients
+ * are contiguous.  A pointer or stride that is no multiple of 4 (8) channels takes element-wise loads, no error.
+ * The caller gives the workspace the matching sed_*_workspace function asks for (bytes, 16-byte aligned); its contents need not
+ * live past the call's work on `stream`.  Results do not depend on timing: no sum is formed with atomics.  The entry points only
+ * launch kernels, so they can be captured into a HIP graph; two graphs that may run at the same time need workspaces of their own.
+ * All pointers belong to the current device. */
+enum { SED_F32 = 0, SED_BF16 = 1, SED_F16 = 2 };
+enum { SED_ACT_NONE = 0, SED_ACT_SILU = 1, SED_ACT_RELU = 2, SED_ACT_GELU = 3 };
+
+/* h_t[d,n] = exp(delta_t[d] A[d,n]) h_{t-1}[d,n] + delta_t[d] x_t[d] B_t[g,n],  delta = softplus(dt + dt_bias) or dt + dt_bias,
+ * y_t[d] = (sum_n C_t[g,n] h_t[d,n] + skip[d] x_t[d]) * silu(z_t[d]); channel d belongs to group g = d / (D / G). */
+typedef struct sed_scan_args {
+  int64_t B, L, D;          /* clips, frames, channels                                             */
+  int32_t N, G;             /* states of a channel (1..32), groups of B and C (D % G == 0)         */
+  int32_t dtype;            /* SED_F32 ..: x, dt, z, Bm, Cm, y and their gradients                 */
+  int32_t softplus;         /* 1: delta = softplus(dt + dt_bias)                                   */
+  int32_t reverse;          /* 1: from a clip's last own frame to its first                        */
+  const int32_t* frames;    /* [B] or NULL                                                         */
+  const void *x, *dt, *z;   /* [B][L][D]; z may be NULL (no gate)                                  */
+  const void *Bm, *Cm;      /* [B][L][G][N]                                                        */
+  int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, Bm_b, Bm_t, Bm_g, Cm_b, Cm_t, Cm_g;
+  const float *A, *skip, *dt_bias; /* [D][N], [D] or NULL, [D] or NULL                             */
+  const float* h0;          /* [B][D][N] state in front of the first frame, or NULL (zero)         */
+  float* h_last;            /* [B][D][N] state behind the last, or NULL; the state of a step       */
+  void* y;                  /* [B][L][D]                                                           */
+  float* saved;             /* sed_gated_scan_saved_floats floats for the gradient, or NULL        */
+  /* the gradient */
+  const void* dy;           /* [B][L][D]                                                           */
+  int64_t dy_b, dy_t;
+  const float* dh_last;     /* [B][D][N] or NULL                                                   */
+  void *dx, *ddt, *dz;      /* [B][L][D]; dz when z                                                */
+  void *dB, *dC;            /* [B][L][G][N]                                                        */
+  float *dA, *dskip, *ddt_bias, *dh0; /* [D][N], [D], [D], [B][D][N]; all but dA may be NULL       */
+  void* ws;
+  int64_t ws_bytes;
+} sed_scan_args;
+
+int64_t sed_gated_scan_saved_floats(int64_t B, int64_t L, int64_t D, int32_t N);
+int64_t sed_gated_scan_workspace(int64_t B, int64_t L, int64_t D, int32_t N, int32_t G, int32_t backward);
+int sed_gated_scan_forward(const sed_scan_args* args, void* stream);
+/* Reads the inputs of the forward call and its `saved`. */
+int sed_gated_scan_backward(const sed_scan_args* args, void* stream);
+/* One frame (L = 1) of B streams: h_last is read and overwritten; frames, h0, saved and the workspace are not used. */
+int sed_gated_scan_step(const sed_scan_args* args, void* stream);
+
+/* y_t[d] = act(bias[d] + sum_k weight[d,k] x_{t-W+1+k}[d]), x in front of the first frame = state or zero. */
+typedef struct sed_conv_args {
+  int64_t B, L, D;
+  int32_t W;                /* taps, 1..8                                                          */
+  int32_t dtype;            /* x, y, state and their gradients                                     */
+  int32_t act;              /* SED_ACT_NONE or SED_ACT_SILU                                        */
+  int32_t reverse;          /* 1: the window looks to later frames, the walk starts at the last    */
+  const int32_t* frames;    /* [B] or NULL                                                         */
+  const void* x;            /* [B][L][D]                                                           */
+  int64_t x_b, x_t;
+  const float *weight, *bias; /* [D][W], [D] or NULL                                               */
+  const void* state;        /* [B][W-1][D], oldest row first, or NULL                              */
+  void* y;                  /* [B][L][D]                                                           */
+  void* state_out;          /* [B][W-1][D] the last rows seen, or NULL; the state of a step        */
+  /* the gradient */
+  const void* dy;
+  int64_t dy_b, dy_t;
+  const void* dstate_out;   /* [B][W-1][D] or NULL                                                 */
+  void *dx, *dstate;        /* [B][L][D]; [B][W-1][D] or NULL                                      */
+  float *dw, *db;           /* [D][W]; [D] or NULL                                                 */
+  void* ws;
+  int64_t ws_bytes;
+} sed_conv_args;
+
+int64_t sed_causal_conv_workspace(int64_t B, int64_t L, int64_t D, int32_t W); /* of the gradient    */
+int sed_causal_conv_forward(const sed_conv_args* args, void* stream);
+int sed_causal_conv_backward(const sed_conv_args* args, void* stream);
+/* One frame (L = 1) of B streams: state_out moves up by the new row in place. */
+int sed_causal_conv_step(const sed_conv_args* args, void* stream);
+
+/* y = act((x - mean) * rstd * weight + bias), mean and biased variance over a clip's own frames, F and a group's channels. */
+typedef struct sed_norm_args {
+  int64_t B, T, F, C, G;    /* x is [B][T][F][C], C % G == 0, B <= 65535                           */
+  int32_t dtype, act;
+  float eps;
+  const int32_t* frames;    /* [B] of T, or NULL                                                   */
+  const void* x;
+  const float *weight, *bias; /* [C] or NULL                                                       */
+  void* y;
+  float *mean, *rstd;       /* [B][G]: written by the forward call, read by the gradient           */
+  const void* dy;
+  void* dx;
+  float *dw, *db;           /* [C] or NULL                                                         */
+  void* ws;
+  int64_t ws_bytes;
+} sed_norm_args;
+
+int64_t sed_group_norm_workspace(int64_t B, int64_t T, int64_t F, int64_t C, int64_t G);
+int sed_group_norm_forward(const sed_norm_args* args, void* stream);
+int sed_group_norm_backward(const sed_norm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

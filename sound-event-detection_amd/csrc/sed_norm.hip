@@ -1,0 +1,436 @@
+// Group norm with an activation on channels-last maps (B, T, F, C), over a clip's own frames, and its gradient, for gfx950.
+//
+//   y = act((x - mean[b,g]) rstd[b,g] w[c] + bias[c]),  mean and variance over the clip's frames x F x the group's channels
+//
+// Bound: HBM.  The maps are walked row by row (a row = the C channels of one place), 16 bytes a lane, lanes along channels, so
+// every access is whole lines whatever the group's width.  Every lane sums its own channels relative to the first value it
+// meets there (a far mean costs no precision), joined per channel, then per group with the exact formula for joined means.
+// The gradient needs two sums a group, sum q and sum q n (q = du w, n the normalised value), which follow from the channels'
+// sums of du and du n: those are the bias' and the weight's gradients at the same time.
+#include "seq_core.h"
+
+#include <algorithm>
+
+namespace sed {
+namespace {
+
+struct NormParams {
+  sed_norm_args a;
+  int64_t S;         // places of a clip
+  int32_t nv, nb;    // vectors of a row, lanes along a row
+  int32_t blocks;    // blocks a clip is cut into
+  int64_t rows;      // places of a block
+  float* part;       // [B][blocks][2][C]: (mean, sum of squares about it), or (sum du, sum du n)
+  float* chan;       // [B][2][C]
+  float* gsum;       // [B][G][2]: means of q and q n
+};
+
+__device__ __forceinline__ int64_t own_of(const NormParams& p, int64_t b) {
+  const sed_norm_args& a = p.a;
+  const int64_t t = a.frames ? std::max<int64_t>(0, std::min<int64_t>(a.T, a.frames[b])) : a.T;
+  return t * a.F;
+}
+
+struct Cell {
+  int64_t b, r0, r1, c;
+  int ty, step;
+  bool in;
+};
+template <int V>
+__device__ __forceinline__ Cell cell(const NormParams& p) {
+  Cell q;
+  q.b = blockIdx.y;
+  q.r0 = blockIdx.x * p.rows;
+  q.r1 = std::min<int64_t>(q.r0 + p.rows, p.S);
+  const int tx = threadIdx.x % p.nb, v = blockIdx.z * p.nb + tx;
+  q.ty = threadIdx.x / p.nb;
+  q.step = 256 / p.nb;
+  q.c = (int64_t)v * V;
+  q.in = v < p.nv && q.ty < q.step;
+  return q;
+}
+
+// Sums of a block per channel: the lanes of a channel put (count, value, value) into LDS, lane 0 of it joins them.
+template <class T, int V, bool VEC>
+__global__ void __launch_bounds__(256) norm_stats_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  const Cell q = cell<V>(p);
+  const int64_t end = std::min<int64_t>(q.r1, own_of(p, q.b));
+  if (q.r0 >= end) return;
+  __shared__ float s_m[256][V + 1], s_v[256][V + 1];
+  __shared__ int s_n[256];
+  float k[V], s1[V], s2[V];
+  int64_t n = 0;
+  if (q.in) {
+    const T* x = static_cast<const T*>(a.x) + q.b * p.S * a.C + q.c;
+    int64_t r = q.r0 + q.ty;
+    if (r < end) {
+      load_n<T, V, VEC>(x + r * a.C, V, k);
+#pragma unroll
+      for (int c = 0; c < V; ++c) s1[c] = s2[c] = 0.0f;
+      n = 1;
+      r += q.step;
+#pragma unroll 4
+      for (; r < end; r += q.step) {
+        float v[V];
+        load_n<T, V, VEC>(x + r * a.C, V, v);
+        ++n;
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          const float e = v[c] - k[c];
+          s1[c] += e;
+          s2[c] = fmaf(e, e, s2[c]);
+        }
+      }
+      const float inv = 1.0f / (float)n;
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const float m = s1[c] * inv;
+        s_m[threadIdx.x][c] = k[c] + m;
+        s_v[threadIdx.x][c] = fmaf(-m, s1[c], s2[c]);
+      }
+    }
+  }
+  s_n[threadIdx.x] = (int)n;
+  __syncthreads();
+  if (q.in && q.ty == 0) {
+    float mean[V], var[V];
+    float count = 0.0f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) mean[c] = var[c] = 0.0f;
+    for (int y = 0; y < q.step; ++y) {
+      const int at = y * p.nb + threadIdx.x;
+      const float m = (float)s_n[at];
+      if (m == 0.0f) break;
+      const float all = count + m, part = m / all;
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const float e = s_m[at][c] - mean[c];
+        mean[c] = fmaf(e, part, mean[c]);
+        var[c] += fmaf(e * e, count * part, s_v[at][c]);
+      }
+      count = all;
+    }
+    float* to = p.part + (q.b * p.blocks + blockIdx.x) * 2 * a.C + q.c;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      to[c] = mean[c];
+      to[a.C + c] = var[c];
+    }
+  }
+}
+
+__device__ __forceinline__ float block_sum(float v, float* s) {
+  v = wave_sum(v);
+  __syncthreads();
+  if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
+  __syncthreads();
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+// mean and rstd of a (clip, group) out of the blocks' channels.
+__global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  __shared__ float s[4];
+  const int64_t g = blockIdx.x % a.G, b = blockIdx.x / a.G, cg = a.C / a.G, own = own_of(p, b);
+  const int64_t blocks = (own + p.rows - 1) / p.rows, n = blocks * cg;
+  const float total = (float)own * (float)cg;
+  const float* part = p.part + b * p.blocks * 2 * a.C + g * cg;
+  float mean = 0.0f, var = 0.0f;
+  if (own > 0) {
+    // means relative to the first one: their spread is what counts
+    const float k = part[0];
+    float v = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+      const int64_t q = i / cg;
+      const float m = (float)(std::min<int64_t>((q + 1) * p.rows, own) - q * p.rows);
+      v = fmaf(m, part[q * 2 * a.C + i % cg] - k, v);
+    }
+    mean = k + block_sum(v, s) / total;
+    v = 0.0f;
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+      const int64_t q = i / cg;
+      const float m = (float)(std::min<int64_t>((q + 1) * p.rows, own) - q * p.rows);
+      const float e = part[q * 2 * a.C + i % cg] - mean;
+      v += fmaf(m * e, e, part[q * 2 * a.C + a.C + i % cg]);
+    }
+    var = block_sum(v, s) / total;
+  }
+  if (threadIdx.x == 0) {
+    a.mean[b * a.G + g] = mean;
+    a.rstd[b * a.G + g] = 1.0f / sqrtf(var + a.eps);
+  }
+}
+
+// mean, scale and shift of a lane's channels: n = (x - mean) rstd, u = n w + bias.
+template <int V>
+__device__ __forceinline__ void channels(const NormParams& p, const Cell& q, float (&mean)[V], float (&rstd)[V], float (&w)[V], float (&bias)[V]) {
+  const sed_norm_args& a = p.a;
+  const int64_t cg = a.C / a.G;
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int64_t g = (q.c + c) / cg;
+    mean[c] = a.mean[q.b * a.G + g];
+    rstd[c] = a.rstd[q.b * a.G + g];
+    w[c] = a.weight ? a.weight[q.c + c] : 1.0f;
+    bias[c] = a.bias ? a.bias[q.c + c] : 0.0f;
+  }
+}
+
+template <class T, int V, bool VEC, int ACT>
+__global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  const Cell q = cell<V>(p);
+  if (!q.in) return;
+  const int64_t own = own_of(p, q.b);
+  float mean[V], rstd[V], w[V], bias[V];
+  channels<V>(p, q, mean, rstd, w, bias);
+#pragma unroll
+  for (int c = 0; c < V; ++c) w[c] *= rstd[c];
+  const int64_t at = q.b * p.S * a.C + q.c;
+  const T* x = static_cast<const T*>(a.x) + at;
+  T* y = static_cast<T*>(a.y) + at;
+#pragma unroll 4
+  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
+    float v[V];
+    load_n<T, V, VEC>(x + r * a.C, r < own ? V : 0, v);
+#pragma unroll
+    for (int c = 0; c < V; ++c) v[c] = r < own ? act<ACT>(fmaf(v[c] - mean[c], w[c], bias[c])) : 0.0f;
+    store_n<T, V, VEC>(y + r * a.C, V, v);
+  }
+}
+
+template <class T, int V, bool VEC, int ACT>
+__global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  const Cell q = cell<V>(p);
+  const int64_t end = std::min<int64_t>(q.r1, own_of(p, q.b));
+  __shared__ float s_1[256][V + 1], s_2[256][V + 1];
+  float s1[V], s2[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) s1[c] = s2[c] = 0.0f;
+  if (q.in) {
+    float mean[V], rstd[V], w[V], bias[V];
+    channels<V>(p, q, mean, rstd, w, bias);
+    const int64_t at = q.b * p.S * a.C + q.c;
+    const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
+#pragma unroll 2
+    for (int64_t r = q.r0 + q.ty; r < end; r += q.step) {
+      float v[V], g[V];
+      load_n<T, V, VEC>(x + r * a.C, V, v);
+      load_n<T, V, VEC>(dy + r * a.C, V, g);
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        const float n = (v[c] - mean[c]) * rstd[c], du = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c]));
+        s1[c] += du;
+        s2[c] = fmaf(du, n, s2[c]);
+      }
+    }
+  }
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    s_1[threadIdx.x][c] = s1[c];
+    s_2[threadIdx.x][c] = s2[c];
+  }
+  __syncthreads();
+  if (q.in && q.ty == 0) {
+    for (int y = 1; y < q.step; ++y)
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        s1[c] += s_1[y * p.nb + threadIdx.x][c];
+        s2[c] += s_2[y * p.nb + threadIdx.x][c];
+      }
+    float* to = p.part + (q.b * p.blocks + blockIdx.x) * 2 * a.C + q.c;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      to[c] = s1[c];
+      to[a.C + c] = s2[c];
+    }
+  }
+}
+
+// A clip's channels over its blocks, and the group's two means.
+__global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  __shared__ float s[4];
+  const int64_t g = blockIdx.x % a.G, b = blockIdx.x / a.G, cg = a.C / a.G, own = own_of(p, b);
+  const float total = (float)own * (float)cg;
+  float q1 = 0.0f, q2 = 0.0f;
+  for (int64_t i = threadIdx.x; i < cg; i += 256) {
+    const int64_t c = g * cg + i;
+    const float* part = p.part + b * p.blocks * 2 * a.C + c;
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < p.blocks; ++k) {
+      s1 += part[(int64_t)k * 2 * a.C];
+      s2 += part[(int64_t)k * 2 * a.C + a.C];
+    }
+    p.chan[b * 2 * a.C + c] = s1;
+    p.chan[b * 2 * a.C + a.C + c] = s2;
+    const float w = a.weight ? a.weight[c] : 1.0f;
+    q1 = fmaf(w, s1, q1);
+    q2 = fmaf(w, s2, q2);
+  }
+  q1 = block_sum(q1, s);
+  q2 = block_sum(q2, s);
+  if (threadIdx.x == 0) {
+    p.gsum[(b * a.G + g) * 2] = own > 0 ? q1 / total : 0.0f;
+    p.gsum[(b * a.G + g) * 2 + 1] = own > 0 ? q2 / total : 0.0f;
+  }
+}
+
+// dw and db: the clips' channels, added in order.
+__global__ void __launch_bounds__(256) norm_param_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= 2 * a.C) return;
+  float v = 0.0f;
+#pragma unroll 4
+  for (int64_t b = 0; b < a.B; ++b) v += p.chan[b * 2 * a.C + c];
+  if (c < a.C) {
+    if (a.db) a.db[c] = v;
+  } else if (a.dw) {
+    a.dw[c - a.C] = v;
+  }
+}
+
+template <class T, int V, bool VEC, int ACT>
+__global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  const Cell q = cell<V>(p);
+  if (!q.in) return;
+  const int64_t own = own_of(p, q.b), cg = a.C / a.G;
+  float mean[V], rstd[V], w[V], bias[V], m1[V], m2[V];
+  channels<V>(p, q, mean, rstd, w, bias);
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    const int64_t g = (q.c + c) / cg;
+    m1[c] = p.gsum[(q.b * a.G + g) * 2];
+    m2[c] = p.gsum[(q.b * a.G + g) * 2 + 1];
+  }
+  const int64_t at = q.b * p.S * a.C + q.c;
+  const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
+  T* dx = static_cast<T*>(a.dx) + at;
+#pragma unroll 2
+  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
+    float v[V], g[V];
+    load_n<T, V, VEC>(x + r * a.C, r < own ? V : 0, v);
+    load_n<T, V, VEC>(dy + r * a.C, r < own ? V : 0, g);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const float n = (v[c] - mean[c]) * rstd[c], qv = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c])) * w[c];
+      v[c] = r < own ? rstd[c] * (qv - fmaf(n, m2[c], m1[c])) : 0.0f;
+    }
+    store_n<T, V, VEC>(dx + r * a.C, V, v);
+  }
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+
+bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+int check_args(const sed_norm_args* a) {
+  if (!a || a->B < 0 || a->T < 0 || a->F < 1 || a->C < 1 || a->G < 1 || a->C % a->G || !(a->eps >= 0.0f)) return SED_ERR_BAD_ARG;
+  if (a->dtype != SED_F32 && a->dtype != SED_BF16 && a->dtype != SED_F16) return SED_ERR_BAD_ARG;
+  if (a->act < SED_ACT_NONE || a->act > SED_ACT_GELU) return SED_ERR_BAD_ARG;
+  if (a->B > 0 && a->T > 0 && (!a->x || !a->mean || !a->rstd)) return SED_ERR_BAD_ARG;
+  if (a->B > 65535) return SED_ERR_CAPACITY;
+  return SED_OK;
+}
+
+struct Layout {
+  int64_t rows, part, chan, gsum, total;
+  int32_t blocks;
+};
+// Blocks of a clip: 4096 over the batch fill the card eight times over; a block walks 32 places at least, so that its sums cost
+// little beside its rows.
+Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
+  Layout l{};
+  int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + 31) / 32, std::max<int64_t>(1, 4096 / std::max<int64_t>(1, B))));
+  l.rows = std::max<int64_t>(1, (S + n - 1) / n);
+  l.blocks = (int32_t)std::max<int64_t>(1, (S + l.rows - 1) / l.rows);
+  int64_t at = 0;
+  const auto take = [&](int64_t k) { const int64_t o = at; at += (k + 63) / 64 * 64; return o; };
+  l.part = take(B * l.blocks * 2 * C);
+  l.chan = take(B * 2 * C);
+  l.gsum = take(B * G * 2);
+  l.total = at;
+  return l;
+}
+
+template <class T, int V, bool VEC, int ACT>
+int launch(const NormParams& p, bool back, hipStream_t s) {
+  const sed_norm_args& a = p.a;
+  const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb));
+  const unsigned groups = (unsigned)(a.B * a.G);
+  if (!back) {
+    norm_stats_kernel<T, V, VEC><<<grid, 256, 0, s>>>(p);
+    norm_join_kernel<<<groups, 256, 0, s>>>(p);
+    norm_apply_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
+  } else {
+    norm_grad_sums_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
+    norm_grad_join_kernel<<<groups, 256, 0, s>>>(p);
+    norm_grad_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
+    if (a.dw || a.db) norm_param_kernel<<<(unsigned)((2 * a.C + 255) / 256), 256, 0, s>>>(p);
+  }
+  return seq_status(hipGetLastError());
+}
+
+template <class T, int V, bool VEC>
+int go_act(const NormParams& p, bool back, hipStream_t s) {
+  switch (p.a.act) {
+    case SED_ACT_SILU: return launch<T, V, VEC, SED_ACT_SILU>(p, back, s);
+    case SED_ACT_RELU: return launch<T, V, VEC, SED_ACT_RELU>(p, back, s);
+    case SED_ACT_GELU: return launch<T, V, VEC, SED_ACT_GELU>(p, back, s);
+    default: return launch<T, V, VEC, SED_ACT_NONE>(p, back, s);
+  }
+}
+
+int run(const sed_norm_args* args, bool back, void* stream) {
+  NormParams p{};
+  p.a = *args;
+  sed_norm_args& a = p.a;
+  p.S = a.T * a.F;
+  const Layout l = layout_of(a.B, p.S, a.C, a.G);
+  if (!a.ws || a.ws_bytes < l.total * 4 || !aligned(a.ws, 16)) return SED_ERR_CAPACITY;
+  if (a.B * a.G > 0x7fffffff) return SED_ERR_CAPACITY;
+  const int V = a.dtype == SED_F32 ? 4 : 8;
+  const bool vec = a.C % V == 0 && aligned(a.x, 16) && aligned(a.y, 16) && aligned(a.dy, 16) && aligned(a.dx, 16);
+  p.nv = (int32_t)(vec ? a.C / V : a.C);
+  p.nb = std::min(p.nv, 256);
+  if ((p.nv + p.nb - 1) / p.nb > 65535) return SED_ERR_CAPACITY;
+  p.blocks = l.blocks;
+  p.rows = l.rows;
+  float* ws = static_cast<float*>(a.ws);
+  p.part = ws + l.part;
+  p.chan = ws + l.chan;
+  p.gsum = ws + l.gsum;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.dtype == SED_F32) return vec ? go_act<float, 4, true>(p, back, s) : go_act<float, 1, false>(p, back, s);
+  if (a.dtype == SED_BF16) return vec ? go_act<bf16, 8, true>(p, back, s) : go_act<bf16, 1, false>(p, back, s);
+  return vec ? go_act<f16, 8, true>(p, back, s) : go_act<f16, 1, false>(p, back, s);
+}
+
+}  // namespace
+}  // namespace sed
+
+extern "C" int64_t sed_group_norm_workspace(int64_t B, int64_t T, int64_t F, int64_t C, int64_t G) {
+  if (B < 0 || T < 0 || F < 1 || C < 1 || G < 1 || C % G) return SED_ERR_BAD_ARG;
+  return sed::layout_of(B, T * F, C, G).total * 4;
+}
+
+extern "C" int sed_group_norm_forward(const sed_norm_args* args, void* stream) {
+  const int rc = sed::check_args(args);
+  if (rc != SED_OK) return rc;
+  if (args->B == 0 || args->T == 0) return SED_OK;
+  if (!args->y) return SED_ERR_BAD_ARG;
+  return sed::run(args, false, stream);
+}
+
+extern "C" int sed_group_norm_backward(const sed_norm_args* args, void* stream) {
+  const int rc = sed::check_args(args);
+  if (rc != SED_OK) return rc;
+  if (args->B == 0 || args->T == 0) return SED_OK;
+  if (!args->dy || !args->dx) return SED_ERR_BAD_ARG;
+  return sed::run(args, true, stream);
+}

@@ -1,0 +1,135 @@
+// What the sequence operators (sed_scan.hip, sed_conv.hip, sed_norm.hip) share: loads and stores of several channels at a
+// time in the three element types, the activations with their slopes, and cross-lane sums.  gfx950 only, 64-lane waves.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sed_hip.h"
+
+namespace sed {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// 2^x and 1/x as the hardware has them (1 ulp; results below the normal range are zero)
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float rcp_hw(float x) { return __builtin_amdgcn_rcpf(x); }
+
+// 1 / (1 + e^-x); e^-x overflows to infinity for x < -88, whose reciprocal is the right 0
+__device__ __forceinline__ float sigmoid(float x) { return rcp_hw(1.0f + exp2_hw(-kLog2e * x)); }
+
+// ln(1 + e^x) = max(x, 0) + log1p(e), e = e^-|x| in (0, 1].  log1p(e) = 2 atanh(e / (2 + e)), the odd series in
+// s = e / (2 + e) <= 1/3 to s^15 (the next term is below 1.4e-9 of the sum), so small e keep their relative precision.
+__device__ __forceinline__ float softplus(float x) {
+  const float e = exp2_hw(-kLog2e * fabsf(x));
+  const float s = e * rcp_hw(2.0f + e), q = s * s;
+  float p = 1.0f / 15.0f;
+  p = fmaf(p, q, 1.0f / 13.0f);
+  p = fmaf(p, q, 1.0f / 11.0f);
+  p = fmaf(p, q, 1.0f / 9.0f);
+  p = fmaf(p, q, 1.0f / 7.0f);
+  p = fmaf(p, q, 1.0f / 5.0f);
+  p = fmaf(p, q, 1.0f / 3.0f);
+  p = fmaf(p, q, 1.0f);
+  return fmaf(2.0f * s, p, fmaxf(x, 0.0f));  // a NaN stays one through e
+}
+
+// ---- element types: fp32 arithmetic, one rounding (to nearest, ties to even) at the store ------------------------------
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+
+// V consecutive elements as fp32.  VEC: the address is a multiple of the vector's size, one load.  Otherwise the first n.
+template <class T, int V, bool VEC>
+__device__ __forceinline__ void load_n(const T* p, int n, float* out) {
+  if constexpr (VEC) {
+    typedef T vt __attribute__((ext_vector_type(V)));
+    if (n > 0) {
+      const vt v = *reinterpret_cast<const vt*>(p);
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = (float)v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) out[i] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) out[i] = i < n ? (float)p[i] : 0.0f;
+  }
+}
+
+template <class T, int V, bool VEC>
+__device__ __forceinline__ void store_n(T* p, int n, const float* in) {
+  if constexpr (VEC) {
+    typedef T vt __attribute__((ext_vector_type(V)));
+    vt v;
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = (T)in[i];
+    if (n > 0) *reinterpret_cast<vt*>(p) = v;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = (T)in[i];
+  }
+}
+
+// ---- activations --------------------------------------------------------------------------------------------------------
+
+// act(u) and, where SLOPE, act'(u).
+template <int ACT>
+__device__ __forceinline__ float act(float u) {
+  if constexpr (ACT == SED_ACT_SILU) return u * sigmoid(u);
+  if constexpr (ACT == SED_ACT_RELU) return u > 0.0f ? u : (u != u ? u : 0.0f);
+  if constexpr (ACT == SED_ACT_GELU) return u * (0.5f * erfcf(-0.70710678118654752440f * u));
+  return u;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float u) {
+  if constexpr (ACT == SED_ACT_SILU) {
+    const float s = sigmoid(u);
+    return s * fmaf(u, 1.0f - s, 1.0f);
+  }
+  if constexpr (ACT == SED_ACT_RELU) return u > 0.0f ? 1.0f : 0.0f;
+  if constexpr (ACT == SED_ACT_GELU)
+    return fmaf(u * 0.39894228040143267794f, exp2_hw(-0.5f * kLog2e * u * u), 0.5f * erfcf(-0.70710678118654752440f * u));
+  return 1.0f;
+}
+
+// ---- cross-lane sums ----------------------------------------------------------------------------------------------------
+
+// Exchanges between lane halves (32) or between neighbouring rows of 16 lanes (16), then one add: lanes whose bit is 0 get
+// a's sum over the pair of lanes that differ in that bit, the others b's.
+__device__ __forceinline__ float fold32(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128;  // quad_perm [1,0,3,2], [2,3,0,1]; i -> 7 - i in eights; i -> i ^ 8
+// Sum over the 16 lanes of a row, in every lane of it.
+__device__ __forceinline__ float row_sum(float x) {
+  x += dpp<kXor1>(x);
+  x += dpp<kXor2>(x);
+  x += dpp<kHalfMirror>(x);
+  x += dpp<kRor8>(x);
+  return x;
+}
+// Sum over the wave, in every lane.
+__device__ __forceinline__ float wave_sum(float x) {
+  x = row_sum(x);
+  x = fold16(x, x);
+  return fold32(x, x);
+}
+
+inline int seq_status(hipError_t e) { return e == hipSuccess ? SED_OK : SED_ERR_HIP - (int)e; }
+
+}  // namespace sed

@@ -9,6 +9,7 @@ from .decode import (decode_predictions, decode_probabilities, detect_onsets_off
 from .handoff import cut_events, cut_events_from_audio, fbank_of_events, logmel_of_events
 from .metrics import EventBasedMetrics, SegmentBasedMetrics, calculate_metrics
 from .resample import Resampler, resample
+from .sequence import causal_conv, causal_conv_step, gated_scan, gated_scan_step, group_norm_act
 from . import sharding
 
 __version__ = _lib.lib.sed_version().decode()

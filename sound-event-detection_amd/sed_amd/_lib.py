@@ -28,6 +28,8 @@ PCM_F32, PCM_I16 = 0, 1
 WIN_CENTER, WIN_LEFT = 0, 1
 WINDOW_HANN_PERIODIC, WINDOW_HANN_SYMMETRIC = 0, 1
 SMOOTH_NONE, SMOOTH_MEDIAN3, SMOOTH_GAUSS25 = 0, 1, 2
+F32, BF16, F16 = 0, 1, 2
+ACT_NONE, ACT_SILU, ACT_RELU, ACT_GELU = 0, 1, 2, 3
 
 
 class FrontendCfg(C.Structure):
@@ -45,6 +47,31 @@ class FrontendCfg(C.Structure):
 
 
 _vp, _i32, _i64, _f32, _f64 = C.c_void_p, C.c_int32, C.c_int64, C.c_float, C.c_double
+
+
+def _fields(spec):
+    """[("a", c_int64), ..] of "i64 a b, ptr c": the members of a struct of the header in order."""
+    types = {"i32": _i32, "i64": _i64, "f32": _f32, "ptr": _vp}
+    return [(name, types[words[0]]) for words in (part.split() for part in spec.split(",")) for name in words[1:]]
+
+
+class ScanArgs(C.Structure):
+    """sed_scan_args."""
+    _fields_ = _fields("i64 B L D, i32 N G dtype softplus reverse, ptr frames x dt z Bm Cm, "
+                       "i64 x_b x_t dt_b dt_t z_b z_t Bm_b Bm_t Bm_g Cm_b Cm_t Cm_g, ptr A skip dt_bias h0 h_last y saved dy, "
+                       "i64 dy_b dy_t, ptr dh_last dx ddt dz dB dC dA dskip ddt_bias dh0 ws, i64 ws_bytes")
+
+
+class ConvArgs(C.Structure):
+    """sed_conv_args."""
+    _fields_ = _fields("i64 B L D, i32 W dtype act reverse, ptr frames x, i64 x_b x_t, ptr weight bias state y state_out dy, "
+                       "i64 dy_b dy_t, ptr dstate_out dx dstate dw db ws, i64 ws_bytes")
+
+
+class NormArgs(C.Structure):
+    """sed_norm_args."""
+    _fields_ = _fields("i64 B T F C G, i32 dtype act, f32 eps, ptr frames x weight bias y mean rstd dy dx dw db ws, i64 ws_bytes")
+
 
 # name -> (restype, argtypes); every symbol declared in include/sed_hip.h
 SIGNATURES = {
@@ -86,6 +113,18 @@ SIGNATURES = {
     "sed_resampler_out_len": (_i64, [_vp, _i64]),
     "sed_resampler_get_filter": (C.c_int, [_vp, C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32), _vp]),
     "sed_resampler_forward": (C.c_int, [_vp, _vp, _i32, _f32, _i64, _i64, _i64, _vp, _i64, _vp]),
+    "sed_gated_scan_saved_floats": (_i64, [_i64, _i64, _i64, _i32]),
+    "sed_gated_scan_workspace": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32]),
+    "sed_gated_scan_forward": (C.c_int, [C.POINTER(ScanArgs), _vp]),
+    "sed_gated_scan_backward": (C.c_int, [C.POINTER(ScanArgs), _vp]),
+    "sed_gated_scan_step": (C.c_int, [C.POINTER(ScanArgs), _vp]),
+    "sed_causal_conv_workspace": (_i64, [_i64, _i64, _i64, _i32]),
+    "sed_causal_conv_forward": (C.c_int, [C.POINTER(ConvArgs), _vp]),
+    "sed_causal_conv_backward": (C.c_int, [C.POINTER(ConvArgs), _vp]),
+    "sed_causal_conv_step": (C.c_int, [C.POINTER(ConvArgs), _vp]),
+    "sed_group_norm_workspace": (_i64, [_i64, _i64, _i64, _i64, _i64]),
+    "sed_group_norm_forward": (C.c_int, [C.POINTER(NormArgs), _vp]),
+    "sed_group_norm_backward": (C.c_int, [C.POINTER(NormArgs), _vp]),
     "sed_cut_events": (C.c_int, [_vp, _i32, _f32, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _vp]),
 }
 

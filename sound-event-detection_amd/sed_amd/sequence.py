@@ -1,0 +1,463 @@
+"""Sequence operators between the front-ends and the decoders: what the networks that read this package's features need besides
+matrix products, with gradients, and in the form a stream calls frame by frame.
+
+`gated_scan` is the gated linear recurrence along the frames that the Audio-Mamba classifier mixes its patches with
+(external/audio_mamba imports it from a native extension that is not in its tree), `causal_conv` the short depthwise
+convolution in front of it, `group_norm_act` a group norm with an activation on channels-last feature maps (B, T, F, C) or
+sequences (B, T, C).  All take `frames`, the clips' own row counts, as reshape_wav2img does: rows behind a clip's own are never
+read, and are zero in every output and gradient.  Arithmetic, states and sums are fp32 whatever the element type (fp32, bf16,
+fp16); every output is rounded once.  There is no CPU path.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+
+_DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
+_ACTIVATIONS = {None: L.ACT_NONE, "silu": L.ACT_SILU, "relu": L.ACT_RELU, "gelu": L.ACT_GELU}
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _rows(t):
+    """t with a contiguous last axis (views of a joint projection are read in place)."""
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _param(t):
+    """A parameter as the kernels read it; its gradient comes back in the parameter's own type."""
+    return None if t is None else t.float().contiguous()
+
+
+def _check_x(what, x, dim):
+    if not torch.is_tensor(x) or not x.is_cuda:
+        raise RuntimeError(f"{what}: x is on {getattr(x, 'device', type(x))}; the sequence operators run only on a ROCm device (no CPU path)")
+    if x.dtype not in _DTYPES:
+        raise TypeError(f"{what}: x is {x.dtype}; fp32, bf16 and fp16 are supported")
+    if x.dim() != dim or x.shape[-1] < 1:
+        raise ValueError(f"{what}: x has shape {tuple(x.shape)}; {dim} axes with at least one channel are needed")
+
+
+def _check(what, name, t, x, shape, dtype=None):
+    """t: a tensor of this shape on x's device, of x's type (dtype None), of one type, or of any floating type ('float')."""
+    if not torch.is_tensor(t) or t.device != x.device:
+        raise RuntimeError(f"{what}: {name} has to be a tensor on {x.device}")
+    if dtype == "float":
+        if not t.is_floating_point():
+            raise TypeError(f"{what}: {name} is {t.dtype}; a floating type is needed")
+    elif t.dtype != (dtype or x.dtype):
+        raise TypeError(f"{what}: {name} is {t.dtype}; {dtype or x.dtype} is needed")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}; {tuple(shape)} is needed")
+
+
+def _check_frames(what, frames, x):
+    if frames is not None and not (torch.is_tensor(frames) and frames.device == x.device and frames.dtype == torch.int32 and
+                                   frames.shape == (x.shape[0],) and frames.is_contiguous()):
+        raise TypeError(f"{what}: frames: a contiguous int32 tensor with one entry per clip on x's device")
+
+
+def _workspace(nbytes, dev):
+    L.check(nbytes, "workspace")
+    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
+
+
+def _call(fn, args, dev, what):
+    if torch.cuda.current_device() == dev.index:
+        L.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream), what)
+    else:
+        with torch.cuda.device(dev):
+            L.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream), what)
+
+
+def _no_grad_only(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} updates the state in place and keeps nothing for a gradient: call it under torch.no_grad()")
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---- gated linear recurrence --------------------------------------------------------------------------------------------
+
+
+def _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state):
+    a = L.ScanArgs()
+    a.B, a.L, a.D = x.shape
+    a.G, a.N = B.shape[2], B.shape[3]
+    a.dtype, a.softplus, a.reverse = _DTYPES[x.dtype], int(softplus), int(reverse)
+    a.frames = _ptr(frames)
+    a.x, a.dt, a.z, a.Bm, a.Cm = x.data_ptr(), dt.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr()
+    a.x_b, a.x_t = x.stride(0), x.stride(1)
+    a.dt_b, a.dt_t = dt.stride(0), dt.stride(1)
+    if z is not None:
+        a.z_b, a.z_t = z.stride(0), z.stride(1)
+    a.Bm_b, a.Bm_t, a.Bm_g = B.stride()[:3]
+    a.Cm_b, a.Cm_t, a.Cm_g = Cm.stride()[:3]
+    a.A, a.skip, a.dt_bias, a.h0 = A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(state)
+    return a
+
+
+def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state, want_last, want_saved):
+    b, n_frames, d = x.shape
+    g, n = B.shape[2], B.shape[3]
+    dev = x.device
+    y = torch.empty((b, n_frames, d), dtype=x.dtype, device=dev)
+    last = torch.empty((b, d, n), dtype=torch.float32, device=dev) if want_last else None
+    saved = None
+    if b == 0 or n_frames == 0:
+        if want_last:
+            last.zero_() if state is None else last.copy_(state)
+        return y, last, saved
+    a = _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state)
+    if want_saved:
+        saved = torch.empty(L.lib.sed_gated_scan_saved_floats(b, n_frames, d, n), dtype=torch.float32, device=dev)
+        a.saved = saved.data_ptr()
+    nbytes = L.lib.sed_gated_scan_workspace(b, n_frames, d, n, g, 0)
+    if nbytes:
+        ws = _workspace(nbytes, dev)
+        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+    a.y, a.h_last = y.data_ptr(), _ptr(last)
+    _call(L.lib.sed_gated_scan_forward, a, dev, "sed_gated_scan_forward")
+    return y, last, saved
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, B, Cm, D, z, dt_bias, state, softplus, frames, reverse, want_last):
+        y, last, saved = _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state, want_last, True)
+        ctx.save_for_backward(x, dt, A, B, Cm, D, z, dt_bias, state, frames, saved)
+        ctx.flags = (softplus, reverse)
+        ctx.set_materialize_grads(False)
+        return (y, last) if want_last else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dlast=None):
+        x, dt, A, B, Cm, D, z, dt_bias, state, frames, saved = ctx.saved_tensors
+        softplus, reverse = ctx.flags
+        b, n_frames, d = x.shape
+        g, n = B.shape[2], B.shape[3]
+        dev = x.device
+        new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=dev)  # noqa: E731
+        dx, ddt, dA, dB, dC, dD, dz, dbias, dstate = (new(t) for t in (x, dt, A, B, Cm, D, z, dt_bias, state))
+        if b == 0 or n_frames == 0:
+            for t in (dA, dD, dbias, dstate):
+                if t is not None:
+                    t.zero_()
+            if dstate is not None and dlast is not None:
+                dstate.copy_(dlast)
+            return dx, ddt, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None
+        dy = torch.zeros((b, n_frames, d), dtype=x.dtype, device=dev) if dy is None else _rows(dy)
+        dlast = None if dlast is None else dlast.contiguous()
+        a = _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state)
+        a.saved = saved.data_ptr()
+        a.dy, a.dy_b, a.dy_t, a.dh_last = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
+        a.dx, a.ddt, a.dz, a.dB, a.dC = dx.data_ptr(), ddt.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
+        a.dA, a.dskip, a.ddt_bias, a.dh0 = dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dstate)
+        nbytes = L.lib.sed_gated_scan_workspace(b, n_frames, d, n, g, 1)
+        ws = _workspace(nbytes, dev)
+        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+        _call(L.lib.sed_gated_scan_backward, a, dev, "sed_gated_scan_backward")
+        return dx, ddt, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None
+
+
+def _scan_checks(what, x, dt, A, B, Cm, D, z, dt_bias, lead):
+    d = x.shape[-1]
+    _check(what, "dt", dt, x, x.shape)
+    if not torch.is_tensor(A) or A.dim() != 2:
+        raise ValueError(f"{what}: A: a (channels, states) tensor")
+    n = A.shape[1]
+    if not 1 <= n <= 32:
+        raise ValueError(f"{what}: {n} states a channel; 1 to 32 are supported")
+    _check(what, "A", A, x, (d, n), "float")
+    if not torch.is_tensor(B) or B.dim() not in (lead + 1, lead + 2):
+        raise ValueError(f"{what}: B: {'(clips, frames, [groups,] states)' if lead == 2 else '(streams, [groups,] states)'}")
+    g = B.shape[lead] if B.dim() == lead + 2 else 1
+    if g < 1 or d % g:
+        raise ValueError(f"{what}: {d} channels do not divide into {g} groups")
+    shape = (*x.shape[:lead], g, n) if B.dim() == lead + 2 else (*x.shape[:lead], n)
+    _check(what, "B", B, x, shape)
+    _check(what, "C", Cm, x, shape)
+    if D is not None:
+        _check(what, "D", D, x, (d,), "float")
+    if z is not None:
+        _check(what, "z", z, x, x.shape)
+    if dt_bias is not None:
+        _check(what, "dt_bias", dt_bias, x, (d,), "float")
+    return g, n
+
+
+def gated_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, frames=None, reverse=False, state=None, return_state=False):
+    """The gated linear recurrence along the frames, with a gradient for every tensor but `frames`:
+
+        delta_t[d] = softplus(dt_t[d] + dt_bias[d])          (softplus=False: dt + dt_bias)
+        h_t[d,n]   = exp(delta_t[d] A[d,n]) h_{t-1}[d,n] + delta_t[d] B_t[g,n] x_t[d]
+        y_t[d]     = (sum_n C_t[g,n] h_t[d,n] + D[d] x_t[d]) * silu(z_t[d])
+
+    x, dt, z (clips, frames, channels); B, C (clips, frames, states) or (clips, frames, groups, states), channel d reading group
+    d // (channels // groups); all of one type (fp32, bf16, fp16) and of any strides.  A (channels, states), 1 to 32 states;
+    D, dt_bias (channels,): any floating type, read as fp32.
+    frames (clips,) int32 on the device: the clips' own row counts; rows behind them give zero and are not read.
+    reverse: from a clip's last own row to its first.  state (clips, channels, states) fp32: h in front of the first row walked.
+    Returns y (clips, frames, channels), and with return_state also h behind the last row walked (fp32): passing it on as the
+    next call's state continues the sequence."""
+    what = "gated_scan"
+    _check_x(what, x, 3)
+    g, n = _scan_checks(what, x, dt, A, B, C, D, z, dt_bias, 2)
+    _check_frames(what, frames, x)
+    if state is not None:
+        _check(what, "state", state, x, (x.shape[0], x.shape[2], n), torch.float32)
+        state = state.contiguous()
+    if B.dim() == 3:
+        B, C = B.unsqueeze(2), C.unsqueeze(2)
+    x, dt, z, B, C = (_rows(t) for t in (x, dt, z, B, C))
+    A, D, dt_bias = _param(A), _param(D), _param(dt_bias)
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
+        return _GatedScan.apply(x, dt, A, B, C, D, z, dt_bias, state, bool(softplus), frames, bool(reverse), bool(return_state))
+    y, last, _ = _scan_forward(x, dt, A, B, C, D, z, dt_bias, softplus, frames, reverse, state, return_state, False)
+    return (y, last) if return_state else y
+
+
+def gated_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False):
+    """One frame of gated_scan for a batch of streams: state (streams, channels, states) fp32, contiguous, is updated in place;
+    x, dt, z (streams, channels), B, C (streams, states) or (streams, groups, states).  Returns y (streams, channels).  For
+    inference: it has no gradient."""
+    what = "gated_scan_step"
+    _check_x(what, x, 2)
+    g, n = _scan_checks(what, x, dt, A, B, C, D, z, dt_bias, 1)
+    _check(what, "state", state, x, (x.shape[0], x.shape[1], n), torch.float32)
+    if not state.is_contiguous():
+        raise ValueError(f"{what}: state is updated in place and has to be contiguous")
+    _no_grad_only(what, state, x, dt, A, B, C, D, z, dt_bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.shape[0] == 0:
+        return y
+    x, dt, z, B, C = (_rows(t) for t in (x, dt, z, B, C))
+    A, D, dt_bias = _param(A), _param(D), _param(dt_bias)
+    a = L.ScanArgs()
+    a.B, a.D = x.shape
+    a.L, a.G, a.N = 1, g, n
+    a.dtype, a.softplus = _DTYPES[x.dtype], int(softplus)
+    a.x, a.dt, a.Bm, a.Cm, a.A = x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), A.data_ptr()
+    a.x_b, a.dt_b, a.Bm_b, a.Cm_b = x.stride(0), dt.stride(0), B.stride(0), C.stride(0)
+    if B.dim() == 3:
+        a.Bm_g, a.Cm_g = B.stride(1), C.stride(1)
+    if z is not None:
+        a.z, a.z_b = z.data_ptr(), z.stride(0)
+    a.skip, a.dt_bias = _ptr(D), _ptr(dt_bias)
+    a.y, a.h_last = y.data_ptr(), state.data_ptr()
+    _call(L.lib.sed_gated_scan_step, a, x.device, "sed_gated_scan_step")
+    return y
+
+
+# ---- causal convolution -------------------------------------------------------------------------------------------------
+
+
+def _conv_args(x, weight, bias, act, frames, reverse, state):
+    a = L.ConvArgs()
+    a.B, a.L, a.D = x.shape
+    a.W = weight.shape[1]
+    a.dtype, a.act, a.reverse = _DTYPES[x.dtype], act, int(reverse)
+    a.frames, a.x, a.x_b, a.x_t = _ptr(frames), x.data_ptr(), x.stride(0), x.stride(1)
+    a.weight, a.bias, a.state = weight.data_ptr(), _ptr(bias), _ptr(state)
+    return a
+
+
+def _conv_forward(x, weight, bias, act, frames, reverse, state, want_last):
+    b, n_frames, d = x.shape
+    y = torch.empty((b, n_frames, d), dtype=x.dtype, device=x.device)
+    last = torch.empty((b, weight.shape[1] - 1, d), dtype=x.dtype, device=x.device) if want_last else None
+    if b == 0 or n_frames == 0:
+        if want_last:
+            last.zero_() if state is None else last.copy_(state)
+        return y, last
+    a = _conv_args(x, weight, bias, act, frames, reverse, state)
+    a.y, a.state_out = y.data_ptr(), _ptr(last)
+    _call(L.lib.sed_causal_conv_forward, a, x.device, "sed_causal_conv_forward")
+    return y, last
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, act, frames, reverse, want_last):
+        y, last = _conv_forward(x, weight, bias, act, frames, reverse, state, want_last)
+        ctx.save_for_backward(x, weight, bias, state, frames)
+        ctx.flags = (act, reverse)
+        ctx.set_materialize_grads(False)
+        return (y, last) if want_last else y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dlast=None):
+        x, weight, bias, state, frames = ctx.saved_tensors
+        act, reverse = ctx.flags
+        b, n_frames, d = x.shape
+        dev = x.device
+        dx, dw, db, dstate = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (x, weight, bias, state))
+        if b == 0 or n_frames == 0:
+            for t in (dw, db, dstate):
+                if t is not None:
+                    t.zero_()
+            if dstate is not None and dlast is not None:
+                dstate.copy_(dlast)
+            return dx, dw, db, dstate, None, None, None, None
+        dy = torch.zeros((b, n_frames, d), dtype=x.dtype, device=dev) if dy is None else _rows(dy)
+        dlast = None if dlast is None else dlast.contiguous()
+        a = _conv_args(x, weight, bias, act, frames, reverse, state)
+        a.dy, a.dy_b, a.dy_t, a.dstate_out = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
+        a.dx, a.dw, a.db, a.dstate = dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(dstate)
+        nbytes = L.lib.sed_causal_conv_workspace(b, n_frames, d, weight.shape[1])
+        ws = _workspace(nbytes, dev)
+        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+        _call(L.lib.sed_causal_conv_backward, a, dev, "sed_causal_conv_backward")
+        return dx, dw, db, dstate, None, None, None, None
+
+
+def _conv_checks(what, x, weight, bias, activation):
+    if activation not in (None, "silu"):
+        raise ValueError(f"{what}: activation {activation!r}; None and 'silu' are supported")
+    if torch.is_tensor(weight) and weight.dim() == 3 and weight.shape[1] == 1:  # as a depthwise convolution layer holds it
+        weight = weight.squeeze(1)
+    if not torch.is_tensor(weight) or weight.dim() != 2 or not 1 <= weight.shape[1] <= 8:
+        raise ValueError(f"{what}: weight: a (channels, taps) tensor of 1 to 8 taps")
+    _check(what, "weight", weight, x, (x.shape[-1], weight.shape[1]), "float")
+    if bias is not None:
+        _check(what, "bias", bias, x, (x.shape[-1],), "float")
+    return weight
+
+
+def causal_conv(x, weight, bias=None, activation=None, frames=None, reverse=False, state=None, return_state=False):
+    """Depthwise convolution of every channel with its own taps over the frames in front, with a gradient for every tensor but
+    `frames`: y_t = act(bias + sum_k weight[:, k] x_{t - W + 1 + k}).
+
+    x (clips, frames, channels) fp32, bf16 or fp16, any strides; weight (channels, W) or (channels, 1, W), 1 to 8 taps; bias
+    (channels,); activation None or "silu".  frames: the clips' own row counts.  reverse: the window looks to later frames.
+    state (clips, W - 1, channels): the rows in front of the first row walked, oldest first (zero if None).  With return_state
+    also returns the last W - 1 rows seen, the next call's state."""
+    what = "causal_conv"
+    _check_x(what, x, 3)
+    weight = _conv_checks(what, x, weight, bias, activation)
+    _check_frames(what, frames, x)
+    if state is not None:
+        _check(what, "state", state, x, (x.shape[0], weight.shape[1] - 1, x.shape[2]))
+        state = state.contiguous()
+    x, weight, bias, act = _rows(x), _param(weight), _param(bias), _ACTIVATIONS[activation]
+    if _wants_grad(x, weight, bias, state):
+        return _CausalConv.apply(x, weight, bias, state, act, frames, bool(reverse), bool(return_state))
+    y, last = _conv_forward(x, weight, bias, act, frames, reverse, state, return_state)
+    return (y, last) if return_state else y
+
+
+def causal_conv_step(state, x, weight, bias=None, activation=None):
+    """One frame of causal_conv for a batch of streams: state (streams, W - 1, channels) of x's type, contiguous, moves up by the
+    new row in place; x (streams, channels).  Returns y (streams, channels).  For inference: it has no gradient."""
+    what = "causal_conv_step"
+    _check_x(what, x, 2)
+    weight = _conv_checks(what, x, weight, bias, activation)
+    _check(what, "state", state, x, (x.shape[0], weight.shape[1] - 1, x.shape[1]))
+    if not state.is_contiguous():
+        raise ValueError(f"{what}: state is updated in place and has to be contiguous")
+    _no_grad_only(what, state, x, weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    if x.shape[0] == 0:
+        return y
+    x, weight, bias = _rows(x), _param(weight), _param(bias)
+    a = L.ConvArgs()
+    a.B, a.D = x.shape
+    a.L, a.W = 1, weight.shape[1]
+    a.dtype, a.act = _DTYPES[x.dtype], _ACTIVATIONS[activation]
+    a.x, a.x_b, a.weight, a.bias = x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias)
+    a.y, a.state_out = y.data_ptr(), _ptr(state)
+    _call(L.lib.sed_causal_conv_step, a, x.device, "sed_causal_conv_step")
+    return y
+
+
+# ---- group norm ---------------------------------------------------------------------------------------------------------
+
+
+def _norm_args(x, shape, groups, weight, bias, act, eps, frames, mean, rstd):
+    a = L.NormArgs()
+    a.B, a.T, a.F, a.C = shape
+    a.G, a.dtype, a.act, a.eps = groups, _DTYPES[x.dtype], act, eps
+    a.frames, a.x, a.weight, a.bias = _ptr(frames), x.data_ptr(), _ptr(weight), _ptr(bias)
+    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
+    return a
+
+
+def _norm_forward(x, groups, weight, bias, eps, act, frames):
+    shape = (x.shape[0], x.shape[1], x[0, 0].numel() // x.shape[-1] if x.numel() else 1, x.shape[-1])
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = (torch.empty((shape[0], groups), dtype=torch.float32, device=x.device) for _ in range(2))
+    if x.numel():
+        a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, mean, rstd)
+        nbytes = L.lib.sed_group_norm_workspace(*shape, groups)
+        ws = _workspace(nbytes, x.device)
+        a.ws, a.ws_bytes, a.y = ws.data_ptr(), nbytes, y.data_ptr()
+        _call(L.lib.sed_group_norm_forward, a, x.device, "sed_group_norm_forward")
+    return y, mean, rstd, shape
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, groups, eps, act, frames):
+        y, mean, rstd, shape = _norm_forward(x, groups, weight, bias, eps, act, frames)
+        ctx.save_for_backward(x, weight, bias, frames, mean, rstd)
+        ctx.rest = (shape, groups, eps, act)
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias, frames, mean, rstd = ctx.saved_tensors
+        shape, groups, eps, act = ctx.rest
+        dx, dw, db = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, weight, bias))
+        if x.numel() == 0:
+            for t in (dw, db):
+                if t is not None:
+                    t.zero_()
+            return dx, dw, db, None, None, None, None
+        dy = dy.contiguous()
+        a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, mean, rstd)
+        a.dy, a.dx, a.dw, a.db = dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
+        nbytes = L.lib.sed_group_norm_workspace(*shape, groups)
+        ws = _workspace(nbytes, x.device)
+        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
+        _call(L.lib.sed_group_norm_backward, a, x.device, "sed_group_norm_backward")
+        return dx, dw, db, None, None, None, None
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation=None, frames=None):
+    """act(group norm of x) on channels-last data, with a gradient for x, weight and bias.
+
+    x (clips, frames, ..., channels) fp32, bf16 or fp16: mean and (biased) variance are taken per clip and group of
+    channels // groups neighbouring channels over the clip's own frames and all axes in between.  weight, bias (channels,), any
+    floating type, or None; activation None, "silu", "relu" or "gelu" (the exact one).  frames (clips,) int32 on the device:
+    rows behind a clip's own give zero and are not read."""
+    what = "group_norm_act"
+    if not torch.is_tensor(x) or x.dim() < 3:
+        raise ValueError(f"{what}: x: (clips, frames, ..., channels)")
+    _check_x(what, x, x.dim())
+    if activation not in _ACTIVATIONS:
+        raise ValueError(f"{what}: activation {activation!r}; None, 'silu', 'relu' and 'gelu' are supported")
+    groups, c = int(groups), x.shape[-1]
+    if groups < 1 or c % groups:
+        raise ValueError(f"{what}: {c} channels do not divide into {groups} groups")
+    if not float(eps) >= 0:
+        raise ValueError(f"{what}: eps {eps} is negative")
+    if x.shape[0] > 65535:
+        raise ValueError(f"{what}: {x.shape[0]} clips; 65535 at most")
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None:
+            _check(what, name, t, x, (c,), "float")
+    _check_frames(what, frames, x)
+    x, weight, bias, act = x.contiguous(), _param(weight), _param(bias), _ACTIVATIONS[activation]
+    if _wants_grad(x, weight, bias):
+        return _GroupNormAct.apply(x, weight, bias, groups, float(eps), act, frames)
+    return _norm_forward(x, groups, weight, bias, float(eps), act, frames)[0]
