@@ -27,10 +27,10 @@ namespace {
 
 struct ScanParams {
   sed_scan_args a;
-  int64_t L_chunk;  // frames of a chunk, a multiple of TT
-  int32_t K;        // chunks
+  int32_t nt;       // tiles of frames, ceil(L / TT)
+  int32_t four;     // N % 4 == 0 and A, h0, dh_last are aligned to 16 bytes
+  int32_t K;        // chunks: chunk k has the tiles from k nt / K on
   int32_t tiles;    // channel tiles of a group
-  int32_t saved_n;  // ceil(L / TT)
   float* chunk_h;   // [B][K][NP][D]  end states from zero, then the states in front of the chunks
   float* chunk_s;   // [B][K][D]      sums of delta
   float* part_bc;   // [B][G * tiles][L][2 * NP]  dB, dC of one wave's channels
@@ -44,7 +44,8 @@ struct Geo {
   static constexpr int NP = NS * SPLIT;       // states, padded
   static constexpr int J = 64 / SPLIT;        // lanes along channels
   static constexpr int CW = 4 * J;            // channels of a wave
-  static constexpr int TT = NS == 8 ? 4 : 8;  // frames of a tile: TT * 4 * NS = 128 registers hold a tile's states (fewer with NS < 4)
+  static constexpr int TT = SPLIT >= 4 ? 8 : 4;  // frames of a tile
+  static constexpr int TB = 4;                // frames whose states the gradient holds at a time: 16 NS <= 64 registers
   static constexpr int R = TT / SPLIT;        // rows a lane loads
   static constexpr int PB = (TT * NP + 63) / 64;
   static_assert(R * SPLIT == TT, "");
@@ -53,82 +54,121 @@ struct Geo {
 // Where a wave works.
 struct Where {
   int b, chunk, g, s, j;
-  int64_t own;       // frames of the clip's own
-  int64_t c0;        // first channel of the lane
-  int nc;            // channels of the lane (0..4)
-  int tile;          // over all groups
+  int own;         // frames of the clip's own
+  int begin, end;  // the chunk's frames of the clip's own
+  int c0, cl;      // first channel of the lane; the same, or the group's first where the lane has none
+  int nc;          // channels of the lane (0..4)
+  int tile;        // over all groups
+  int flip;        // TT - 1 where the walk goes to earlier rows
 };
+
+template <class G>
+__device__ __forceinline__ int chunk_begin(const ScanParams& p, int k) { return (int)((int64_t)k * p.nt / p.K) * G::TT; }
 
 template <class G>
 __device__ __forceinline__ Where where(const ScanParams& p) {
   Where w;
   const sed_scan_args& a = p.a;
-  const int all = p.tiles * a.G;
+  const unsigned all = p.tiles * a.G;
   unsigned i = blockIdx.x;
   w.tile = i % all;
   i /= all;
   w.chunk = i % p.K;
   w.b = i / p.K;
   w.g = w.tile / p.tiles;
+  w.flip = a.reverse ? G::TT - 1 : 0;
   w.s = threadIdx.x / G::J;
   w.j = threadIdx.x % G::J;
-  const int64_t cg = a.D / a.G, in = (int64_t)(w.tile % p.tiles) * G::CW + 4 * w.j;
+  const int cg = (int)a.D / a.G, in = (w.tile % p.tiles) * G::CW + 4 * w.j;
   w.c0 = w.g * cg + in;
-  w.nc = (int)std::max<int64_t>(0, std::min<int64_t>(4, cg - in));
-  w.own = a.L;
-  if (a.frames) w.own = std::max<int64_t>(0, std::min<int64_t>(a.L, a.frames[w.b]));
+  w.nc = std::max(0, std::min(4, cg - in));
+  w.cl = w.nc ? w.c0 : w.g * cg;
+  w.own = (int)a.L;
+  if (a.frames) w.own = std::max(0, std::min((int)a.L, a.frames[w.b]));
+  w.begin = chunk_begin<G>(p, w.chunk);
+  w.end = std::min(chunk_begin<G>(p, w.chunk + 1), w.own);
   return w;
 }
 
 // Row of the clip that comes i-th: behind the clip's own rows every row is itself.
-__device__ __forceinline__ int64_t row_of(const ScanParams& p, int64_t own, int64_t i) {
-  return p.a.reverse && i < own ? own - 1 - i : i;
-}
+__device__ __forceinline__ int row_of(const ScanParams& p, int own, int i) { return p.a.reverse && i < own ? own - 1 - i : i; }
 
-// Rows of a tile as a lane loads them: 4 channels of rows i0 + r * SPLIT + s.
+template <class T>
+using T4 = T __attribute__((ext_vector_type(4)));
+
+// Rows of a tensor in the order of the walk.  An address is a uniform base that moves with the tile (a scalar) and 32 bits of
+// the lane's own: row i0 + t lies t rows behind the tile's first, or TT - 1 - t = t ^ (TT - 1) behind the tile's last where the
+// walk goes to earlier rows, so the lane's part is never negative.  Rows are at most 2^26 elements apart (checked on the host).
+template <class G, class T>
+struct Rows {
+  const char* base;  // tile of i0 = 0
+  int64_t step;      // bytes from one frame of the walk to the next
+  uint32_t apart;    // bytes between rows
+  __device__ __forceinline__ Rows(const ScanParams& q, const Where& w, const void* p, int64_t sb, int64_t st) {
+    const int64_t bytes = st * (int64_t)sizeof(T);
+    apart = (uint32_t)bytes;
+    step = q.a.reverse ? -bytes : bytes;
+    base = static_cast<const char*>(p) + w.b * sb * (int64_t)sizeof(T) + (q.a.reverse ? (int64_t)(w.own - G::TT) * bytes : 0);
+  }
+  __device__ __forceinline__ const char* tile(int i0) const { return base + i0 * step; }
+  __device__ __forceinline__ uint32_t lane(const Where& w, uint32_t t, uint32_t c) const { return (t ^ w.flip) * apart + c * (uint32_t)sizeof(T); }
+};
+
+// 4 channels of the rows i0 + r * SPLIT + s of a tile.  Every load is in bounds, so none is conditional: rows behind the clip's
+// own read its last one, lanes and channels without a channel read one that exists; what they read is replaced where it is used.
 template <class G, class T, bool VEC>
-__device__ __forceinline__ void load_rows(const ScanParams& p, const Where& w, const void* base, int64_t sb, int64_t st, int64_t i0,
-                                          float (&out)[G::R][4]) {
+__device__ __forceinline__ void load_rows(const Rows<G, T>& rows, const Where& w, int i0, T4<T> (&out)[G::R]) {
+  const char* at = rows.tile(i0);
 #pragma unroll
   for (int r = 0; r < G::R; ++r) {
-    const int64_t i = i0 + r * (64 / G::J) + w.s;
-    const bool in = i < w.own;
-    const T* q = static_cast<const T*>(base) + w.b * sb + (in ? row_of(p, w.own, i) : 0) * st + w.c0;
-    load_n<T, 4, VEC>(q, in ? w.nc : 0, out[r]);
+    const T* q = reinterpret_cast<const T*>(at + rows.lane(w, std::min(r * (64 / G::J) + w.s, w.own - 1 - i0), w.cl));
+    if constexpr (VEC) {
+      out[r] = *reinterpret_cast<const T4<T>*>(q);
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) out[r][c] = q[c < w.nc ? c : 0];
+    }
   }
 }
 
-// B or C of a tile: element e = lane + 64 i is state e % NP of row e / NP.
+// One of the same rows of an output; rows behind the clip's own are not written.
+template <class G, class T, bool VEC>
+__device__ __forceinline__ void store_row(const Rows<G, T>& rows, const Where& w, int i0, int r, const float (&v)[4]) {
+  const int t = r * (64 / G::J) + w.s;
+  store_n<T, 4, VEC>(reinterpret_cast<T*>(const_cast<char*>(rows.tile(i0)) + rows.lane(w, t, w.c0)), i0 + t < w.own ? w.nc : 0, v);
+}
+
+// B or C of a tile: element e = lane + 64 k is state e % NP of row e / NP.
 template <class G, class T>
-__device__ __forceinline__ void load_bc(const ScanParams& p, const Where& w, const void* base, int64_t sb, int64_t st, int64_t sg, int64_t i0,
-                                        float (&out)[G::PB]) {
+__device__ __forceinline__ void load_states(const Rows<G, T>& rows, const ScanParams& q, const Where& w, int i0, T (&out)[G::PB]) {
+  const char* at = rows.tile(i0);
+  const int last = std::min(w.own - 1 - i0, G::TT - 1);
 #pragma unroll
-  for (int q = 0; q < G::PB; ++q) {
-    const int e = threadIdx.x + 64 * q, n = e % G::NP;
-    const int64_t i = i0 + e / G::NP;
-    const bool in = e < G::TT * G::NP && n < p.a.N && i < w.own;
-    const T* at = static_cast<const T*>(base) + w.b * sb + (in ? row_of(p, w.own, i) : 0) * st + w.g * sg + (in ? n : 0);
-    out[q] = in ? (float)*at : 0.0f;
+  for (int k = 0; k < G::PB; ++k) {
+    const int e = threadIdx.x + 64 * k, n = e % G::NP, t = e / G::NP;
+    out[k] = *reinterpret_cast<const T*>(at + rows.lane(w, std::min(t, last), n < q.a.N ? n : 0));
   }
 }
-template <class G>
-__device__ __forceinline__ void put_bc(const float (&v)[G::PB], float* to) {
+// Into LDS; the padding states are zero, and so are rows behind the clip's own.
+template <class G, class T>
+__device__ __forceinline__ void put_states(const ScanParams& q, const Where& w, int i0, const T (&v)[G::PB], float* to) {
 #pragma unroll
-  for (int q = 0; q < G::PB; ++q) {
-    const int e = threadIdx.x + 64 * q;
-    if (e < G::TT * G::NP) to[e] = v[q];
+  for (int k = 0; k < G::PB; ++k) {
+    const int e = threadIdx.x + 64 * k, n = e % G::NP, t = e / G::NP;
+    if (G::TT * G::NP % 64 == 0 || e < G::TT * G::NP) to[e] = n < q.a.N && i0 + t < w.own ? (float)v[k] : 0.0f;
   }
 }
 
 template <int NS>
 __device__ __forceinline__ void get_states(const float* from, float (&v)[NS]) {
-  if constexpr (NS % 4 == 0) {
+  if constexpr (NS == 4) {
+    const f32x4 t = *reinterpret_cast<const f32x4*>(from);
 #pragma unroll
-    for (int q = 0; q < NS / 4; ++q) {
-      const f32x4 t = reinterpret_cast<const f32x4*>(from)[q];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) v[4 * q + i] = t[i];
-    }
+    for (int i = 0; i < 4; ++i) v[i] = t[i];
+  } else if constexpr (NS == 2) {
+    const f32x2 t = *reinterpret_cast<const f32x2*>(from);
+    v[0] = t[0];
+    v[1] = t[1];
   } else {
 #pragma unroll
     for (int i = 0; i < NS; ++i) v[i] = from[i];
@@ -144,11 +184,27 @@ __device__ __forceinline__ void put4(const float (&v)[4], float* to) {
   *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
-// Sums of v[4] over the SPLIT lanes that share a channel; afterwards lane s of a channel group holds, for SPLIT = 4, channel s
-// (out[0]); for SPLIT = 2, channels s and 2 + s... as `put_sums` writes them.
+// What a frame of a tile needs out of LDS.
+template <int NS>
+struct Step {
+  float dl[4], dx[4], B[NS], C[NS];
+  template <class G, bool X, bool WITH_C>
+  __device__ __forceinline__ void get(const Where& w, int t, const float* s_dl, const float* s_dx, const float* s_B, const float* s_C) {
+    get4(s_dl + t * G::CW + 4 * w.j, dl);
+    if (X) get4(s_dx + t * G::CW + 4 * w.j, dx);
+    if (X) get_states<NS>(s_B + t * G::NP + w.s * NS, B);
+    if (WITH_C) get_states<NS>(s_C + t * G::NP + w.s * NS, C);
+  }
+};
+
+// Writes the sums of v[4] over the SPLIT lanes that share a channel to the lane group's 4 places of a row.
 template <int SPLIT, int CW>
 __device__ __forceinline__ void put_sums(const float (&v)[4], int s, int j, float* row) {
-  if constexpr (SPLIT == 4) {
+  if constexpr (SPLIT == 8) {
+    // as below, and the two halves of a row of 16 lanes hold the same channel
+    const float v4 = fold16(fold32(v[0], v[2]), fold32(v[1], v[3]));
+    row[4 * j + s / 2] = v4 + dpp<kRor8>(v4);
+  } else if constexpr (SPLIT == 4) {
     // rows of 16 lanes s = 0..3: halves first (channels 0 | 2 and 1 | 3), then neighbouring rows
     const float lo = fold32(v[0], v[2]), hi = fold32(v[1], v[3]);
     row[4 * j + s] = fold16(lo, hi);
@@ -160,81 +216,160 @@ __device__ __forceinline__ void put_sums(const float (&v)[4], int s, int j, floa
   }
 }
 
-// states of a lane from / to a [NP][D] plane
-template <class G, int NS, bool VEC>
+__device__ __forceinline__ void per_channel(const float* from, const Where& w, float (&v)[4]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = from ? from[w.cl + (c < w.nc ? c : 0)] : 0.0f;
+}
+
+// states of a lane from / to a [NP][D] plane: a uniform base per state and 32 bits of the lane's own (32 D floats at most)
+template <int NS, bool VEC>
 __device__ __forceinline__ void load_plane(const float* plane, int64_t D, const Where& w, float (&h)[4][NS]) {
+  const uint32_t off = (uint32_t)(w.s * NS * (int)D + w.cl) * 4u;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
-    float v[4];
-    load_n<float, 4, VEC>(plane + (int64_t)(w.s * NS + n) * D + w.c0, w.nc, v);
+    const float* q = reinterpret_cast<const float*>(reinterpret_cast<const char*>(plane + n * D) + off);
+    if constexpr (VEC) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(q);
 #pragma unroll
-    for (int c = 0; c < 4; ++c) h[c][n] = v[c];
+      for (int c = 0; c < 4; ++c) h[c][n] = v[c];
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) h[c][n] = q[c < w.nc ? c : 0];
+    }
   }
 }
-template <class G, int NS, bool VEC>
+template <int NS, bool VEC>
 __device__ __forceinline__ void store_plane(float* plane, int64_t D, const Where& w, const float (&h)[4][NS]) {
+  const uint32_t off = (uint32_t)(w.s * NS * (int)D + w.c0) * 4u;
 #pragma unroll
   for (int n = 0; n < NS; ++n) {
     float v[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) v[c] = h[c][n];
-    store_n<float, 4, VEC>(plane + (int64_t)(w.s * NS + n) * D + w.c0, w.nc, v);
+    store_n<float, 4, VEC>(reinterpret_cast<float*>(reinterpret_cast<char*>(plane + n * D) + off), w.nc, v);
   }
 }
-// states of a lane from / to the caller's [D][N]
-template <class G, int NS>
-__device__ __forceinline__ void load_dn(const float* base, int N, const Where& w, float (&h)[4][NS]) {
+// states of a lane from / to the caller's [D][N]; padding states are zero, a lane without a channel reads another's
+template <int NS>
+__device__ __forceinline__ void load_dn(const ScanParams& p, const float* base, const Where& w, float (&h)[4][NS]) {
+  const int N = p.a.N;
+  if (NS == 4 && p.four) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(base + (int64_t)(w.cl + (c < w.nc ? c : 0)) * N + std::min(w.s * NS, N - 4));
+#pragma unroll
+      for (int n = 0; n < NS; ++n) h[c][n] = w.s * NS < N ? v[n % 4] : 0.0f;
+    }
+    return;
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       const int k = w.s * NS + n;
-      h[c][n] = c < w.nc && k < N ? base[(w.c0 + c) * N + k] : 0.0f;
+      const float v = base[(int64_t)(w.cl + (c < w.nc ? c : 0)) * N + std::min(k, N - 1)];
+      h[c][n] = k < N ? v : 0.0f;
     }
 }
-template <class G, int NS>
+template <int NS>
 __device__ __forceinline__ void store_dn(float* base, int N, const Where& w, const float (&h)[4][NS]) {
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int n = 0; n < NS; ++n) {
       const int k = w.s * NS + n;
-      if (c < w.nc && k < N) base[(w.c0 + c) * N + k] = h[c][n];
+      if (c < w.nc && k < N) base[(int64_t)(w.c0 + c) * N + k] = h[c][n];
     }
 }
 
-__device__ __forceinline__ float delta_of(const ScanParams& p, float v) { return p.a.softplus ? softplus(v) : v; }
-
-__device__ __forceinline__ void per_channel(const float* from, const Where& w, float (&v)[4]) {
+// delta of a tile's rows; zero where the row or the channel is none (exp(0) = 1 leaves the state as it is)
+template <class G, class T, bool VEC>
+__device__ __forceinline__ void deltas(const ScanParams& p, const Where& w, int i0, const T4<T> (&dt)[G::R], const float (&bias)[4], float (&dl)[G::R][4]) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) v[c] = from && c < w.nc ? from[w.c0 + c] : 0.0f;
+  for (int r = 0; r < G::R; ++r)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) dl[r][c] = (float)dt[r][c] + bias[c];
+  if (p.a.softplus) {
+#pragma unroll
+    for (int r = 0; r < G::R; ++r)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) dl[r][c] = softplus(dl[r][c]);
+  }
+#pragma unroll
+  for (int r = 0; r < G::R; ++r) {
+    const bool in = i0 + r * (64 / G::J) + w.s < w.own;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) dl[r][c] = in && (VEC ? w.nc > 0 : c < w.nc) ? dl[r][c] : 0.0f;
+  }
 }
+// v where the row and the channel exist (a row behind the clip's own can hold anything)
+template <class G, bool VEC>
+__device__ __forceinline__ void only_own(const Where& w, int i0, int r, float (&v)[4]) {
+  const bool in = i0 + r * (64 / G::J) + w.s < w.own;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) v[c] = in && (VEC ? w.nc > 0 : c < w.nc) ? v[c] : 0.0f;
+}
+
+// Zero rows of the clip behind its own, this chunk's share of them.
+template <class G, class T, bool VEC>
+__device__ __forceinline__ void clear_rows(const ScanParams& p, const Where& w, void* base) {
+  const float zero[4] = {0, 0, 0, 0};
+  const int stop = std::min(chunk_begin<G>(p, w.chunk + 1), (int)p.a.L);
+  for (int i = std::max(w.begin, w.own) + w.s; i < stop; i += 64 / G::J)
+    store_n<T, 4, VEC>(static_cast<T*>(base) + ((int64_t)w.b * p.a.L + i) * p.a.D + w.c0, w.nc, zero);
+}
+
 
 // ---- forward ------------------------------------------------------------------------------------------------------------
 
 // ENDS: only the chunk's end state from zero and its sum of delta.  Otherwise the chunk's outputs.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64) scan_forward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
   const Where w = where<G>(p);
   __shared__ __attribute__((aligned(16))) float s_dl[G::TT][G::CW], s_dx[G::TT][G::CW], s_y[ENDS ? 1 : G::TT][G::CW];
   __shared__ __attribute__((aligned(16))) float s_B[G::TT][G::NP], s_C[G::TT][G::NP];
-  const int64_t begin = w.chunk * p.L_chunk, end = std::min<int64_t>(begin + p.L_chunk, a.L);
-  if (ENDS && (w.chunk == p.K - 1 || begin >= w.own)) return;  // chunk_join_kernel reads no such chunk
+  if (ENDS && (w.chunk == p.K - 1 || w.begin >= w.own)) return;  // chunk_join_kernel reads no such chunk
+  if (!ENDS) {
+    clear_rows<G, T, VEC>(p, w, a.y);
+    if (w.begin >= w.own) {
+      if (a.h_last && w.own == 0 && w.chunk == 0) {
+        float h[4][NS] = {};
+        if (a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
+        store_dn<NS>(a.h_last + (int64_t)w.b * a.D * a.N, a.N, w, h);
+      }
+      return;
+    }
+  }
+
+  const Rows<G, T> rx(p, w, a.x, a.x_b, a.x_t), rdt(p, w, a.dt, a.dt_b, a.dt_t), rz(p, w, a.z, a.z_b, a.z_t), ry(p, w, a.y, a.L * a.D, a.D);
+  const Rows<G, T> rB(p, w, static_cast<const T*>(a.Bm) + w.g * a.Bm_g, a.Bm_b, a.Bm_t), rC(p, w, static_cast<const T*>(a.Cm) + w.g * a.Cm_g, a.Cm_b, a.Cm_t);
+  T4<T> x[G::R], dt[G::R], z[G::R];
+  T bv[G::PB], cv[G::PB];
+  const auto fetch = [&](int i0) {
+    load_rows<G, T, VEC>(rx, w, i0, x);
+    load_rows<G, T, VEC>(rdt, w, i0, dt);
+    load_states<G, T>(rB, p, w, i0, bv);
+    if (!ENDS) {
+      if (a.z) load_rows<G, T, VEC>(rz, w, i0, z);
+      load_states<G, T>(rC, p, w, i0, cv);
+    }
+  };
+  fetch(w.begin);
 
   float A2[4][NS], h[4][NS], bias[4], skip[4], sum[4] = {0, 0, 0, 0};
-  load_dn<G, NS>(a.A, a.N, w, A2);
+  load_dn<NS>(p, a.A, w, A2);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
     for (int n = 0; n < NS; ++n) A2[c][n] *= kLog2e;
   per_channel(a.dt_bias, w, bias);
   per_channel(a.skip, w, skip);
-  if (!ENDS && p.K > 1 && begin < w.own) {
-    load_plane<G, NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
+  if (!ENDS && p.K > 1) {
+    load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
   } else if (!ENDS && a.h0) {
-    load_dn<G, NS>(a.h0 + (int64_t)w.b * a.D * a.N, a.N, w, h);
+    load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
@@ -242,82 +377,68 @@ __global__ void __launch_bounds__(64) scan_forward_kernel(const ScanParams p) {
       for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
   }
 
-  float x[G::R][4], dt[G::R][4], z[G::R][4], bv[G::PB], cv[G::PB];
-  const auto fetch = [&](int64_t i0) {
-    load_rows<G, T, VEC>(p, w, a.x, a.x_b, a.x_t, i0, x);
-    load_rows<G, T, VEC>(p, w, a.dt, a.dt_b, a.dt_t, i0, dt);
-    load_bc<G, T>(p, w, a.Bm, a.Bm_b, a.Bm_t, a.Bm_g, i0, bv);
-    if (!ENDS) {
-      if (a.z) load_rows<G, T, VEC>(p, w, a.z, a.z_b, a.z_t, i0, z);
-      load_bc<G, T>(p, w, a.Cm, a.Cm_b, a.Cm_t, a.Cm_g, i0, cv);
-    }
-  };
-  fetch(begin);
-  for (int64_t i0 = begin; i0 < end; i0 += G::TT) {
-    const bool live = i0 < w.own;
-    float xs[G::R][4], zs[G::R][4];
-    if (live) {
+  for (int i0 = w.begin; i0 < w.end; i0 += G::TT) {
+    T4<T> xs[G::R], zs[G::R];
+    float dl[G::R][4];
+    deltas<G, T, VEC>(p, w, i0, dt, bias, dl);
 #pragma unroll
-      for (int r = 0; r < G::R; ++r) {
-        const bool in = i0 + r * SPLIT + w.s < w.own;
-        float dl[4], dx[4];
+    for (int r = 0; r < G::R; ++r) {
+      float dx[4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          dl[c] = in ? delta_of(p, dt[r][c] + bias[c]) : 0.0f;
-          dx[c] = in ? dl[c] * x[r][c] : 0.0f;
-          if (ENDS) sum[c] += dl[c];
-          xs[r][c] = x[r][c];
-          zs[r][c] = z[r][c];
-        }
-        put4(dl, &s_dl[r * SPLIT + w.s][4 * w.j]);
-        put4(dx, &s_dx[r * SPLIT + w.s][4 * w.j]);
+      for (int c = 0; c < 4; ++c) {
+        dx[c] = dl[r][c] * (float)x[r][c];
+        if (ENDS) sum[c] += dl[r][c];
       }
-      put_bc<G>(bv, &s_B[0][0]);
-      if (!ENDS) put_bc<G>(cv, &s_C[0][0]);
-      if (!ENDS && a.saved) store_plane<G, NS, VEC>(a.saved + ((int64_t)w.b * p.saved_n + i0 / G::TT) * G::NP * a.D, a.D, w, h);
-      if (i0 + G::TT < end) fetch(i0 + G::TT);
-      __syncthreads();
-#pragma unroll
-      for (int t = 0; t < G::TT; ++t) {
-        float dl[4], dx[4], B[NS], C[NS], y[4];
-        get4(&s_dl[t][4 * w.j], dl);
-        get4(&s_dx[t][4 * w.j], dx);
-        get_states<NS>(&s_B[t][w.s * NS], B);
-        if (!ENDS) get_states<NS>(&s_C[t][w.s * NS], C);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          y[c] = 0.0f;
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            h[c][n] = fmaf(exp2_hw(dl[c] * A2[c][n]), h[c][n], dx[c] * B[n]);
-            if (!ENDS) y[c] = fmaf(C[n], h[c][n], y[c]);
-          }
-        }
-        if (!ENDS) put_sums<SPLIT, G::CW>(y, w.s, w.j, &s_y[t][0]);
-      }
-      __syncthreads();
+      only_own<G, VEC>(w, i0, r, dx);
+      put4(dl[r], &s_dl[r * SPLIT + w.s][4 * w.j]);
+      put4(dx, &s_dx[r * SPLIT + w.s][4 * w.j]);
+      xs[r] = x[r];
+      zs[r] = z[r];
     }
+    put_states<G, T>(p, w, i0, bv, &s_B[0][0]);
+    if (!ENDS) put_states<G, T>(p, w, i0, cv, &s_C[0][0]);
+    if (i0 + G::TT < w.end) fetch(i0 + G::TT);
+    if (!ENDS && a.saved) store_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.nt + i0 / G::TT) * G::NP * a.D, a.D, w, h);
+    __syncthreads();
+// a frame's values are read while the frame in front of it is worked on
+    Step<NS> f[2];
+    f[0].template get<G, true, !ENDS>(w, 0, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+#pragma unroll
+    for (int t = 0; t < G::TT; ++t) {
+      const Step<NS>& q = f[t % 2];
+      if (t + 1 < G::TT) f[(t + 1) % 2].template get<G, true, !ENDS>(w, t + 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+      float y[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        y[c] = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          h[c][n] = fmaf(exp2_hw(q.dl[c] * A2[c][n]), h[c][n], q.dx[c] * q.B[n]);
+          if (!ENDS) y[c] = fmaf(q.C[n], h[c][n], y[c]);
+        }
+      }
+      if (!ENDS) put_sums<SPLIT, G::CW>(y, w.s, w.j, &s_y[t][0]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    __syncthreads();
     if (!ENDS) {
 #pragma unroll
       for (int r = 0; r < G::R; ++r) {
-        const int64_t i = i0 + r * SPLIT + w.s;
-        float y[4] = {0, 0, 0, 0};
-        if (i < w.own) {
-          get4(&s_y[r * SPLIT + w.s][4 * w.j], y);
+        float y[4];
+        get4(&s_y[r * SPLIT + w.s][4 * w.j], y);
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            y[c] = fmaf(skip[c], xs[r][c], y[c]);
-            if (a.z) y[c] *= zs[r][c] * sigmoid(zs[r][c]);
-          }
+        for (int c = 0; c < 4; ++c) y[c] = fmaf(skip[c], (float)xs[r][c], y[c]);
+        if (a.z) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) y[c] *= (float)zs[r][c] * sigmoid((float)zs[r][c]);
         }
-        if (i < end)
-          store_n<T, 4, VEC>(static_cast<T*>(a.y) + ((int64_t)w.b * a.L + row_of(p, w.own, i)) * a.D + w.c0, w.nc, y);
+        store_row<G, T, VEC>(ry, w, i0, r, y);
       }
       __syncthreads();
     }
   }
   if (ENDS) {
-    store_plane<G, NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
+    store_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
     // every lane of a channel summed its own rows
     __syncthreads();
     put_sums<SPLIT, G::CW>(sum, w.s, w.j, &s_dl[0][0]);
@@ -327,48 +448,73 @@ __global__ void __launch_bounds__(64) scan_forward_kernel(const ScanParams p) {
       get4(&s_dl[0][4 * w.j], v);
       store_n<float, 4, VEC>(p.chunk_s + ((int64_t)w.b * p.K + w.chunk) * a.D + w.c0, w.nc, v);
     }
-  } else if (a.h_last && (w.own > 0 ? begin < w.own && w.own <= begin + p.L_chunk : w.chunk == 0)) {
-    store_dn<G, NS>(a.h_last + (int64_t)w.b * a.D * a.N, a.N, w, h);
+  } else if (a.h_last && w.end == w.own) {
+    store_dn<NS>(a.h_last + (int64_t)w.b * a.D * a.N, a.N, w, h);
   }
 }
 
-// The states in front of the chunks, over the chunks in order (BACK: the gradients behind them, from the last).  One thread
-// per channel and state.  In: every chunk's end state from zero; out, in its place: the state it starts from.
-template <bool BACK>
-__global__ void __launch_bounds__(256) chunk_join_kernel(const ScanParams p, int NP) {
+// The states in front of the chunks, over the chunks in order (BACK: the gradients behind them, from the last).
+// In: every chunk's end state from zero; out, in its place: the state it starts from.  A block has 64 / SEG (channel, state)
+// pairs next to each other in memory and SEG lanes for each, which take a run of chunks: first the run's own end and sum, then
+// the runs in order (LDS), then the run again from its start, so that a long clip's chunks are not one long chain of loads.
+template <class G, bool BACK, int SEG>
+__global__ void __launch_bounds__(256) chunk_join_kernel(const ScanParams p) {
   const sed_scan_args& a = p.a;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.B * NP * a.D) return;
-  const int64_t d = i % a.D, n = i / a.D % NP, b = i / a.D / NP;
-  int64_t own = a.L;
-  if (a.frames) own = std::max<int64_t>(0, std::min<int64_t>(a.L, a.frames[b]));
-  const int k_own = (int)((own + p.L_chunk - 1) / p.L_chunk);
+  constexpr int NP = G::NP, W = 256 / SEG;
+  __shared__ float s_h[SEG][W], s_s[SEG][W];
+  const int seg = threadIdx.x / W, lane = threadIdx.x % W;
+  const int64_t i = (int64_t)blockIdx.x * W + lane;
+  const bool live = i < a.B * NP * a.D;
+  const int64_t d = live ? i % a.D : 0, n = live ? i / a.D % NP : 0, b = live ? i / a.D / NP : 0;
+  int own = (int)a.L;
+  if (a.frames) own = std::max(0, std::min((int)a.L, a.frames[b]));
+  int k_own = 0;  // chunks with frames of the clip's own
+  if (own > 0) {
+    k_own = (int)((int64_t)((own - 1) / G::TT) * p.K / p.nt);
+    while (k_own < p.K && chunk_begin<G>(p, k_own) < own) ++k_own;
+  }
   const bool real = n < a.N;
   const float A2 = real ? a.A[d * a.N + n] * kLog2e : 0.0f;
   const float* first = BACK ? a.dh_last : a.h0;
-  float h = first && real ? first[(b * a.D + d) * a.N + n] : 0.0f;
-  float* hp = p.chunk_h + ((int64_t)b * p.K * NP + n) * a.D + d;
-  const float* sp = p.chunk_s + (int64_t)b * p.K * a.D + d;
+  float* hp = p.chunk_h + (b * p.K * NP + n) * a.D + d;
+  const float* sp = p.chunk_s + b * p.K * a.D + d;
+  const int per = (k_own + SEG - 1) / SEG, q0 = seg * per, q1 = live ? std::min(q0 + per, k_own) : 0;
+  const auto at = [&](int q) { return (int64_t)(BACK ? k_own - 1 - q : q); };
+  // the last chunk of the walk hands nothing on
+  if (SEG > 1) {
+    float h = 0.0f, s = 0.0f;
 #pragma unroll 4
-  for (int q = 0; q < k_own; ++q) {
-    const int k = BACK ? k_own - 1 - q : q;
-    const float end = q < k_own - 1 ? hp[(int64_t)k * NP * a.D] : 0.0f, s = q < k_own - 1 ? sp[(int64_t)k * a.D] : 0.0f;
-    hp[(int64_t)k * NP * a.D] = h;
-    h = fmaf(exp2_hw(A2 * s), h, end);
+    for (int q = q0; q < std::min(q1, k_own - 1); ++q) {
+      const float sk = sp[at(q) * a.D];
+      h = fmaf(exp2_hw(A2 * sk), h, hp[at(q) * NP * a.D]);
+      s += sk;
+    }
+    s_h[seg][lane] = h;
+    s_s[seg][lane] = s;
+    __syncthreads();
+  }
+  float h = first && real && live ? first[(b * a.D + d) * a.N + n] : 0.0f;
+  for (int k = 0; k < seg; ++k) h = fmaf(exp2_hw(A2 * s_s[k][lane]), h, s_h[k][lane]);
+#pragma unroll 4
+  for (int q = q0; q < q1; ++q) {
+    const bool more = q < k_own - 1;
+    const float end = more ? hp[at(q) * NP * a.D] : 0.0f, sk = more ? sp[at(q) * a.D] : 0.0f;
+    hp[at(q) * NP * a.D] = h;
+    h = fmaf(exp2_hw(A2 * sk), h, end);
   }
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------
 
-// 2 NS values v over the J lanes of a channel row; afterwards `value` is the sum of v[index] in the lanes where `write` holds.
+// Sums of NV values over the J lanes that share states: returned in lane j is the sum of v[sum_index(j)].
 template <int NV, int J>
-__device__ __forceinline__ void sum_lanes(float (&v)[NV], int j, float& value, int& index, bool& write) {
+__device__ __forceinline__ float sum_lanes(float (&v)[NV], int j) {
   int n = NV;
-  index = 0;
-  write = true;
 #pragma unroll
   for (int bit = J / 2; bit >= 1; bit /= 2) {
-    const bool up = j & bit;
+    const auto other = [&](float x) {
+      return bit == 8 ? dpp<kRor8>(x) : bit == 4 ? dpp<kHalfMirror>(x) : bit == 2 ? dpp<kXor2>(x) : dpp<kXor1>(x);
+    };
     if (n > 1) {
       n /= 2;
 #pragma unroll
@@ -377,41 +523,76 @@ __device__ __forceinline__ void sum_lanes(float (&v)[NV], int j, float& value, i
           if (bit == 32) v[i] = fold32(v[i], v[i + n]);
           if (bit == 16) v[i] = fold16(v[i], v[i + n]);
           if (bit < 16) {
-            const float lo = bit == 8 ? v[i] + dpp<kRor8>(v[i]) : bit == 4 ? v[i] + dpp<kHalfMirror>(v[i]) : bit == 2 ? v[i] + dpp<kXor2>(v[i]) : v[i] + dpp<kXor1>(v[i]);
-            const float hi = bit == 8 ? v[i + n] + dpp<kRor8>(v[i + n]) : bit == 4 ? v[i + n] + dpp<kHalfMirror>(v[i + n])
-                             : bit == 2 ? v[i + n] + dpp<kXor2>(v[i + n]) : v[i + n] + dpp<kXor1>(v[i + n]);
-            v[i] = up ? hi : lo;
+            const float lo = v[i] + other(v[i]), hi = v[i + n] + other(v[i + n]);
+            v[i] = j & bit ? hi : lo;
           }
         }
-      if (up) index += n;
     } else {
-      if (bit == 32) v[0] = fold32(v[0], v[0]);
-      if (bit == 16) v[0] = fold16(v[0], v[0]);
-      if (bit == 8) v[0] += dpp<kRor8>(v[0]);
-      if (bit == 4) v[0] += dpp<kHalfMirror>(v[0]);
-      if (bit == 2) v[0] += dpp<kXor2>(v[0]);
-      if (bit == 1) v[0] += dpp<kXor1>(v[0]);
-      write = write && !up;
+      v[0] = bit == 32 ? fold32(v[0], v[0]) : bit == 16 ? fold16(v[0], v[0]) : v[0] + other(v[0]);
     }
   }
-  value = v[0];
+  return v[0];
+}
+// The value lane j holds, or -1 where a lane in front of it holds the same.
+template <int NV, int J>
+__device__ __forceinline__ int sum_index(int j) {
+  int n = NV, index = 0;
+  bool first = true;
+#pragma unroll
+  for (int bit = J / 2; bit >= 1; bit /= 2) {
+    if (n > 1) {
+      n /= 2;
+      if (j & bit) index += n;
+    } else if (j & bit) {
+      first = false;
+    }
+  }
+  return first ? index : -1;
 }
 
 // ENDS: only the gradient that reaches the frame in front of the chunk from the chunk's own outputs, and the sum of delta.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64) scan_backward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
   const Where w = where<G>(p);
-  constexpr int TX = ENDS ? 1 : G::TT;
-  __shared__ __attribute__((aligned(16))) float s_dl[G::TT][G::CW], s_gy[G::TT][G::CW], s_dx[TX][G::CW];
-  __shared__ __attribute__((aligned(16))) float s_y[TX][G::CW], s_1[TX][G::CW], s_2[TX][G::CW];
+  constexpr int TX = ENDS ? 1 : G::TT, TB = G::TB;
+  // a row's gy and dx make room for the sums S2 and S1 that its frame leaves behind
+  __shared__ __attribute__((aligned(16))) float s_dl[G::TT][G::CW], s_gy[G::TT][G::CW], s_dx[TX][G::CW], s_y[TX][G::CW];
   __shared__ __attribute__((aligned(16))) float s_B[G::TT][G::NP], s_C[G::TT][G::NP];
-  const int64_t begin = w.chunk * p.L_chunk, stop = std::min<int64_t>(begin + p.L_chunk, a.L), end = std::min<int64_t>(stop, w.own);
-  if (ENDS && (w.chunk == 0 || begin >= w.own)) return;
+  // the tile's rows and the state in front of it, each lane its own: registers are short
+  __shared__ __attribute__((aligned(16))) T4<T> s_raw[ENDS ? 1 : 4][ENDS ? 1 : G::R][64];
+  __shared__ __attribute__((aligned(16))) float s_h[ENDS ? 1 : NS][ENDS ? 4 : 256], s_ch[2][G::CW];
+  float(&s_1)[TX][G::CW] = s_dx;
+  if (ENDS && (w.chunk == 0 || w.begin >= w.own)) return;
 
-  float A2[4][NS], g[4][NS], dA[4][NS], bias[4], skip[4], sum[4] = {0, 0, 0, 0}, dskip[4] = {0, 0, 0, 0}, dbias[4] = {0, 0, 0, 0};
-  load_dn<G, NS>(a.A, a.N, w, A2);
+  // rows behind the clip's own have no gradient
+  if (!ENDS) {
+    clear_rows<G, T, VEC>(p, w, a.dx);
+    clear_rows<G, T, VEC>(p, w, a.ddt);
+    if (a.dz) clear_rows<G, T, VEC>(p, w, a.dz);
+  }
+  const int tiles = w.begin < w.end ? (w.end - w.begin + G::TT - 1) / G::TT : 0;
+
+  const Rows<G, T> rx(p, w, a.x, a.x_b, a.x_t), rdt(p, w, a.dt, a.dt_b, a.dt_t), rz(p, w, a.z, a.z_b, a.z_t), rdy(p, w, a.dy, a.dy_b, a.dy_t);
+  const Rows<G, T> rB(p, w, static_cast<const T*>(a.Bm) + w.g * a.Bm_g, a.Bm_b, a.Bm_t), rC(p, w, static_cast<const T*>(a.Cm) + w.g * a.Cm_g, a.Cm_b, a.Cm_t);
+  const Rows<G, T> wx(p, w, a.dx, a.L * a.D, a.D), wdt(p, w, a.ddt, a.L * a.D, a.D), wz(p, w, a.dz, a.L * a.D, a.D);
+  T4<T> nx[G::R], ndt[G::R], nz[G::R], ndy[G::R];
+  T bv[G::PB], cv[G::PB];
+  const auto fetch = [&](int i0) {
+    load_rows<G, T, VEC>(rdt, w, i0, ndt);
+    load_rows<G, T, VEC>(rdy, w, i0, ndy);
+    if (a.z) load_rows<G, T, VEC>(rz, w, i0, nz);
+    load_states<G, T>(rC, p, w, i0, cv);
+    if (!ENDS) {
+      load_rows<G, T, VEC>(rx, w, i0, nx);
+      load_states<G, T>(rB, p, w, i0, bv);
+    }
+  };
+  if (tiles) fetch(w.begin + (tiles - 1) * G::TT);
+
+  float A2[4][NS], g[4][NS], dA[4][NS], sum[4] = {0, 0, 0, 0}, dskip[4] = {0, 0, 0, 0}, dbias[4] = {0, 0, 0, 0};
+  load_dn<NS>(p, a.A, w, A2);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -419,162 +600,214 @@ __global__ void __launch_bounds__(64) scan_backward_kernel(const ScanParams p) {
       A2[c][n] *= kLog2e;
       dA[c][n] = g[c][n] = 0.0f;
     }
-  per_channel(a.dt_bias, w, bias);
-  per_channel(a.skip, w, skip);
+  {
+    float v[4];
+    per_channel(a.dt_bias, w, v);
+    put4(v, &s_ch[0][4 * w.j]);
+    per_channel(a.skip, w, v);
+    put4(v, &s_ch[1][4 * w.j]);
+  }
+  __syncthreads();
   // g: exp(delta_{t+1} A) g_{t+1}, what reaches frame t from behind
-  if (!ENDS && begin < w.own) {
-    if (p.K > 1)
-      load_plane<G, NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
-    else if (a.dh_last)
-      load_dn<G, NS>(a.dh_last + (int64_t)w.b * a.D * a.N, a.N, w, g);
-  }
-  if (!ENDS && w.own == 0 && a.dh_last) load_dn<G, NS>(a.dh_last + (int64_t)w.b * a.D * a.N, a.N, w, g);
+  if (!ENDS && tiles && p.K > 1)
+    load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
+  else if (!ENDS && a.dh_last && (tiles || w.own == 0))
+    load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
 
-  // rows behind the clip's own have no gradient
-  if (!ENDS) {
-    const float zero[4] = {0, 0, 0, 0};
-    for (int64_t i = std::max<int64_t>(begin, w.own) + w.s; i < stop; i += SPLIT) {
-      const int64_t at = ((int64_t)w.b * a.L + i) * a.D + w.c0;
-      store_n<T, 4, VEC>(static_cast<T*>(a.dx) + at, w.nc, zero);
-      store_n<T, 4, VEC>(static_cast<T*>(a.ddt) + at, w.nc, zero);
-      if (a.dz) store_n<T, 4, VEC>(static_cast<T*>(a.dz) + at, w.nc, zero);
-    }
-  }
+  // what the lane adds to dB and dC: one of its 2 NS sums, or none
+  const int held = sum_index<2 * NS, G::J>(w.j), place = held < 0 ? -1 : held < NS ? w.s * NS + held : G::NP + w.s * NS + held - NS;
+  float* const part_bc = p.part_bc + ((int64_t)w.b * p.tiles * a.G + w.tile) * a.L * (2 * G::NP);
 
-  float x[G::R][4], dt[G::R][4], z[G::R][4], dy[G::R][4], bv[G::PB], cv[G::PB];
-  const auto fetch = [&](int64_t i0) {
-    load_rows<G, T, VEC>(p, w, a.dt, a.dt_b, a.dt_t, i0, dt);
-    load_rows<G, T, VEC>(p, w, a.dy, a.dy_b, a.dy_t, i0, dy);
-    if (a.z) load_rows<G, T, VEC>(p, w, a.z, a.z_b, a.z_t, i0, z);
-    load_bc<G, T>(p, w, a.Cm, a.Cm_b, a.Cm_t, a.Cm_g, i0, cv);
-    if (!ENDS) {
-      load_rows<G, T, VEC>(p, w, a.x, a.x_b, a.x_t, i0, x);
-      load_bc<G, T>(p, w, a.Bm, a.Bm_b, a.Bm_t, a.Bm_g, i0, bv);
-    }
+  // the state in front of a tile
+  float h0[ENDS ? 1 : 4][NS];
+  const auto plane = [&](int i0) {
+    if constexpr (!ENDS) load_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.nt + i0 / G::TT) * G::NP * a.D, a.D, w, h0);
   };
-  const int64_t tiles = begin < end ? (end - begin + G::TT - 1) / G::TT : 0;
-  if (tiles) fetch(begin + (tiles - 1) * G::TT);
-  for (int64_t k = tiles - 1; k >= 0; --k) {
-    const int64_t i0 = begin + k * G::TT;
-    float h[4][NS];
-    if (!ENDS) load_plane<G, NS, VEC>(a.saved + ((int64_t)w.b * p.saved_n + i0 / G::TT) * G::NP * a.D, a.D, w, h);
-    float xs[G::R][4], dls[G::R][4], vs[G::R][4], zs[G::R][4], dys[G::R][4], gys[G::R][4];
-#pragma unroll
-    for (int r = 0; r < G::R; ++r) {
-      const bool in = i0 + r * SPLIT + w.s < w.own;
-      float dx[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        vs[r][c] = dt[r][c] + bias[c];
-        dls[r][c] = in ? delta_of(p, vs[r][c]) : 0.0f;
-        dys[r][c] = dy[r][c];
-        zs[r][c] = z[r][c];
-        gys[r][c] = a.z ? dy[r][c] * z[r][c] * sigmoid(z[r][c]) : dy[r][c];
-        if (!in) gys[r][c] = 0.0f;
-        if (ENDS) sum[c] += dls[r][c];
-        xs[r][c] = x[r][c];
-        dx[c] = ENDS ? 0.0f : dls[r][c] * x[r][c];
-        if (!in) dx[c] = 0.0f;
-      }
-      put4(dls[r], &s_dl[r * SPLIT + w.s][4 * w.j]);
-      put4(gys[r], &s_gy[r * SPLIT + w.s][4 * w.j]);
-      if (!ENDS) put4(dx, &s_dx[r * SPLIT + w.s][4 * w.j]);
-    }
-    put_bc<G>(cv, &s_C[0][0]);
-    if (!ENDS) put_bc<G>(bv, &s_B[0][0]);
-    if (k) fetch(i0 - G::TT);
-    __syncthreads();
-    float P[ENDS ? 1 : G::TT][4][NS];  // exp(delta_t A) h_{t-1}
-    if (!ENDS) {
-#pragma unroll
-      for (int t = 0; t < G::TT; ++t) {
-        float dl[4], dx[4], B[NS], C[NS], y[4];
-        get4(&s_dl[t][4 * w.j], dl);
-        get4(&s_dx[t][4 * w.j], dx);
-        get_states<NS>(&s_B[t][w.s * NS], B);
-        get_states<NS>(&s_C[t][w.s * NS], C);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          y[c] = 0.0f;
-#pragma unroll
-          for (int n = 0; n < NS; ++n) {
-            P[t][c][n] = exp2_hw(dl[c] * A2[c][n]) * h[c][n];
-            h[c][n] = fmaf(dx[c], B[n], P[t][c][n]);
-            y[c] = fmaf(C[n], h[c][n], y[c]);
-          }
-        }
-        put_sums<SPLIT, G::CW>(y, w.s, w.j, &s_y[t][0]);
-      }
-    }
-#pragma unroll
-    for (int t = G::TT - 1; t >= 0; --t) {
-      float dl[4], gy[4], dx[4], B[NS], C[NS], S1[4], S2[4], v[2 * NS];
-      get4(&s_dl[t][4 * w.j], dl);
-      get4(&s_gy[t][4 * w.j], gy);
-      get_states<NS>(&s_C[t][w.s * NS], C);
-      if (!ENDS) {
-        get4(&s_dx[t][4 * w.j], dx);
-        get_states<NS>(&s_B[t][w.s * NS], B);
-      }
-#pragma unroll
-      for (int n = 0; n < 2 * NS; ++n) v[n] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        S1[c] = S2[c] = 0.0f;
-#pragma unroll
-        for (int n = 0; n < NS; ++n) {
-          const float gt = fmaf(C[n], gy[c], g[c][n]);
-          if (!ENDS) {
-            const float gp = gt * P[t][c][n];
-            v[n] = fmaf(gt, dx[c], v[n]);
-            v[NS + n] = fmaf(gy[c], fmaf(dx[c], B[n], P[t][c][n]), v[NS + n]);
-            S1[c] = fmaf(gt, B[n], S1[c]);
-            S2[c] = fmaf(gp, A2[c][n], S2[c]);
-            dA[c][n] = fmaf(gp, dl[c], dA[c][n]);
-          }
-          g[c][n] = exp2_hw(dl[c] * A2[c][n]) * gt;
-        }
-      }
-      if (!ENDS) {
-        put_sums<SPLIT, G::CW>(S1, w.s, w.j, &s_1[t][0]);
-        put_sums<SPLIT, G::CW>(S2, w.s, w.j, &s_2[t][0]);
-        float value;
-        int index;
-        bool write;
-        sum_lanes<2 * NS, G::J>(v, w.j, value, index, write);
-        const int64_t i = i0 + t;
-        if (write && i < w.own) {
-          const int at = index < NS ? w.s * NS + index : G::NP + w.s * NS + index - NS;
-          p.part_bc[(((int64_t)w.b * p.tiles * a.G + w.tile) * a.L + row_of(p, w.own, i)) * (2 * G::NP) + at] = value;
-        }
-      }
-    }
-    __syncthreads();
-    if (!ENDS) {
+  if (tiles) plane(w.begin + (tiles - 1) * G::TT);
+
+  for (int k = tiles - 1; k >= 0; --k) {
+    const int i0 = w.begin + k * G::TT;
+    {
+      float bias[4], dl[G::R][4];
+      get4(&s_ch[0][4 * w.j], bias);
+      deltas<G, T, VEC>(p, w, i0, ndt, bias, dl);
 #pragma unroll
       for (int r = 0; r < G::R; ++r) {
-        const int64_t i = i0 + r * SPLIT + w.s;
-        if (i < w.own) {
-          float y[4], s1[4], s2[4], dx[4], ddt[4], dz[4];
-          get4(&s_y[r * SPLIT + w.s][4 * w.j], y);
-          get4(&s_1[r * SPLIT + w.s][4 * w.j], s1);
-          get4(&s_2[r * SPLIT + w.s][4 * w.j], s2);
+        float dx[4], gy[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) gy[c] = (float)ndy[r][c];
+        if (a.z) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) gy[c] *= (float)nz[r][c] * sigmoid((float)nz[r][c]);
+        }
+        only_own<G, VEC>(w, i0, r, gy);
+        put4(dl[r], &s_dl[r * SPLIT + w.s][4 * w.j]);
+        put4(gy, &s_gy[r * SPLIT + w.s][4 * w.j]);
+        if (ENDS) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sum[c] += dl[r][c];
+        } else {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) dx[c] = dl[r][c] * (float)nx[r][c];
+          only_own<G, VEC>(w, i0, r, dx);
+          put4(dx, &s_dx[r * SPLIT + w.s][4 * w.j]);
+          s_raw[0][r][threadIdx.x] = nx[r];
+          s_raw[1][r][threadIdx.x] = ndt[r];
+          s_raw[2][r][threadIdx.x] = ndy[r];
+          if (a.z) s_raw[3][r][threadIdx.x] = nz[r];
+        }
+      }
+      if (!ENDS) {
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          const float v[4] = {h0[0][n], h0[1][n], h0[2][n], h0[3][n]};
+          put4(v, &s_h[n][4 * threadIdx.x]);
+        }
+      }
+    }
+    put_states<G, T>(p, w, i0, cv, &s_C[0][0]);
+    if (!ENDS) put_states<G, T>(p, w, i0, bv, &s_B[0][0]);
+    if (k) fetch(i0 - G::TT);
+    __syncthreads();
+    Step<NS> f[2];
+    float gy[2][4];
+    if constexpr (ENDS) {
+#pragma unroll
+      for (int t = G::TT; t >= 0; --t) {
+        if (t > 0) {
+          f[(t - 1) % 2].template get<G, false, true>(w, t - 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+          get4(&s_gy[t - 1][4 * w.j], gy[(t - 1) % 2]);
+        }
+        if (t == G::TT) continue;
+        const Step<NS>& q = f[t % 2];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int n = 0; n < NS; ++n) g[c][n] = exp2_hw(q.dl[c] * A2[c][n]) * fmaf(q.C[n], gy[t % 2][c], g[c][n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      // the last TB frames first: their states from the tile's start, those of the frames in front not kept
+#pragma unroll 1
+      for (int t0 = G::TT - TB; t0 >= 0; t0 -= TB) {
+        float h[4][NS];
+#pragma unroll
+        for (int n = 0; n < NS; ++n) {
+          float v[4];
+          get4(&s_h[n][4 * threadIdx.x], v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) h[c][n] = v[c];
+        }
+#pragma unroll 1
+        for (int t = 0; t < t0; ++t) {
+          Step<NS> q;
+          q.template get<G, true, false>(w, t, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) h[c][n] = fmaf(exp2_hw(q.dl[c] * A2[c][n]), h[c][n], q.dx[c] * q.B[n]);
+        }
+        float P[TB][4][NS];  // exp(delta_t A) h_{t-1}
+        f[0].template get<G, true, true>(w, t0, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+#pragma unroll
+        for (int i = 0; i < TB; ++i) {
+          const Step<NS>& q = f[i % 2];
+          if (i + 1 < TB) f[(i + 1) % 2].template get<G, true, true>(w, t0 + i + 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+          float y[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            dx[c] = fmaf(dls[r][c], s1[c], skip[c] * gys[r][c]);
-            ddt[c] = fmaf(xs[r][c], s1[c], kLn2 * s2[c]);
-            if (a.softplus) ddt[c] *= sigmoid(vs[r][c]);
-            dskip[c] = fmaf(gys[r][c], xs[r][c], dskip[c]);
-            dbias[c] += ddt[c];
-            if (a.z) {
-              const float sg = sigmoid(zs[r][c]);
-              dz[c] = dys[r][c] * fmaf(skip[c], xs[r][c], y[c]) * sg * fmaf(zs[r][c], 1.0f - sg, 1.0f);
+            y[c] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+              P[i][c][n] = exp2_hw(q.dl[c] * A2[c][n]) * h[c][n];
+              h[c][n] = fmaf(q.dx[c], q.B[n], P[i][c][n]);
+              y[c] = fmaf(q.C[n], h[c][n], y[c]);
             }
           }
-          const int64_t at = ((int64_t)w.b * a.L + row_of(p, w.own, i)) * a.D + w.c0;
-          store_n<T, 4, VEC>(static_cast<T*>(a.dx) + at, w.nc, dx);
-          store_n<T, 4, VEC>(static_cast<T*>(a.ddt) + at, w.nc, ddt);
-          if (a.dz) store_n<T, 4, VEC>(static_cast<T*>(a.dz) + at, w.nc, dz);
+          put_sums<SPLIT, G::CW>(y, w.s, w.j, &s_y[t0 + i][0]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        get4(&s_gy[t0 + TB - 1][4 * w.j], gy[(TB - 1) % 2]);
+#pragma unroll
+        for (int i = TB - 1; i >= 0; --i) {
+          const int t = t0 + i;
+          Step<NS>& q = f[i % 2];  // still there for the last frame
+          // the decays are formed again: kept from above they would take TB * 4 * NS registers more
+#pragma unroll
+          for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(q.dl[c]));
+          if (i > 0) {
+            f[(i - 1) % 2].template get<G, true, true>(w, t - 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+            get4(&s_gy[t - 1][4 * w.j], gy[(i - 1) % 2]);
+          }
+          float S1[4], S2[4], v[2 * NS];
+#pragma unroll
+          for (int n = 0; n < 2 * NS; ++n) v[n] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            S1[c] = S2[c] = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+              const float gt = fmaf(q.C[n], gy[i % 2][c], g[c][n]), gp = gt * P[i][c][n];
+              v[n] = fmaf(gt, q.dx[c], v[n]);
+              v[NS + n] = fmaf(gy[i % 2][c], fmaf(q.dx[c], q.B[n], P[i][c][n]), v[NS + n]);
+              S1[c] = fmaf(gt, q.B[n], S1[c]);
+              S2[c] = fmaf(gp, A2[c][n], S2[c]);
+              dA[c][n] = fmaf(gp, q.dl[c], dA[c][n]);
+              g[c][n] = exp2_hw(q.dl[c] * A2[c][n]) * gt;
+            }
+          }
+          put_sums<SPLIT, G::CW>(S1, w.s, w.j, &s_1[t][0]);
+          put_sums<SPLIT, G::CW>(S2, w.s, w.j, &s_gy[t][0]);
+          const float value = sum_lanes<2 * NS, G::J>(v, w.j);
+          if (place >= 0 && i0 + t < w.own) part_bc[(int64_t)row_of(p, w.own, i0 + t) * (2 * G::NP) + (uint32_t)place] = value;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+    __syncthreads();
+    if constexpr (!ENDS) {
+      if (k) plane(i0 - G::TT);
+      float bias[4], skip[4];
+      get4(&s_ch[0][4 * w.j], bias);
+      get4(&s_ch[1][4 * w.j], skip);
+#pragma unroll
+      for (int r = 0; r < G::R; ++r) {
+        const int row = r * SPLIT + w.s;
+        if (i0 + row < w.own) {
+          const T4<T> x = s_raw[0][r][threadIdx.x], dt = s_raw[1][r][threadIdx.x], dy = s_raw[2][r][threadIdx.x];
+          float s1[4], s2[4], dl[4], gy[4], v[4];
+          get4(&s_1[row][4 * w.j], s1);
+          get4(&s_gy[row][4 * w.j], s2);
+          get4(&s_dl[row][4 * w.j], dl);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) gy[c] = (float)dy[c];
+          if (a.z) {
+            const T4<T> z = s_raw[3][r][threadIdx.x];
+            float y[4];
+            get4(&s_y[row][4 * w.j], y);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const float zc = (float)z[c], sg = sigmoid(zc);
+              v[c] = gy[c] * fmaf(skip[c], (float)x[c], y[c]) * sg * fmaf(zc, 1.0f - sg, 1.0f);
+              gy[c] *= zc * sg;
+            }
+            store_row<G, T, VEC>(wz, w, i0, r, v);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            v[c] = fmaf(dl[c], s1[c], skip[c] * gy[c]);
+            dskip[c] = fmaf(gy[c], (float)x[c], dskip[c]);
+          }
+          store_row<G, T, VEC>(wx, w, i0, r, v);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) v[c] = fmaf((float)x[c], s1[c], kLn2 * s2[c]);
+          if (a.softplus) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c) v[c] *= sigmoid((float)dt[c] + bias[c]);
+          }
+#pragma unroll
+          for (int c = 0; c < 4; ++c) dbias[c] += v[c];
+          store_row<G, T, VEC>(wdt, w, i0, r, v);
         }
       }
       __syncthreads();
@@ -582,7 +815,7 @@ __global__ void __launch_bounds__(64) scan_backward_kernel(const ScanParams p) {
   }
   __syncthreads();
   if (ENDS) {
-    store_plane<G, NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
+    store_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
     put_sums<SPLIT, G::CW>(sum, w.s, w.j, &s_dl[0][0]);
     __syncthreads();
     if (w.s == 0) {
@@ -592,15 +825,15 @@ __global__ void __launch_bounds__(64) scan_backward_kernel(const ScanParams p) {
     }
     return;
   }
-  if (a.dh0 && w.chunk == 0) store_dn<G, NS>(a.dh0 + (int64_t)w.b * a.D * a.N, a.N, w, g);
-  store_plane<G, NS, VEC>(p.part_a + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, dA);
+  if (a.dh0 && w.chunk == 0) store_dn<NS>(a.dh0 + (int64_t)w.b * a.D * a.N, a.N, w, g);
+  store_plane<NS, VEC>(p.part_a + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, dA);
   put_sums<SPLIT, G::CW>(dskip, w.s, w.j, &s_1[0][0]);
-  put_sums<SPLIT, G::CW>(dbias, w.s, w.j, &s_2[0][0]);
+  put_sums<SPLIT, G::CW>(dbias, w.s, w.j, &s_gy[0][0]);
   __syncthreads();
   if (w.s == 0) {
     float u[4], v[4];
     get4(&s_1[0][4 * w.j], u);
-    get4(&s_2[0][4 * w.j], v);
+    get4(&s_gy[0][4 * w.j], v);
     float* to = p.part_d + ((int64_t)w.b * p.K + w.chunk) * 2 * a.D;
     store_n<float, 4, VEC>(to + w.c0, w.nc, u);
     store_n<float, 4, VEC>(to + a.D + w.c0, w.nc, v);
@@ -707,31 +940,32 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const sed_scan_args a) {
 // Instance of a state count: NS states a lane, SPLIT lanes a channel.
 struct Shape { int NS, SPLIT, NP, CW, TT; };
 Shape shape_of(int N) {
-  if (N <= 1) return {1, 1, 1, 256, 8};
-  if (N <= 4) return {4, 1, 4, 256, 8};
-  if (N <= 8) return {4, 2, 8, 128, 8};
+  if (N <= 1) return {1, 1, 1, 256, 4};
+  if (N <= 4) return {2, 2, 4, 128, 4};
+  if (N <= 8) return {2, 4, 8, 64, 8};
   if (N <= 16) return {4, 4, 16, 64, 8};
-  return {8, 4, 32, 64, 4};
+  return {4, 8, 32, 32, 8};
 }
 
+#ifndef SED_WAVES
+#define SED_WAVES 4096
+#define SED_WHOLE 2048
+#endif
 struct Layout {
-  int64_t L_chunk, saved_n;
-  int32_t K, tiles;
+  int32_t K, tiles, nt;
   int64_t h, s, bc, pa, pd, total;  // float offsets into the workspace
 };
 
-// Chunks: 2048 waves keep the 1024 vector units busy; a chunk costs its frames almost twice (once for its end state, once for
+// Chunks: 4096 waves keep the 1024 vector units busy; a chunk costs its frames almost twice (once for its end state, once for
 // its outputs), so a clip stays whole where there are waves enough, and no chunk is shorter than two tiles.
 Layout layout_of(const sed_scan_args& a, bool back) {
   const Shape s = shape_of(a.N);
   Layout l{};
   const int64_t cg = a.D / a.G;
   l.tiles = (int32_t)((cg + s.CW - 1) / s.CW);
-  l.saved_n = (a.L + s.TT - 1) / s.TT;
-  const int64_t waves = a.B * a.G * l.tiles, most = std::max<int64_t>(1, a.L / (2 * s.TT));
-  int64_t K = waves >= 1024 ? 1 : std::min<int64_t>(most, (2048 + waves - 1) / waves);
-  l.L_chunk = ((a.L + K - 1) / K + s.TT - 1) / s.TT * s.TT;
-  K = std::max<int64_t>(1, (a.L + l.L_chunk - 1) / l.L_chunk);
+  l.nt = (int32_t)((a.L + s.TT - 1) / s.TT);
+  const int64_t waves = a.B * a.G * l.tiles, most = std::max<int64_t>(1, l.nt / 2);
+  const int64_t K = waves >= SED_WHOLE ? 1 : std::min<int64_t>(most, (SED_WAVES + waves - 1) / std::max<int64_t>(1, waves));
   l.K = (int32_t)K;
   int64_t at = 0;
   const auto take = [&](int64_t n) { const int64_t o = at; at += (n + 63) / 64 * 64; return o; };
@@ -751,9 +985,11 @@ Layout layout_of(const sed_scan_args& a, bool back) {
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 int check_args(const sed_scan_args* a) {
-  if (!a || a->B < 0 || a->L < 0 || a->D < 1 || a->N < 1 || a->N > 32 || a->G < 1 || a->D % a->G) return SED_ERR_BAD_ARG;
+  if (!a || a->B < 0 || a->L < 0 || a->L > 0x7fffff00 || a->D < 1 || a->D > (1 << 24) || a->N < 1 || a->N > 32 || a->G < 1 || a->D % a->G) return SED_ERR_BAD_ARG;
   if (a->dtype != SED_F32 && a->dtype != SED_BF16 && a->dtype != SED_F16) return SED_ERR_BAD_ARG;
   if (a->B > 0 && a->L > 0 && (!a->x || !a->dt || !a->A || !a->Bm || !a->Cm)) return SED_ERR_BAD_ARG;
+  for (const int64_t t : {a->x_t, a->dt_t, a->z_t, a->dy_t, a->Bm_t, a->Cm_t})
+    if (t < 0 || t > (1 << 26)) return SED_ERR_CAPACITY;
   return SED_OK;
 }
 
@@ -767,16 +1003,25 @@ bool vector_rows(const sed_scan_args& a, bool back) {
   return ok(a.dy, a.dy_b, a.dy_t) && aligned(a.dx, bytes) && aligned(a.ddt, bytes) && aligned(a.dz, bytes);
 }
 
+template <class G, bool BACK>
+void launch_join(const ScanParams& p, hipStream_t stream) {
+  const int64_t n = p.a.B * G::NP * p.a.D;
+  if (p.K <= 16)
+    chunk_join_kernel<G, BACK, 1><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(p);
+  else
+    chunk_join_kernel<G, BACK, 16><<<(unsigned)((n + 15) / 16), 256, 0, stream>>>(p);
+}
+
 template <int NS, int SPLIT, class T, bool VEC>
 int launch(const ScanParams& p, bool back, hipStream_t stream) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
-  const int64_t grid = a.B * p.K * a.G * p.tiles, joins = (a.B * G::NP * a.D + 255) / 256;
-  if (grid > 0x7fffffff || joins > 0x7fffffff) return SED_ERR_CAPACITY;
+  const int64_t grid = a.B * p.K * a.G * p.tiles, joins = a.B * G::NP * a.D / 16;
+  if (grid > 0x7fffffff || joins >= 0x7fffffff) return SED_ERR_CAPACITY;
   if (!back) {
     if (p.K > 1) {
       scan_forward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
-      chunk_join_kernel<false><<<(unsigned)joins, 256, 0, stream>>>(p, G::NP);
+      launch_join<G, false>(p, stream);
     }
     scan_forward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
     return seq_status(hipGetLastError());
@@ -785,7 +1030,7 @@ int launch(const ScanParams& p, bool back, hipStream_t stream) {
   if (bc > 0x7fffffff) return SED_ERR_CAPACITY;
   if (p.K > 1) {
     scan_backward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
-    chunk_join_kernel<true><<<(unsigned)joins, 256, 0, stream>>>(p, G::NP);
+    launch_join<G, true>(p, stream);
   }
   scan_backward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
   scan_bc_kernel<T><<<(unsigned)bc, 256, 0, stream>>>(p, G::NP);
@@ -810,10 +1055,10 @@ int run(const sed_scan_args* args, bool back, void* stream) {
   const Layout l = layout_of(p.a, back);
   if (l.total > 0 && (!args->ws || args->ws_bytes < l.total * 4 || !aligned(args->ws, 16))) return SED_ERR_CAPACITY;
   float* ws = static_cast<float*>(args->ws);
-  p.L_chunk = l.L_chunk;
   p.K = l.K;
+  p.nt = l.nt;
+  p.four = p.a.N % 4 == 0 && aligned(p.a.A, 16) && aligned(p.a.h0, 16) && aligned(p.a.dh_last, 16);
   p.tiles = l.tiles;
-  p.saved_n = (int32_t)l.saved_n;
   p.chunk_h = ws + l.h;
   p.chunk_s = ws + l.s;
   p.part_bc = ws + l.bc;
@@ -823,10 +1068,10 @@ int run(const sed_scan_args* args, bool back, void* stream) {
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const Shape sh = shape_of(p.a.N);
   if (sh.NP == 1) return launch_t<1, 1>(p, back, vec, s);
-  if (sh.NP == 4) return launch_t<4, 1>(p, back, vec, s);
-  if (sh.NP == 8) return launch_t<4, 2>(p, back, vec, s);
+  if (sh.NP == 4) return launch_t<2, 2>(p, back, vec, s);
+  if (sh.NP == 8) return launch_t<2, 4>(p, back, vec, s);
   if (sh.NP == 16) return launch_t<4, 4>(p, back, vec, s);
-  return launch_t<8, 4>(p, back, vec, s);
+  return launch_t<4, 8>(p, back, vec, s);
 }
 
 template <class T>
