@@ -364,14 +364,14 @@ enum { SED_ACT_NONE = 0, SED_ACT_SILU = 1, SED_ACT_RELU = 2, SED_ACT_GELU = 3 };
  * y_t[d] = (sum_n C_t[g,n] h_t[d,n] + skip[d] x_t[d]) * silu(z_t[d]); channel d belongs to group g = d / (D / G). */
 typedef struct sed_scan_args {
   int64_t B, L, D;          /* clips, frames, channels                                             */
-  int32_t N, G;             /* states of a channel (1..32), groups of B and C (D % G == 0)         */
+  int32_t N, G;             /* states of a channel (1..32), groups of B and C (D % G == 0); D <= 2^24 */
   int32_t dtype;            /* SED_F32 ..: x, dt, z, Bm, Cm, y and their gradients                 */
   int32_t softplus;         /* 1: delta = softplus(dt + dt_bias)                                   */
   int32_t reverse;          /* 1: from a clip's last own frame to its first                        */
   const int32_t* frames;    /* [B] or NULL                                                         */
   const void *x, *dt, *z;   /* [B][L][D]; z may be NULL (no gate)                                  */
   const void *Bm, *Cm;      /* [B][L][G][N]                                                        */
-  int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, Bm_b, Bm_t, Bm_g, Cm_b, Cm_t, Cm_g;
+  int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, Bm_b, Bm_t, Bm_g, Cm_b, Cm_t, Cm_g; /* rows (.._t) 0..2^26 apart */
   const float *A, *skip, *dt_bias; /* [D][N], [D] or NULL, [D] or NULL                             */
   const float* h0;          /* [B][D][N] state in front of the first frame, or NULL (zero)         */
   float* h_last;            /* [B][D][N] state behind the last, or NULL; the state of a step       */
@@ -389,7 +389,8 @@ typedef struct sed_scan_args {
 } sed_scan_args;
 
 int64_t sed_gated_scan_saved_floats(int64_t B, int64_t L, int64_t D, int32_t N);
-int64_t sed_gated_scan_workspace(int64_t B, int64_t L, int64_t D, int32_t N, int32_t G, int32_t backward);
+/* Bytes of workspace of a call with these sizes (B, L, D, N, G, and whether frames is NULL; nothing is read through pointers). */
+int64_t sed_gated_scan_workspace(const sed_scan_args* args, int32_t backward);
 int sed_gated_scan_forward(const sed_scan_args* args, void* stream);
 /* Reads the inputs of the forward call and its `saved`. */
 int sed_gated_scan_backward(const sed_scan_args* args, void* stream);

@@ -22,6 +22,9 @@
 
 #include <algorithm>
 
+#ifndef OCCB
+#define OCCB 2
+#endif
 namespace sed {
 namespace {
 
@@ -102,16 +105,14 @@ using T4 = T __attribute__((ext_vector_type(4)));
 template <class G, class T>
 struct Rows {
   const char* base;  // tile of i0 = 0
-  int64_t step;      // bytes from one frame of the walk to the next
-  uint32_t apart;    // bytes between rows
+  int32_t step;      // bytes from one frame of the walk to the next
   __device__ __forceinline__ Rows(const ScanParams& q, const Where& w, const void* p, int64_t sb, int64_t st) {
     const int64_t bytes = st * (int64_t)sizeof(T);
-    apart = (uint32_t)bytes;
-    step = q.a.reverse ? -bytes : bytes;
+    step = (int32_t)(q.a.reverse ? -bytes : bytes);
     base = static_cast<const char*>(p) + w.b * sb * (int64_t)sizeof(T) + (q.a.reverse ? (int64_t)(w.own - G::TT) * bytes : 0);
   }
-  __device__ __forceinline__ const char* tile(int i0) const { return base + i0 * step; }
-  __device__ __forceinline__ uint32_t lane(const Where& w, uint32_t t, uint32_t c) const { return (t ^ w.flip) * apart + c * (uint32_t)sizeof(T); }
+  __device__ __forceinline__ const char* tile(int i0) const { return base + (int64_t)i0 * step; }
+  __device__ __forceinline__ uint32_t lane(const Where& w, uint32_t t, uint32_t c) const { return (t ^ w.flip) * (uint32_t)(w.flip ? -step : step) + c * (uint32_t)sizeof(T); }
 };
 
 // 4 channels of the rows i0 + r * SPLIT + s of a tile.  Every load is in bounds, so none is conditional: rows behind the clip's
@@ -145,7 +146,7 @@ __device__ __forceinline__ void load_states(const Rows<G, T>& rows, const ScanPa
   const int last = std::min(w.own - 1 - i0, G::TT - 1);
 #pragma unroll
   for (int k = 0; k < G::PB; ++k) {
-    const int e = threadIdx.x + 64 * k, n = e % G::NP, t = e / G::NP;
+    const int e = w.s * G::J + w.j + 64 * k, n = e % G::NP, t = e / G::NP;
     out[k] = *reinterpret_cast<const T*>(at + rows.lane(w, std::min(t, last), n < q.a.N ? n : 0));
   }
 }
@@ -154,7 +155,7 @@ template <class G, class T>
 __device__ __forceinline__ void put_states(const ScanParams& q, const Where& w, int i0, const T (&v)[G::PB], float* to) {
 #pragma unroll
   for (int k = 0; k < G::PB; ++k) {
-    const int e = threadIdx.x + 64 * k, n = e % G::NP, t = e / G::NP;
+    const int e = w.s * G::J + w.j + 64 * k, n = e % G::NP, t = e / G::NP;
     if (G::TT * G::NP % 64 == 0 || e < G::TT * G::NP) to[e] = n < q.a.N && i0 + t < w.own ? (float)v[k] : 0.0f;
   }
 }
@@ -184,35 +185,32 @@ __device__ __forceinline__ void put4(const float (&v)[4], float* to) {
   *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
-// What a frame of a tile needs out of LDS.
+// What a frame of a tile needs out of LDS; row, state: the lane's places in the tile's first frame.
 template <int NS>
 struct Step {
-  float dl[4], dx[4], B[NS], C[NS];
-  template <class G, bool X, bool WITH_C>
-  __device__ __forceinline__ void get(const Where& w, int t, const float* s_dl, const float* s_dx, const float* s_B, const float* s_C) {
-    get4(s_dl + t * G::CW + 4 * w.j, dl);
-    if (X) get4(s_dx + t * G::CW + 4 * w.j, dx);
-    if (X) get_states<NS>(s_B + t * G::NP + w.s * NS, B);
-    if (WITH_C) get_states<NS>(s_C + t * G::NP + w.s * NS, C);
+  float dl[4], dx[4], gy[4], B[NS], C[NS];
+  template <class G, bool X, bool GY, bool WITH_C>
+  __device__ __forceinline__ void get(int row, int state, int t, const float* s_dl, const float* s_dx, const float* s_gy, const float* s_B, const float* s_C) {
+    get4(s_dl + row + t * G::CW, dl);
+    if (X) get4(s_dx + row + t * G::CW, dx);
+    if (X) get_states<NS>(s_B + state + t * G::NP, B);
+    if (GY) get4(s_gy + row + t * G::CW, gy);
+    if (WITH_C) get_states<NS>(s_C + state + t * G::NP, C);
   }
 };
 
-// Writes the sums of v[4] over the SPLIT lanes that share a channel to the lane group's 4 places of a row.
-template <int SPLIT, int CW>
-__device__ __forceinline__ void put_sums(const float (&v)[4], int s, int j, float* row) {
-  if constexpr (SPLIT == 8) {
-    // as below, and the two halves of a row of 16 lanes hold the same channel
-    const float v4 = fold16(fold32(v[0], v[2]), fold32(v[1], v[3]));
-    row[4 * j + s / 2] = v4 + dpp<kRor8>(v4);
-  } else if constexpr (SPLIT == 4) {
-    // rows of 16 lanes s = 0..3: halves first (channels 0 | 2 and 1 | 3), then neighbouring rows
-    const float lo = fold32(v[0], v[2]), hi = fold32(v[1], v[3]);
-    row[4 * j + s] = fold16(lo, hi);
+// Writes the sums of v[4] over the SPLIT lanes that share a channel to the lane group's 4 places.
+template <int SPLIT>
+__device__ __forceinline__ void put_sums(const float (&v)[4], int s, float* at) {
+  if constexpr (SPLIT >= 4) {
+    // rows of 16 lanes: halves of the wave first (channels 0 | 2 and 1 | 3), then neighbouring rows; with SPLIT = 8 the two
+    // halves of a row hold the same channel
+    const float u = fold16(fold32(v[0], v[2]), fold32(v[1], v[3]));
+    at[s / (SPLIT / 4)] = SPLIT == 8 ? u + dpp<kRor8>(u) : u;
   } else if constexpr (SPLIT == 2) {
-    const float a = fold32(v[0], v[2]), b = fold32(v[1], v[3]);
-    *reinterpret_cast<f32x2*>(row + 4 * j + 2 * s) = f32x2{a, b};
+    *reinterpret_cast<f32x2*>(at + 2 * s) = f32x2{fold32(v[0], v[2]), fold32(v[1], v[3])};
   } else {
-    put4(v, row + 4 * j);
+    put4(v, at);
   }
 }
 
@@ -401,12 +399,13 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
     if (!ENDS && a.saved) store_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.nt + i0 / G::TT) * G::NP * a.D, a.D, w, h);
     __syncthreads();
 // a frame's values are read while the frame in front of it is worked on
+    const int row = 4 * w.j, state = w.s * NS;
     Step<NS> f[2];
-    f[0].template get<G, true, !ENDS>(w, 0, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+    f[0].template get<G, true, false, !ENDS>(row, state, 0, s_dl[0], s_dx[0], nullptr, s_B[0], s_C[0]);
 #pragma unroll
     for (int t = 0; t < G::TT; ++t) {
       const Step<NS>& q = f[t % 2];
-      if (t + 1 < G::TT) f[(t + 1) % 2].template get<G, true, !ENDS>(w, t + 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+      if (t + 1 < G::TT) f[(t + 1) % 2].template get<G, true, false, !ENDS>(row, state, t + 1, s_dl[0], s_dx[0], nullptr, s_B[0], s_C[0]);
       float y[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -417,7 +416,7 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
           if (!ENDS) y[c] = fmaf(q.C[n], h[c][n], y[c]);
         }
       }
-      if (!ENDS) put_sums<SPLIT, G::CW>(y, w.s, w.j, &s_y[t][0]);
+      if (!ENDS) put_sums<SPLIT>(y, w.s, &s_y[t][4 * w.j]);
       __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
@@ -441,7 +440,7 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
     store_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
     // every lane of a channel summed its own rows
     __syncthreads();
-    put_sums<SPLIT, G::CW>(sum, w.s, w.j, &s_dl[0][0]);
+    put_sums<SPLIT>(sum, w.s, &s_dl[0][4 * w.j]);
     __syncthreads();
     if (w.s == 0) {
       float v[4];
@@ -552,11 +551,12 @@ __device__ __forceinline__ int sum_index(int j) {
 
 // ENDS: only the gradient that reaches the frame in front of the chunk from the chunk's own outputs, and the sum of delta.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(64, ENDS ? 4 : OCCB) scan_backward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
-  const Where w = where<G>(p);
+  Where w = where<G>(p);
   constexpr int TX = ENDS ? 1 : G::TT, TB = G::TB;
+  constexpr bool EARLY = NS <= 2;  // dC is summed while the states are formed: a multiply-add less, TB * NS registers more
   // a row's gy and dx make room for the sums S2 and S1 that its frame leaves behind
   __shared__ __attribute__((aligned(16))) float s_dl[G::TT][G::CW], s_gy[G::TT][G::CW], s_dx[TX][G::CW], s_y[TX][G::CW];
   __shared__ __attribute__((aligned(16))) float s_B[G::TT][G::NP], s_C[G::TT][G::NP];
@@ -627,6 +627,9 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
 
   for (int k = tiles - 1; k >= 0; --k) {
     const int i0 = w.begin + k * G::TT;
+    // every tile forms its lanes' addresses again: kept over the loop they would take forty registers
+    asm volatile("" : "+v"(w.s), "+v"(w.j), "+v"(w.cl), "+v"(w.c0));
+    const int lane = w.s * G::J + w.j;
     {
       float bias[4], dl[G::R][4];
       get4(&s_ch[0][4 * w.j], bias);
@@ -651,17 +654,17 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
           for (int c = 0; c < 4; ++c) dx[c] = dl[r][c] * (float)nx[r][c];
           only_own<G, VEC>(w, i0, r, dx);
           put4(dx, &s_dx[r * SPLIT + w.s][4 * w.j]);
-          s_raw[0][r][threadIdx.x] = nx[r];
-          s_raw[1][r][threadIdx.x] = ndt[r];
-          s_raw[2][r][threadIdx.x] = ndy[r];
-          if (a.z) s_raw[3][r][threadIdx.x] = nz[r];
+          s_raw[0][r][lane] = nx[r];
+          s_raw[1][r][lane] = ndt[r];
+          s_raw[2][r][lane] = ndy[r];
+          if (a.z) s_raw[3][r][lane] = nz[r];
         }
       }
       if (!ENDS) {
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           const float v[4] = {h0[0][n], h0[1][n], h0[2][n], h0[3][n]};
-          put4(v, &s_h[n][4 * threadIdx.x]);
+          put4(v, &s_h[n][4 * lane]);
         }
       }
     }
@@ -669,21 +672,18 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
     if (!ENDS) put_states<G, T>(p, w, i0, bv, &s_B[0][0]);
     if (k) fetch(i0 - G::TT);
     __syncthreads();
+    int row = 4 * w.j, state = w.s * NS;
     Step<NS> f[2];
-    float gy[2][4];
     if constexpr (ENDS) {
 #pragma unroll
       for (int t = G::TT; t >= 0; --t) {
-        if (t > 0) {
-          f[(t - 1) % 2].template get<G, false, true>(w, t - 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
-          get4(&s_gy[t - 1][4 * w.j], gy[(t - 1) % 2]);
-        }
+        if (t > 0) f[(t - 1) % 2].template get<G, false, true, true>(row, state, t - 1, s_dl[0], s_dx[0], s_gy[0], s_B[0], s_C[0]);
         if (t == G::TT) continue;
         const Step<NS>& q = f[t % 2];
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int n = 0; n < NS; ++n) g[c][n] = exp2_hw(q.dl[c] * A2[c][n]) * fmaf(q.C[n], gy[t % 2][c], g[c][n]);
+          for (int n = 0; n < NS; ++n) g[c][n] = exp2_hw(q.dl[c] * A2[c][n]) * fmaf(q.C[n], q.gy[c], g[c][n]);
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
@@ -694,26 +694,31 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
 #pragma unroll
         for (int n = 0; n < NS; ++n) {
           float v[4];
-          get4(&s_h[n][4 * threadIdx.x], v);
+          get4(&s_h[n][4 * lane], v);
 #pragma unroll
           for (int c = 0; c < 4; ++c) h[c][n] = v[c];
         }
 #pragma unroll 1
         for (int t = 0; t < t0; ++t) {
           Step<NS> q;
-          q.template get<G, true, false>(w, t, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+          q.template get<G, true, false, false>(4 * w.j, w.s * NS, t, s_dl[0], s_dx[0], s_gy[0], s_B[0], s_C[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int n = 0; n < NS; ++n) h[c][n] = fmaf(exp2_hw(q.dl[c] * A2[c][n]), h[c][n], q.dx[c] * q.B[n]);
         }
         float P[TB][4][NS];  // exp(delta_t A) h_{t-1}
-        f[0].template get<G, true, true>(w, t0, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+        float dC[EARLY ? TB : 1][NS];
+        row = t0 * G::CW + 4 * w.j;
+        state = t0 * G::NP + w.s * NS;
+        f[0].template get<G, true, EARLY, true>(row, state, 0, s_dl[0], s_dx[0], s_gy[0], s_B[0], s_C[0]);
 #pragma unroll
         for (int i = 0; i < TB; ++i) {
           const Step<NS>& q = f[i % 2];
-          if (i + 1 < TB) f[(i + 1) % 2].template get<G, true, true>(w, t0 + i + 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
+          if (i + 1 < TB) f[(i + 1) % 2].template get<G, true, EARLY, true>(row, state, i + 1, s_dl[0], s_dx[0], s_gy[0], s_B[0], s_C[0]);
           float y[4];
+#pragma unroll
+          for (int n = 0; EARLY && n < NS; ++n) dC[i][n] = 0.0f;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             y[c] = 0.0f;
@@ -722,51 +727,51 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
               P[i][c][n] = exp2_hw(q.dl[c] * A2[c][n]) * h[c][n];
               h[c][n] = fmaf(q.dx[c], q.B[n], P[i][c][n]);
               y[c] = fmaf(q.C[n], h[c][n], y[c]);
+              if (EARLY) dC[i][n] = fmaf(q.gy[c], h[c][n], dC[i][n]);
             }
           }
-          put_sums<SPLIT, G::CW>(y, w.s, w.j, &s_y[t0 + i][0]);
+          put_sums<SPLIT>(y, w.s, s_y[0] + row + i * G::CW);
           __builtin_amdgcn_sched_barrier(0);
         }
-        get4(&s_gy[t0 + TB - 1][4 * w.j], gy[(TB - 1) % 2]);
+        if (t0 == 0 && k) plane(i0 - G::TT);  // the next tile's state takes the registers that h leaves
+        // Everything is read again, and the decays are formed again: kept from above they would take more registers than there
+        // are.  The compiler does not know that these are the same places.
+        asm volatile("" : "+v"(row), "+v"(state));
+        f[(TB - 1) % 2].template get<G, true, true, true>(row, state, TB - 1, s_dl[0], s_dx[0], s_gy[0], s_B[0], s_C[0]);
 #pragma unroll
         for (int i = TB - 1; i >= 0; --i) {
-          const int t = t0 + i;
-          Step<NS>& q = f[i % 2];  // still there for the last frame
-          // the decays are formed again: kept from above they would take TB * 4 * NS registers more
-#pragma unroll
-          for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(q.dl[c]));
-          if (i > 0) {
-            f[(i - 1) % 2].template get<G, true, true>(w, t - 1, s_dl[0], s_dx[0], s_B[0], s_C[0]);
-            get4(&s_gy[t - 1][4 * w.j], gy[(i - 1) % 2]);
-          }
+          const Step<NS>& q = f[i % 2];
+          if (i > 0) f[(i - 1) % 2].template get<G, true, true, true>(row, state, i - 1, s_dl[0], s_dx[0], s_gy[0], s_B[0], s_C[0]);
           float S1[4], S2[4], v[2 * NS];
 #pragma unroll
-          for (int n = 0; n < 2 * NS; ++n) v[n] = 0.0f;
+          for (int n = 0; n < NS; ++n) {
+            v[n] = 0.0f;
+            v[NS + n] = EARLY ? dC[EARLY ? i : 0][n] : 0.0f;
+          }
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             S1[c] = S2[c] = 0.0f;
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
-              const float gt = fmaf(q.C[n], gy[i % 2][c], g[c][n]), gp = gt * P[i][c][n];
+              const float gt = fmaf(q.C[n], q.gy[c], g[c][n]), gp = gt * P[i][c][n];
               v[n] = fmaf(gt, q.dx[c], v[n]);
-              v[NS + n] = fmaf(gy[i % 2][c], fmaf(q.dx[c], q.B[n], P[i][c][n]), v[NS + n]);
+              if (!EARLY) v[NS + n] = fmaf(q.gy[c], fmaf(q.dx[c], q.B[n], P[i][c][n]), v[NS + n]);
               S1[c] = fmaf(gt, q.B[n], S1[c]);
               S2[c] = fmaf(gp, A2[c][n], S2[c]);
               dA[c][n] = fmaf(gp, q.dl[c], dA[c][n]);
               g[c][n] = exp2_hw(q.dl[c] * A2[c][n]) * gt;
             }
           }
-          put_sums<SPLIT, G::CW>(S1, w.s, w.j, &s_1[t][0]);
-          put_sums<SPLIT, G::CW>(S2, w.s, w.j, &s_gy[t][0]);
+          put_sums<SPLIT>(S1, w.s, s_1[0] + row + i * G::CW);
+          put_sums<SPLIT>(S2, w.s, s_gy[0] + row + i * G::CW);
           const float value = sum_lanes<2 * NS, G::J>(v, w.j);
-          if (place >= 0 && i0 + t < w.own) part_bc[(int64_t)row_of(p, w.own, i0 + t) * (2 * G::NP) + (uint32_t)place] = value;
+          if (place >= 0 && i0 + t0 + i < w.own) part_bc[(int64_t)row_of(p, w.own, i0 + t0 + i) * (2 * G::NP) + (uint32_t)place] = value;
           __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
     __syncthreads();
     if constexpr (!ENDS) {
-      if (k) plane(i0 - G::TT);
       float bias[4], skip[4];
       get4(&s_ch[0][4 * w.j], bias);
       get4(&s_ch[1][4 * w.j], skip);
@@ -774,7 +779,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
       for (int r = 0; r < G::R; ++r) {
         const int row = r * SPLIT + w.s;
         if (i0 + row < w.own) {
-          const T4<T> x = s_raw[0][r][threadIdx.x], dt = s_raw[1][r][threadIdx.x], dy = s_raw[2][r][threadIdx.x];
+          const T4<T> x = s_raw[0][r][lane], dt = s_raw[1][r][lane], dy = s_raw[2][r][lane];
           float s1[4], s2[4], dl[4], gy[4], v[4];
           get4(&s_1[row][4 * w.j], s1);
           get4(&s_gy[row][4 * w.j], s2);
@@ -782,7 +787,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
 #pragma unroll
           for (int c = 0; c < 4; ++c) gy[c] = (float)dy[c];
           if (a.z) {
-            const T4<T> z = s_raw[3][r][threadIdx.x];
+            const T4<T> z = s_raw[3][r][lane];
             float y[4];
             get4(&s_y[row][4 * w.j], y);
 #pragma unroll
@@ -816,7 +821,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
   __syncthreads();
   if (ENDS) {
     store_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
-    put_sums<SPLIT, G::CW>(sum, w.s, w.j, &s_dl[0][0]);
+    put_sums<SPLIT>(sum, w.s, &s_dl[0][4 * w.j]);
     __syncthreads();
     if (w.s == 0) {
       float v[4];
@@ -827,8 +832,8 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
   }
   if (a.dh0 && w.chunk == 0) store_dn<NS>(a.dh0 + (int64_t)w.b * a.D * a.N, a.N, w, g);
   store_plane<NS, VEC>(p.part_a + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, dA);
-  put_sums<SPLIT, G::CW>(dskip, w.s, w.j, &s_1[0][0]);
-  put_sums<SPLIT, G::CW>(dbias, w.s, w.j, &s_gy[0][0]);
+  put_sums<SPLIT>(dskip, w.s, &s_1[0][4 * w.j]);
+  put_sums<SPLIT>(dbias, w.s, &s_gy[0][4 * w.j]);
   __syncthreads();
   if (w.s == 0) {
     float u[4], v[4];
@@ -859,21 +864,31 @@ __global__ void __launch_bounds__(256) scan_bc_kernel(const ScanParams p, int NP
   static_cast<T*>(e < NP ? a.dB : a.dC)[((b * a.L + t) * a.G + g) * a.N + n] = (T)v;
 }
 
-// dA [D][N], d skip and d dt_bias [D]: sums over clips and chunks in order; dA's partial sums lie [NP][D].
-__global__ void __launch_bounds__(256) scan_param_kernel(const ScanParams p, int NP) {
+// dA [D][N], d skip and d dt_bias [D]: sums over clips and chunks; dA's partial sums lie [NP][D].  A block has 64 columns and
+// 16 lanes for each, which take every 16th row; they are added in order.
+__global__ void __launch_bounds__(1024) scan_param_kernel(const ScanParams p, int NP) {
   const sed_scan_args& a = p.a;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= (int64_t)(a.N + 2) * a.D) return;
-  const int64_t d = i % a.D, n = i / a.D, rows = a.B * p.K;
-  const float* q = n < a.N ? p.part_a + n * a.D + d : p.part_d + (n - a.N) * a.D + d;
-  const int64_t step = n < a.N ? (int64_t)NP * a.D : 2 * a.D;
+  __shared__ float s[16][64];
+  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x % 64, rows = a.B * p.K;
+  const int ty = threadIdx.x / 64;
+  const int64_t d = i % a.D, n = i / a.D;
+  const bool live = n < a.N + 2;
   float v[4] = {0, 0, 0, 0};
-  int64_t r = 0;
-  for (; r + 4 <= rows; r += 4)
+  if (live) {
+    const float* q = n < a.N ? p.part_a + n * a.D + d : p.part_d + (n - a.N) * a.D + d;
+    const int64_t step = n < a.N ? (int64_t)NP * a.D : 2 * a.D;
+    int64_t r = ty;
+    for (; r + 48 < rows; r += 64)
 #pragma unroll
-    for (int k = 0; k < 4; ++k) v[k] += q[(r + k) * step];
-  for (; r < rows; ++r) v[0] += q[r * step];
-  const float sum = (v[0] + v[1]) + (v[2] + v[3]);
+      for (int k = 0; k < 4; ++k) v[k] += q[(r + 16 * k) * step];
+    for (; r < rows; r += 16) v[0] += q[r * step];
+  }
+  s[ty][threadIdx.x % 64] = (v[0] + v[1]) + (v[2] + v[3]);
+  __syncthreads();
+  if (ty != 0 || !live) return;
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) sum += s[k][threadIdx.x];
   if (n < a.N)
     a.dA[d * a.N + n] = sum;
   else if (n == a.N) {
@@ -931,7 +946,7 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const sed_scan_args a) {
       const float z = (float)static_cast<const T*>(a.z)[b * a.z_b + d];
       y *= z * sigmoid(z);
     }
-    static_cast<T*>(a.y)[b * a.D + d] = (T)y;
+    static_cast<T*>(a.y)[b * a.D + d] = rounded<T>(y);
   }
 }
 
@@ -943,29 +958,59 @@ Shape shape_of(int N) {
   if (N <= 1) return {1, 1, 1, 256, 4};
   if (N <= 4) return {2, 2, 4, 128, 4};
   if (N <= 8) return {2, 4, 8, 64, 8};
-  if (N <= 16) return {4, 4, 16, 64, 8};
+#ifndef SH16
+#define SH16 4
+#endif
+  if (N <= 16) return {16 / SH16, SH16, 16, 256 / SH16, 8};
   return {4, 8, 32, 32, 8};
 }
 
-#ifndef SED_WAVES
-#define SED_WAVES 4096
-#define SED_WHOLE 2048
+#ifndef SED_JOIN
+#define SED_JOIN 4.0
 #endif
 struct Layout {
   int32_t K, tiles, nt;
   int64_t h, s, bc, pa, pd, total;  // float offsets into the workspace
 };
 
-// Chunks: 4096 waves keep the 1024 vector units busy; a chunk costs its frames almost twice (once for its end state, once for
-// its outputs), so a clip stays whole where there are waves enough, and no chunk is shorter than two tiles.
+// Time of `waves` waves of `cost` each on 1024 vector units that hold `most` of them at once: waves share a unit's issue slots
+// (one alone gets 55 % of them, two 79 %, three 86 %, four 90 %, measured on multiply-adds), and a round is over with its last
+// wave.  Clips with lengths of their own: about half the chunks are empty, and the rest is spread as it comes.
+double pass_time(double waves, int most, double cost, bool ragged) {
+  static const double together[] = {0.0, 1.82, 2.53, 3.49, 4.44};
+  if (ragged) return cost * (0.55 * waves / 1024 * together[most] / most + 1.5 * together[1]);
+  const int64_t n = (int64_t)((waves + 1023) / 1024);
+  return cost * (double)(n / most) * together[most] + cost * together[n % most];
+}
+
+// Chunks of a clip.  A chunk's frames are walked twice (for its end state, then for its outputs), so a clip stays whole where
+// there are waves enough; else the count that pass_time gives least for, in units of a forward tile: a wave's start costs two
+// tiles, the gradient's tile 3.4 of them, and joining the states two a chunk at most eight waves deep.
+int64_t chunks_of(const sed_scan_args& a, int64_t waves, int64_t nt, bool back) {
+  const double main = back ? 3.4 : 1.0, ends = back ? 0.8 : 0.72;
+  const int occ = back ? OCCB : 4;
+  double best = 0.0;
+  int64_t K = 1;
+  for (int64_t k = 1; k <= std::max<int64_t>(1, nt / 2) && (k == 1 || waves * k <= 16384); ++k) {
+    const double tiles = (double)((nt + k - 1) / k);
+    double t = pass_time((double)(waves * k), occ, tiles * main + 2.0, a.frames != nullptr);
+    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4, tiles * ends + 2.0, a.frames != nullptr) + SED_JOIN + (double)(waves * k) / 512;
+    if (k == 1 || t < best) best = t, K = k;
+  }
+  return K;
+}
+
 Layout layout_of(const sed_scan_args& a, bool back) {
   const Shape s = shape_of(a.N);
   Layout l{};
   const int64_t cg = a.D / a.G;
   l.tiles = (int32_t)((cg + s.CW - 1) / s.CW);
   l.nt = (int32_t)((a.L + s.TT - 1) / s.TT);
-  const int64_t waves = a.B * a.G * l.tiles, most = std::max<int64_t>(1, l.nt / 2);
-  const int64_t K = waves >= SED_WHOLE ? 1 : std::min<int64_t>(most, (SED_WAVES + waves - 1) / std::max<int64_t>(1, waves));
+#ifdef FK
+  const int64_t K = std::min<int64_t>(back ? BK : FK, std::max(1, l.nt / 2));
+#else
+  const int64_t K = chunks_of(a, a.B * a.G * l.tiles, l.nt, back);
+#endif
   l.K = (int32_t)K;
   int64_t at = 0;
   const auto take = [&](int64_t n) { const int64_t o = at; at += (n + 63) / 64 * 64; return o; };
@@ -1026,7 +1071,7 @@ int launch(const ScanParams& p, bool back, hipStream_t stream) {
     scan_forward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
     return seq_status(hipGetLastError());
   }
-  const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 255) / 256;
+  const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 63) / 64;
   if (bc > 0x7fffffff) return SED_ERR_CAPACITY;
   if (p.K > 1) {
     scan_backward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
@@ -1034,7 +1079,7 @@ int launch(const ScanParams& p, bool back, hipStream_t stream) {
   }
   scan_backward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
   scan_bc_kernel<T><<<(unsigned)bc, 256, 0, stream>>>(p, G::NP);
-  scan_param_kernel<<<(unsigned)pr, 256, 0, stream>>>(p, G::NP);
+  scan_param_kernel<<<(unsigned)pr, 1024, 0, stream>>>(p, G::NP);
   return seq_status(hipGetLastError());
 }
 
@@ -1070,7 +1115,7 @@ int run(const sed_scan_args* args, bool back, void* stream) {
   if (sh.NP == 1) return launch_t<1, 1>(p, back, vec, s);
   if (sh.NP == 4) return launch_t<2, 2>(p, back, vec, s);
   if (sh.NP == 8) return launch_t<2, 4>(p, back, vec, s);
-  if (sh.NP == 16) return launch_t<4, 4>(p, back, vec, s);
+  if (sh.NP == 16) return launch_t<16 / SH16, SH16>(p, back, vec, s);
   return launch_t<4, 8>(p, back, vec, s);
 }
 
@@ -1106,11 +1151,9 @@ extern "C" int64_t sed_gated_scan_saved_floats(int64_t B, int64_t L, int64_t D, 
   return B * ((L + s.TT - 1) / s.TT) * s.NP * D;
 }
 
-extern "C" int64_t sed_gated_scan_workspace(int64_t B, int64_t L, int64_t D, int32_t N, int32_t G, int32_t backward) {
-  sed_scan_args a{};
-  a.B = B, a.L = L, a.D = D, a.N = N, a.G = G;
-  if (B < 0 || L < 0 || D < 1 || N < 1 || N > 32 || G < 1 || D % G) return SED_ERR_BAD_ARG;
-  return sed::layout_of(a, backward != 0).total * 4;
+extern "C" int64_t sed_gated_scan_workspace(const sed_scan_args* a, int32_t backward) {
+  if (!a || a->B < 0 || a->L < 0 || a->D < 1 || a->N < 1 || a->N > 32 || a->G < 1 || a->D % a->G) return SED_ERR_BAD_ARG;
+  return sed::layout_of(*a, backward != 0).total * 4;
 }
 
 extern "C" int sed_gated_scan_forward(const sed_scan_args* args, void* stream) {

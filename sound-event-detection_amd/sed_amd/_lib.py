@@ -114,7 +114,7 @@ SIGNATURES = {
     "sed_resampler_get_filter": (C.c_int, [_vp, C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32), C.POINTER(_i32), _vp]),
     "sed_resampler_forward": (C.c_int, [_vp, _vp, _i32, _f32, _i64, _i64, _i64, _vp, _i64, _vp]),
     "sed_gated_scan_saved_floats": (_i64, [_i64, _i64, _i64, _i32]),
-    "sed_gated_scan_workspace": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32]),
+    "sed_gated_scan_workspace": (_i64, [C.POINTER(ScanArgs), _i32]),
     "sed_gated_scan_forward": (C.c_int, [C.POINTER(ScanArgs), _vp]),
     "sed_gated_scan_backward": (C.c_int, [C.POINTER(ScanArgs), _vp]),
     "sed_gated_scan_step": (C.c_int, [C.POINTER(ScanArgs), _vp]),

@@ -25,8 +25,10 @@ def _ptr(t):
 
 
 def _rows(t):
-    """t with a contiguous last axis (views of a joint projection are read in place)."""
-    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    """t with a contiguous last axis and rows at most 2^26 elements apart (views of a joint projection are read in place)."""
+    if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) <= 1 << 26)):
+        return t
+    return t.contiguous()
 
 
 def _param(t):
@@ -106,7 +108,7 @@ def _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state)
 
 def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state, want_last, want_saved):
     b, n_frames, d = x.shape
-    g, n = B.shape[2], B.shape[3]
+    n = B.shape[3]
     dev = x.device
     y = torch.empty((b, n_frames, d), dtype=x.dtype, device=dev)
     last = torch.empty((b, d, n), dtype=torch.float32, device=dev) if want_last else None
@@ -119,7 +121,7 @@ def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, sta
     if want_saved:
         saved = torch.empty(L.lib.sed_gated_scan_saved_floats(b, n_frames, d, n), dtype=torch.float32, device=dev)
         a.saved = saved.data_ptr()
-    nbytes = L.lib.sed_gated_scan_workspace(b, n_frames, d, n, g, 0)
+    nbytes = L.lib.sed_gated_scan_workspace(C.byref(a), 0)
     if nbytes:
         ws = _workspace(nbytes, dev)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
@@ -143,7 +145,6 @@ class _GatedScan(torch.autograd.Function):
         x, dt, A, B, Cm, D, z, dt_bias, state, frames, saved = ctx.saved_tensors
         softplus, reverse = ctx.flags
         b, n_frames, d = x.shape
-        g, n = B.shape[2], B.shape[3]
         dev = x.device
         new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=dev)  # noqa: E731
         dx, ddt, dA, dB, dC, dD, dz, dbias, dstate = (new(t) for t in (x, dt, A, B, Cm, D, z, dt_bias, state))
@@ -161,7 +162,7 @@ class _GatedScan(torch.autograd.Function):
         a.dy, a.dy_b, a.dy_t, a.dh_last = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
         a.dx, a.ddt, a.dz, a.dB, a.dC = dx.data_ptr(), ddt.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
         a.dA, a.dskip, a.ddt_bias, a.dh0 = dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dstate)
-        nbytes = L.lib.sed_gated_scan_workspace(b, n_frames, d, n, g, 1)
+        nbytes = L.lib.sed_gated_scan_workspace(C.byref(a), 1)
         ws = _workspace(nbytes, dev)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
         _call(L.lib.sed_gated_scan_backward, a, dev, "sed_gated_scan_backward")

@@ -97,8 +97,9 @@ def test_structs_match_the_header(name, cls):
 def test_c_entry_points_refuse():
     from sed_amd import _lib as L
     byref = ctypes.byref
-    assert L.lib.sed_gated_scan_workspace(1, 8, 4, 33, 1, 0) == L.SED_ERR_BAD_ARG
-    assert L.lib.sed_gated_scan_workspace(1, 8, 4, 4, 3, 0) == L.SED_ERR_BAD_ARG
+    assert L.lib.sed_gated_scan_workspace(None, 0) == L.SED_ERR_BAD_ARG
+    assert L.lib.sed_gated_scan_workspace(byref(L.ScanArgs(B=1, L=8, D=4, N=33, G=1)), 0) == L.SED_ERR_BAD_ARG
+    assert L.lib.sed_gated_scan_workspace(byref(L.ScanArgs(B=1, L=8, D=4, N=4, G=3)), 0) == L.SED_ERR_BAD_ARG
     assert L.lib.sed_gated_scan_saved_floats(1, 8, 0, 4) == L.SED_ERR_BAD_ARG
     assert L.lib.sed_causal_conv_workspace(1, 8, 4, 9) == L.SED_ERR_BAD_ARG
     assert L.lib.sed_group_norm_workspace(1, 8, 1, 6, 4) == L.SED_ERR_BAD_ARG
@@ -113,7 +114,9 @@ def test_c_entry_points_refuse():
         a = L.ScanArgs(B=0, L=1, D=4, N=4, G=1)
         assert fn(byref(a), None) == L.SED_OK               # nothing to do
     many = dict(B=1, L=512, D=64, N=16, G=1, x=16, dt=16, A=16, Bm=16, Cm=16, y=16)
-    assert L.lib.sed_gated_scan_workspace(1, 512, 64, 16, 1, 0) > 0
+    assert L.lib.sed_gated_scan_workspace(byref(L.ScanArgs(B=1, L=512, D=64, N=16, G=1)), 0) > 0
+    far = many | {"x_t": (1 << 26) + 1}
+    assert L.lib.sed_gated_scan_forward(byref(L.ScanArgs(**far)), None) == L.SED_ERR_CAPACITY
     assert L.lib.sed_gated_scan_forward(byref(L.ScanArgs(**many)), None) == L.SED_ERR_CAPACITY  # no workspace
     assert L.lib.sed_gated_scan_step(byref(L.ScanArgs(**(many | {"h_last": 16}))), None) == L.SED_ERR_BAD_ARG  # 512 frames
     for fn in (L.lib.sed_causal_conv_forward, L.lib.sed_causal_conv_backward, L.lib.sed_causal_conv_step):
