@@ -2,11 +2,13 @@
 //
 //   u_t[d] = bias[d] + sum_k w[d,k] x_{t-W+1+k}[d],  y = act(u),  x before the first frame = state (or 0)
 //
-// Bound: HBM (read x, write y; the gradient reads x and dy and writes dx).  A thread owns V neighbouring channels (16 bytes)
-// and a run of frames, keeps the window of WM rows and the weights in registers, and meets every row once but for the
-// WM - 1 rows in front of its run.  Rows are loaded WM at a time before they are used.  WM is W rounded up to 2, 4 or 8:
-// the weights in front are zero.  The weight gradient is summed per thread over its run, written once per run and added
-// over the runs in a fixed order.  Sums are fp32 and every output is rounded once.
+// Bound: HBM (read x, write y; the gradient reads x and dy and writes dx).  A wave has 64 V neighbouring channels and a run of
+// TL frames of one clip: which rows it meets and where they lie is the same for all its lanes (scalar work), a lane keeps the
+// window of WM rows, the weights and, in the gradient, the sums of its V channels in registers.  Rows come WM at a time, the
+// next WM on their way while WM are worked on.  A row is read once but for the WM - 1 in front of a run (and behind it, in the
+// gradient).  WM is W rounded up to 2, 4 or 8: the weights in front are zero.  V = 4 where rows allow it and there are channels
+// enough for a wave, else 1.  The weight gradient is summed per lane over its run, written once per run and added over the runs
+// in a fixed order.  Sums are fp32 and every output is rounded once.
 #include "seq_core.h"
 
 #include <algorithm>
@@ -16,15 +18,9 @@ namespace {
 
 struct ConvParams {
   sed_conv_args a;
-  int64_t runs;  // runs of TL frames
-  int32_t TL, nv;
-  float* part;   // [B * runs][W + 1][D]
-};
-
-template <class T, int V, bool VEC>
-struct Lane {
-  int64_t d, own, b, run;
-  int n;
+  int64_t runs;    // runs of TL frames
+  int32_t TL, nw;  // nw: waves along the channels
+  float* part;     // [B * runs][W + 1][D]
 };
 
 __device__ __forceinline__ int64_t own_of(const sed_conv_args& a, int64_t b) {
@@ -33,18 +29,11 @@ __device__ __forceinline__ int64_t own_of(const sed_conv_args& a, int64_t b) {
 __device__ __forceinline__ int64_t row_of(const sed_conv_args& a, int64_t own, int64_t i) { return a.reverse && i < own ? own - 1 - i : i; }
 
 // x at place i of the clip in the order of the walk: the state in front of it, nothing behind it.
-template <class T, int V, bool VEC>
-__device__ __forceinline__ void x_at(const sed_conv_args& a, int64_t b, int64_t own, int64_t d, int64_t i, float (&v)[V]) {
-  const T* p = static_cast<const T*>(a.x) + b * a.x_b + d;
-  int n = V;
-  if (i >= 0) {
-    n = i < own ? V : 0;
-    p += (n ? row_of(a, own, i) : 0) * a.x_t;
-  } else {
-    n = a.state && i + a.W - 1 >= 0 ? V : 0;
-    if (n) p = static_cast<const T*>(a.state) + (b * (a.W - 1) + i + a.W - 1) * a.D + d;
-  }
-  load_n<T, V, VEC>(p, n, v);
+template <class T>
+__device__ __forceinline__ float x_at(const sed_conv_args& a, int64_t b, int64_t own, int64_t d, int64_t i) {
+  if (i >= own) return 0.0f;
+  if (i >= 0) return (float)static_cast<const T*>(a.x)[b * a.x_b + row_of(a, own, i) * a.x_t + d];
+  return a.state && i + a.W - 1 >= 0 ? (float)static_cast<const T*>(a.state)[(b * (a.W - 1) + i + a.W - 1) * a.D + d] : 0.0f;
 }
 
 template <int V, int WM>
@@ -57,113 +46,178 @@ __device__ __forceinline__ void load_weights(const sed_conv_args& a, int64_t d, 
   }
 }
 
-template <class T, int V, bool VEC, int WM, int ACT>
-__global__ void __launch_bounds__(256) conv_forward_kernel(const ConvParams p) {
+template <class T, int V>
+using Vec = T __attribute__((ext_vector_type(V)));
+
+// What a wave works on; d: the lane's first channel, or the last V where it has none (it stores nothing then).
+struct Run {
+  int64_t b, own, i0, i1, index;
+  int64_t d;
+  bool in;
+};
+template <int V>
+__device__ __forceinline__ Run run_of(const ConvParams& p) {
   const sed_conv_args& a = p.a;
-  int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= a.B * p.runs * p.nv) return;
-  const int64_t d = q % p.nv * V;
-  q /= p.nv;
-  const int64_t i0 = q % p.runs * p.TL, b = q / p.runs, own = own_of(a, b), i1 = std::min<int64_t>(i0 + p.TL, a.L);
+  Run r;
+  unsigned q = blockIdx.x;
+  r.d = (int64_t)(q % p.nw * 64 + threadIdx.x) * V;
+  r.in = r.d < a.D;
+  if (!r.in) r.d = a.D - V;
+  q /= p.nw;
+  r.index = q;
+  r.b = q / (unsigned)p.runs;
+  r.i0 = (int64_t)(q % (unsigned)p.runs) * p.TL;
+  r.i1 = std::min<int64_t>(r.i0 + p.TL, a.L);
+  r.own = own_of(a, r.b);
+  return r;
+}
+
+// Row i of x in the order of the walk (i is the same for the wave): the state in front of the clip, zero behind it.
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> row_at(const sed_conv_args& a, const Run& r, int64_t i) {
+  const T* p = nullptr;
+  if (i >= 0 && i < r.own) p = static_cast<const T*>(a.x) + r.b * a.x_b + row_of(a, r.own, i) * a.x_t;
+  if (i < 0 && a.state && i + a.W - 1 >= 0) p = static_cast<const T*>(a.state) + (r.b * (a.W - 1) + i + a.W - 1) * a.D;
+  if (!p) return Vec<T, V>{};
+  return *reinterpret_cast<const Vec<T, V>*>(reinterpret_cast<const char*>(p) + (uint32_t)r.d * (uint32_t)sizeof(T));
+}
+template <class T, int V>
+__device__ __forceinline__ Vec<T, V> dy_at(const sed_conv_args& a, const Run& r, int64_t i) {
+  if (i >= r.own) return Vec<T, V>{};
+  const T* p = static_cast<const T*>(a.dy) + r.b * a.dy_b + row_of(a, r.own, i) * a.dy_t;
+  return *reinterpret_cast<const Vec<T, V>*>(reinterpret_cast<const char*>(p) + (uint32_t)r.d * (uint32_t)sizeof(T));
+}
+template <class T, int V>
+__device__ __forceinline__ void put_row(const sed_conv_args& a, const Run& r, void* base, int64_t i, const float (&v)[V]) {
+  T* p = static_cast<T*>(base) + (r.b * a.L + row_of(a, r.own, i)) * a.D;
+  store_n<T, V, (V > 1)>(reinterpret_cast<T*>(reinterpret_cast<char*>(p) + (uint32_t)r.d * (uint32_t)sizeof(T)), r.in ? V : 0, v);
+}
+
+template <class T, int V, int WM, int ACT>
+__global__ void __launch_bounds__(64) conv_forward_kernel(const ConvParams p) {
+  const sed_conv_args& a = p.a;
+  const Run r = run_of<V>(p);
   float w[WM][V], bias[V], win[WM][V];
-  load_weights<V, WM>(a, d, w, bias);
+  Vec<T, V> next[WM];
 #pragma unroll
-  for (int k = 1; k < WM; ++k) x_at<T, V, VEC>(a, b, own, d, i0 - WM + k, win[k]);  // row i lies in win[(i - i0) % WM]
-  for (int64_t i = i0; i < i1; i += WM) {
-    float in[WM][V];
+  for (int k = 0; k < WM; ++k) next[k] = row_at<T, V>(a, r, r.i0 + k);
 #pragma unroll
-    for (int k = 0; k < WM; ++k) x_at<T, V, VEC>(a, b, own, d, i + k, in[k]);
+  for (int k = 1; k < WM; ++k) {  // row i lies in win[(i - i0) % WM]
+    const Vec<T, V> v = row_at<T, V>(a, r, r.i0 - WM + k);
+#pragma unroll
+    for (int c = 0; c < V; ++c) win[k][c] = (float)v[c];
+  }
+  load_weights<V, WM>(a, r.d, w, bias);
+  for (int64_t i = r.i0; i < r.i1; i += WM) {
+    Vec<T, V> in[WM];
+#pragma unroll
+    for (int k = 0; k < WM; ++k) in[k] = next[k];
+    if (i + WM < r.i1) {
+#pragma unroll
+      for (int k = 0; k < WM; ++k) next[k] = row_at<T, V>(a, r, i + WM + k);
+    }
 #pragma unroll
     for (int k = 0; k < WM; ++k) {
       float y[V];
 #pragma unroll
       for (int c = 0; c < V; ++c) {
-        win[k][c] = in[k][c];
+        win[k][c] = (float)in[k][c];
         float u = bias[c];
 #pragma unroll
         for (int m = 0; m < WM; ++m) u = fmaf(w[m][c], win[(k + 1 + m) % WM][c], u);
-        y[c] = i + k < own ? act<ACT>(u) : 0.0f;
+        y[c] = i + k < r.own ? act<ACT>(u) : 0.0f;
       }
-      if (i + k < i1) store_n<T, V, VEC>(static_cast<T*>(a.y) + (b * a.L + row_of(a, own, i + k)) * a.D + d, V, y);
+      if (i + k < r.i1) put_row<T, V>(a, r, a.y, i + k, y);
     }
   }
 }
 
 // Gradient of the run's rows: du_i = dy_i act'(u_i), dx_i = sum_j w[W-1-j] du_{i+j}; the W - 1 rows behind the run are formed
 // again for it, and counted in the weight gradient by the run they belong to.
-template <class T, int V, bool VEC, int WM, int ACT>
-__global__ void __launch_bounds__(256) conv_backward_kernel(const ConvParams p) {
+template <class T, int V, int WM, int ACT>
+__global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
   const sed_conv_args& a = p.a;
-  int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (q >= a.B * p.runs * p.nv) return;
-  const int64_t d = q % p.nv * V;
-  q /= p.nv;
-  const int64_t run = q, i0 = q % p.runs * p.TL, b = q / p.runs, own = own_of(a, b), i1 = std::min<int64_t>(i0 + p.TL, a.L);
+  const Run r = run_of<V>(p);
   float w[WM][V], bias[V], win[WM][V], du[WM][V], dw[WM][V], db[V];
-  load_weights<V, WM>(a, d, w, bias);
+  Vec<T, V> nx[WM], ny[WM];
+#pragma unroll
+  for (int k = 0; k < WM; ++k) {
+    nx[k] = row_at<T, V>(a, r, r.i0 + k);
+    ny[k] = dy_at<T, V>(a, r, r.i0 + k);
+  }
+#pragma unroll
+  for (int k = 1; k < WM; ++k) {
+    const Vec<T, V> v = row_at<T, V>(a, r, r.i0 - WM + k);
+#pragma unroll
+    for (int c = 0; c < V; ++c) win[k][c] = (float)v[c];
+  }
+  load_weights<V, WM>(a, r.d, w, bias);
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     db[c] = 0.0f;
 #pragma unroll
     for (int k = 0; k < WM; ++k) dw[k][c] = du[k][c] = 0.0f;
   }
-#pragma unroll
-  for (int k = 1; k < WM; ++k) x_at<T, V, VEC>(a, b, own, d, i0 - WM + k, win[k]);
-  for (int64_t i = i0; i < i1 + WM - 1; i += WM) {
-    float in[WM][V], dy[WM][V];
+  for (int64_t i = r.i0; i < r.i1 + WM - 1; i += WM) {
+    Vec<T, V> in[WM], dy[WM];
 #pragma unroll
     for (int k = 0; k < WM; ++k) {
-      x_at<T, V, VEC>(a, b, own, d, i + k, in[k]);
-      const bool mine = i + k < own;
-      load_n<T, V, VEC>(static_cast<const T*>(a.dy) + b * a.dy_b + (mine ? row_of(a, own, i + k) : 0) * a.dy_t + d, mine ? V : 0, dy[k]);
+      in[k] = nx[k];
+      dy[k] = ny[k];
+    }
+    if (i + WM < r.i1 + WM - 1) {
+#pragma unroll
+      for (int k = 0; k < WM; ++k) {
+        nx[k] = row_at<T, V>(a, r, i + WM + k);
+        ny[k] = dy_at<T, V>(a, r, i + WM + k);
+      }
     }
 #pragma unroll
     for (int k = 0; k < WM; ++k) {
-      const bool counts = i + k < i1;  // rows behind the clip's own have dy = 0
+      const bool counts = i + k < r.i1;  // rows behind the clip's own have dy = 0
+      const int64_t at = i + k - (WM - 1);
       float dx[V];
 #pragma unroll
       for (int c = 0; c < V; ++c) {
-        win[k][c] = in[k][c];
+        win[k][c] = (float)in[k][c];
         float u = bias[c];
 #pragma unroll
         for (int m = 0; m < WM; ++m) u = fmaf(w[m][c], win[(k + 1 + m) % WM][c], u);
-        const float g = i + k < own ? dy[k][c] * act_slope<ACT>(u) : 0.0f;
-        du[k][c] = g;
-        const float gc = counts ? g : 0.0f;
-        db[c] += gc;
-#pragma unroll
-        for (int m = 0; m < WM; ++m) dw[m][c] = fmaf(gc, win[(k + 1 + m) % WM][c], dw[m][c]);
-        // row i + k - (WM - 1): du of that row and the WM - 1 behind it
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < WM; ++j) s = fmaf(w[WM - 1 - j][c], du[(k + 1 + j) % WM][c], s);
-        dx[c] = s;
+        du[k][c] = i + k < r.own ? (float)dy[k][c] * act_slope<ACT>(u) : 0.0f;
       }
-      const int64_t r = i + k - (WM - 1);
-      if (r >= i0 && r < i1) {
-        const int64_t late = r - (own - (a.W - 1));  // row of the state that the call returned
-        if (r >= own) {
+      if (counts) {
 #pragma unroll
-          for (int c = 0; c < V; ++c) dx[c] = 0.0f;
-        } else if (a.dstate_out && late >= 0) {
-          float e[V];
-          load_n<T, V, VEC>(static_cast<const T*>(a.dstate_out) + (b * (a.W - 1) + late) * a.D + d, V, e);
+        for (int c = 0; c < V; ++c) {
+          db[c] += du[k][c];
 #pragma unroll
-          for (int c = 0; c < V; ++c) dx[c] += e[c];
+          for (int m = 0; m < WM; ++m) dw[m][c] = fmaf(du[k][c], win[(k + 1 + m) % WM][c], dw[m][c]);
         }
-        store_n<T, V, VEC>(static_cast<T*>(a.dx) + (b * a.L + row_of(a, own, r)) * a.D + d, V, dx);
+      }
+      if (at >= r.i0 && at < r.i1) {
+        // row i + k - (WM - 1): du of that row and of the WM - 1 behind it
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          dx[c] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < WM; ++j) dx[c] = fmaf(w[WM - 1 - j][c], du[(k + 1 + j) % WM][c], dx[c]);
+          if (at >= r.own) dx[c] = 0.0f;
+        }
+        const int64_t late = at - (r.own - (a.W - 1));  // row of the state that the call returned
+        if (a.dstate_out && late >= 0 && at < r.own) {
+          const T* e = static_cast<const T*>(a.dstate_out) + (r.b * (a.W - 1) + late) * a.D + r.d;
+#pragma unroll
+          for (int c = 0; c < V; ++c) dx[c] += (float)e[c];
+        }
+        put_row<T, V>(a, r, a.dx, at, dx);
       }
     }
   }
-  float* to = p.part + run * (a.W + 1) * a.D + d;
+  if (!r.in) return;
+  float* to = p.part + r.index * (a.W + 1) * a.D + r.d;
 #pragma unroll
   for (int k = 0; k < WM; ++k)
-    if (k >= WM - a.W) {
-#pragma unroll
-      for (int c = 0; c < V; ++c) to[(int64_t)(k - (WM - a.W)) * a.D + c] = dw[k][c];
-    }
-#pragma unroll
-  for (int c = 0; c < V; ++c) to[(int64_t)a.W * a.D + c] = db[c];
+    if (k >= WM - a.W) store_n<float, V, (V > 1)>(to + (int64_t)(k - (WM - a.W)) * a.D, V, dw[k]);
+  store_n<float, V, (V > 1)>(to + (int64_t)a.W * a.D, V, db);
 }
 
 // The last W - 1 rows the clip has seen, its state in front of them where it has fewer of its own.
@@ -172,9 +226,7 @@ __global__ void __launch_bounds__(256) conv_state_kernel(const sed_conv_args a) 
   const int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x, n = a.W - 1;
   if (q >= a.B * n * a.D) return;
   const int64_t d = q % a.D, r = q / a.D % n, b = q / a.D / n, own = own_of(a, b);
-  float v[1];
-  x_at<T, 1, false>(a, b, own, d, own - n + r, v);
-  static_cast<T*>(a.state_out)[q] = (T)v[0];
+  static_cast<T*>(a.state_out)[q] = (T)x_at<T>(a, b, own, d, own - n + r);
 }
 
 // Gradient of the state: row r is place r - (W - 1) in front of the clip.
@@ -186,17 +238,13 @@ __global__ void __launch_bounds__(256) conv_state_grad_kernel(const sed_conv_arg
   float s = 0.0f;
   for (int64_t t = 0; t <= i + a.W - 1 && t < own; ++t) {
     float u = a.bias ? a.bias[d] : 0.0f;
-    for (int k = 0; k < a.W; ++k) {
-      float v[1];
-      x_at<T, 1, false>(a, b, own, d, t - (a.W - 1) + k, v);
-      u = fmaf(a.weight[d * a.W + k], v[0], u);
-    }
+    for (int k = 0; k < a.W; ++k) u = fmaf(a.weight[d * a.W + k], x_at<T>(a, b, own, d, t - (a.W - 1) + k), u);
     const float g = (float)static_cast<const T*>(a.dy)[b * a.dy_b + row_of(a, own, t) * a.dy_t + d] * act_slope<ACT>(u);
     s = fmaf(a.weight[d * a.W + (i - t + a.W - 1)], g, s);
   }
   const int64_t late = i - (own - n);
   if (a.dstate_out && late >= 0) s += (float)static_cast<const T*>(a.dstate_out)[(b * n + late) * a.D + d];
-  static_cast<T*>(a.dstate)[q] = (T)s;
+  static_cast<T*>(a.dstate)[q] = rounded<T>(s);
 }
 
 // dw [D][W] and db [D] out of the runs' sums [rows][W + 1][D], a thread for every 4th row, added in order.
@@ -263,75 +311,77 @@ __global__ void __launch_bounds__(256) conv_step_kernel(const sed_conv_args a, i
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
 int check_args(const sed_conv_args* a) {
-  if (!a || a->B < 0 || a->L < 0 || a->D < 1 || a->W < 1 || a->W > 8) return SED_ERR_BAD_ARG;
+  if (!a || a->B < 0 || a->L < 0 || a->D < 1 || a->D > (1 << 24) || a->W < 1 || a->W > 8) return SED_ERR_BAD_ARG;
   if (a->dtype != SED_F32 && a->dtype != SED_BF16 && a->dtype != SED_F16) return SED_ERR_BAD_ARG;
   if (a->act != SED_ACT_NONE && a->act != SED_ACT_SILU) return SED_ERR_BAD_ARG;
   if (a->B > 0 && a->L > 0 && (!a->x || !a->weight)) return SED_ERR_BAD_ARG;
   return SED_OK;
 }
 
+// Channels a lane takes: 4 where every row allows such loads and at least one wave of lanes is filled, else 1.
 int vector_of(const sed_conv_args& a) {
-  const int V = a.dtype == SED_F32 ? 4 : 8;
-  const auto ok = [&](const void* p) { return aligned(p, 16); };
-  const bool vec = a.D % V == 0 && a.x_b % V == 0 && a.x_t % V == 0 && (!a.dy || (a.dy_b % V == 0 && a.dy_t % V == 0)) && ok(a.x) && ok(a.dy) &&
-                   ok(a.y) && ok(a.dx) && ok(a.state) && ok(a.state_out) && ok(a.dstate_out);
-  return vec ? V : 1;
+  const int64_t bytes = a.dtype == SED_F32 ? 16 : 8;
+  const auto ok = [&](const void* p) { return aligned(p, bytes); };
+  const bool vec = a.D % 4 == 0 && a.D >= 256 && a.x_b % 4 == 0 && a.x_t % 4 == 0 && a.dy_b % 4 == 0 && a.dy_t % 4 == 0 && ok(a.x) && ok(a.dy) &&
+                   ok(a.y) && ok(a.dx) && ok(a.state) && ok(a.state_out);
+  return vec ? 4 : 1;
 }
 
-// Frames of a run: long runs read fewer rows twice and leave fewer sums behind; short ones keep 256 compute units busy
-// (64 Ki threads at least).
-int run_frames(int64_t B, int64_t L, int64_t nv, bool back) {
-  int TL = back ? 64 : 16;
-  while (TL > 8 && B * nv * ((L + TL - 1) / TL) < 65536) TL /= 2;
+// Frames of a run: long runs read fewer rows twice and leave fewer sums behind; short ones make waves enough for the card
+// (4096, four for each vector unit).
+int run_frames(int64_t B, int64_t L, int64_t nw, bool back) {
+  int TL = back ? 64 : 32;
+  while (TL > 8 && B * nw * ((L + TL - 1) / TL) < 4096) TL /= 2;
   return TL;
 }
+int64_t waves_along(int64_t D, int V) { return (D / V + 63) / 64; }
 
-template <class T, int V, bool VEC, int WM>
+template <class T, int V, int WM>
 int launch(const ConvParams& p, bool back, hipStream_t s) {
   const sed_conv_args& a = p.a;
-  const int64_t grid = (a.B * p.runs * p.nv + 255) / 256;
+  const int64_t grid = a.B * p.runs * p.nw;
   if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
   const unsigned n = (unsigned)grid;
   if (!back) {
     if (a.act == SED_ACT_SILU)
-      conv_forward_kernel<T, V, VEC, WM, SED_ACT_SILU><<<n, 256, 0, s>>>(p);
+      conv_forward_kernel<T, V, WM, SED_ACT_SILU><<<n, 64, 0, s>>>(p);
     else
-      conv_forward_kernel<T, V, VEC, WM, SED_ACT_NONE><<<n, 256, 0, s>>>(p);
+      conv_forward_kernel<T, V, WM, SED_ACT_NONE><<<n, 64, 0, s>>>(p);
     return seq_status(hipGetLastError());
   }
   if (a.act == SED_ACT_SILU)
-    conv_backward_kernel<T, V, VEC, WM, SED_ACT_SILU><<<n, 256, 0, s>>>(p);
+    conv_backward_kernel<T, V, WM, SED_ACT_SILU><<<n, 64, 0, s>>>(p);
   else
-    conv_backward_kernel<T, V, VEC, WM, SED_ACT_NONE><<<n, 256, 0, s>>>(p);
+    conv_backward_kernel<T, V, WM, SED_ACT_NONE><<<n, 64, 0, s>>>(p);
   conv_param_kernel<<<(unsigned)(((a.W + 1) * a.D + 63) / 64), 1024, 0, s>>>(p);
   return seq_status(hipGetLastError());
 }
 
-template <class T, int V, bool VEC, int WM>
+template <class T, int V, int WM>
 int launch_step(const sed_conv_args& a, hipStream_t s) {
   const int nv = (int)(a.D / V);
   const int64_t grid = (a.B * nv + 255) / 256;
   if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
   if (a.act == SED_ACT_SILU)
-    conv_step_kernel<T, V, VEC, WM, SED_ACT_SILU><<<(unsigned)grid, 256, 0, s>>>(a, nv);
+    conv_step_kernel<T, V, (V > 1), WM, SED_ACT_SILU><<<(unsigned)grid, 256, 0, s>>>(a, nv);
   else
-    conv_step_kernel<T, V, VEC, WM, SED_ACT_NONE><<<(unsigned)grid, 256, 0, s>>>(a, nv);
+    conv_step_kernel<T, V, (V > 1), WM, SED_ACT_NONE><<<(unsigned)grid, 256, 0, s>>>(a, nv);
   return seq_status(hipGetLastError());
 }
 
 enum Kind { FORWARD, BACKWARD, STEP };
 
-template <class T, int V, bool VEC>
+template <class T, int V>
 int go_w(const ConvParams& p, Kind kind, hipStream_t s) {
-  if (p.a.W <= 2) return kind == STEP ? launch_step<T, V, VEC, 2>(p.a, s) : launch<T, V, VEC, 2>(p, kind == BACKWARD, s);
-  if (p.a.W <= 4) return kind == STEP ? launch_step<T, V, VEC, 4>(p.a, s) : launch<T, V, VEC, 4>(p, kind == BACKWARD, s);
-  return kind == STEP ? launch_step<T, V, VEC, 8>(p.a, s) : launch<T, V, VEC, 8>(p, kind == BACKWARD, s);
+  if (p.a.W <= 2) return kind == STEP ? launch_step<T, V, 2>(p.a, s) : launch<T, V, 2>(p, kind == BACKWARD, s);
+  if (p.a.W <= 4) return kind == STEP ? launch_step<T, V, 4>(p.a, s) : launch<T, V, 4>(p, kind == BACKWARD, s);
+  return kind == STEP ? launch_step<T, V, 8>(p.a, s) : launch<T, V, 8>(p, kind == BACKWARD, s);
 }
 
-template <class T, int V>
-int go(const ConvParams& p, Kind kind, bool vec, hipStream_t s) {
+template <class T>
+int go(const ConvParams& p, Kind kind, int V, hipStream_t s) {
   const sed_conv_args& a = p.a;
-  int rc = vec ? go_w<T, V, true>(p, kind, s) : go_w<T, 1, false>(p, kind, s);
+  int rc = V == 4 ? go_w<T, 4>(p, kind, s) : go_w<T, 1>(p, kind, s);
   if (rc != SED_OK || kind == STEP || a.W == 1) return rc;
   const int64_t grid = (a.B * (a.W - 1) * a.D + 255) / 256;
   if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
@@ -349,17 +399,17 @@ int run(const sed_conv_args* args, Kind kind, void* stream) {
   ConvParams p{};
   p.a = *args;
   const int V = vector_of(p.a);
-  p.nv = (int32_t)(p.a.D / V);
-  p.TL = run_frames(p.a.B, p.a.L, p.nv, kind == BACKWARD);
+  p.nw = (int32_t)waves_along(p.a.D, V);
+  p.TL = run_frames(p.a.B, p.a.L, p.nw, kind == BACKWARD);
   p.runs = (p.a.L + p.TL - 1) / p.TL;
   if (kind == BACKWARD) {
     if (!p.a.ws || p.a.ws_bytes < 4 * p.a.B * p.runs * (p.a.W + 1) * p.a.D || !aligned(p.a.ws, 16)) return SED_ERR_CAPACITY;
     p.part = static_cast<float*>(p.a.ws);
   }
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (p.a.dtype == SED_F32) return go<float, 4>(p, kind, V > 1, s);
-  if (p.a.dtype == SED_BF16) return go<bf16, 8>(p, kind, V > 1, s);
-  return go<f16, 8>(p, kind, V > 1, s);
+  if (p.a.dtype == SED_F32) return go<float>(p, kind, V, s);
+  if (p.a.dtype == SED_BF16) return go<bf16>(p, kind, V, s);
+  return go<f16>(p, kind, V, s);
 }
 
 }  // namespace
@@ -368,9 +418,9 @@ int run(const sed_conv_args* args, Kind kind, void* stream) {
 extern "C" int64_t sed_causal_conv_workspace(int64_t B, int64_t L, int64_t D, int32_t W) {
   if (B < 0 || L < 0 || D < 1 || W < 1 || W > 8) return SED_ERR_BAD_ARG;
   int64_t most = 0;
-  for (const int V : {1, 4, 8}) {
+  for (const int V : {1, 4}) {
     if (D % V) continue;
-    const int TL = sed::run_frames(B, L, D / V, true);
+    const int TL = sed::run_frames(B, L, sed::waves_along(D, V), true);
     most = std::max<int64_t>(most, 4 * B * ((L + TL - 1) / TL) * (W + 1) * D);
   }
   return most;
