@@ -38,6 +38,16 @@ __device__ __forceinline__ float x_at(const sed_conv_args& a, int64_t b, int64_t
 
 template <int V, int WM>
 __device__ __forceinline__ void load_weights(const sed_conv_args& a, int64_t d, float (&w)[WM][V], float (&bias)[V]) {
+  if (WM == 4 && a.W == 4 && reinterpret_cast<uintptr_t>(a.weight) % 16 == 0) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.weight + (d + c) * 4);
+      bias[c] = a.bias ? a.bias[d + c] : 0.0f;
+#pragma unroll
+      for (int k = 0; k < WM; ++k) w[k][c] = v[k % 4];
+    }
+    return;
+  }
 #pragma unroll
   for (int c = 0; c < V; ++c) {
     bias[c] = a.bias ? a.bias[d + c] : 0.0f;

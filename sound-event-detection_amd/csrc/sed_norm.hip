@@ -18,6 +18,7 @@ struct NormParams {
   sed_norm_args a;
   int64_t S;         // places of a clip
   int32_t nv, nb;    // vectors of a row, lanes along a row
+  int32_t half;      // half the lanes of a channel, rounded up to a power of two
   int32_t blocks;    // blocks a clip is cut into
   int64_t rows;      // places of a block
   float* part;       // [B][blocks][2][C]: (mean, sum of squares about it), or (sum du, sum du n)
@@ -32,15 +33,17 @@ __device__ __forceinline__ int64_t own_of(const NormParams& p, int64_t b) {
 }
 
 struct Cell {
-  int64_t b, r0, r1, c;
+  int64_t b, block, r0, r1, c;
   int ty, step;
   bool in;
 };
-template <int V>
+// LATE: the second walk over the map goes from its end, which the first one read last and the memory-side cache still holds.
+template <int V, bool LATE>
 __device__ __forceinline__ Cell cell(const NormParams& p) {
   Cell q;
-  q.b = blockIdx.y;
-  q.r0 = blockIdx.x * p.rows;
+  q.b = LATE ? p.a.B - 1 - blockIdx.y : blockIdx.y;
+  q.block = LATE ? p.blocks - 1 - blockIdx.x : blockIdx.x;
+  q.r0 = q.block * p.rows;
   q.r1 = std::min<int64_t>(q.r0 + p.rows, p.S);
   const int tx = threadIdx.x % p.nb, v = blockIdx.z * p.nb + tx;
   q.ty = threadIdx.x / p.nb;
@@ -54,7 +57,7 @@ __device__ __forceinline__ Cell cell(const NormParams& p) {
 template <class T, int V, bool VEC>
 __global__ void __launch_bounds__(256) norm_stats_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
-  const Cell q = cell<V>(p);
+  const Cell q = cell<V, false>(p);
   const int64_t end = std::min<int64_t>(q.r1, own_of(p, q.b));
   if (q.r0 >= end) return;
   __shared__ float s_m[256][V + 1], s_v[256][V + 1];
@@ -92,31 +95,28 @@ __global__ void __launch_bounds__(256) norm_stats_kernel(const NormParams p) {
     }
   }
   s_n[threadIdx.x] = (int)n;
-  __syncthreads();
-  if (q.in && q.ty == 0) {
-    float mean[V], var[V];
-    float count = 0.0f;
-#pragma unroll
-    for (int c = 0; c < V; ++c) mean[c] = var[c] = 0.0f;
-    for (int y = 0; y < q.step; ++y) {
-      const int at = y * p.nb + threadIdx.x;
-      const float m = (float)s_n[at];
-      if (m == 0.0f) break;
-      const float all = count + m, part = m / all;
+  // the lanes of a channel in pairs, half as many each time
+  for (int half = p.half; half >= 1; half /= 2) {
+    __syncthreads();
+    const int from = threadIdx.x + half * p.nb;
+    if (q.in && q.ty < half && q.ty + half < q.step && s_n[from] > 0) {
+      const float m = (float)s_n[from], mine = (float)s_n[threadIdx.x], part = m / (mine + m);
+      s_n[threadIdx.x] += s_n[from];
 #pragma unroll
       for (int c = 0; c < V; ++c) {
-        const float e = s_m[at][c] - mean[c];
-        mean[c] = fmaf(e, part, mean[c]);
-        var[c] += fmaf(e * e, count * part, s_v[at][c]);
+        const float e = s_m[from][c] - s_m[threadIdx.x][c];
+        s_m[threadIdx.x][c] = fmaf(e, part, s_m[threadIdx.x][c]);
+        s_v[threadIdx.x][c] += fmaf(e * e, mine * part, s_v[from][c]);
       }
-      count = all;
     }
-    float* to = p.part + (q.b * p.blocks + blockIdx.x) * 2 * a.C + q.c;
+  }
+  if (q.in && q.ty == 0) {
+    float* to = p.part + (q.b * p.blocks + q.block) * 2 * a.C + q.c;
+    float mean[V], var[V];
 #pragma unroll
-    for (int c = 0; c < V; ++c) {
-      to[c] = mean[c];
-      to[a.C + c] = var[c];
-    }
+    for (int c = 0; c < V; ++c) mean[c] = s_m[threadIdx.x][c], var[c] = s_v[threadIdx.x][c];
+    store_n<float, V, false>(to, V, mean);
+    store_n<float, V, false>(to + a.C, V, var);
   }
 }
 
@@ -180,7 +180,7 @@ __device__ __forceinline__ void channels(const NormParams& p, const Cell& q, flo
 template <class T, int V, bool VEC, int ACT>
 __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
-  const Cell q = cell<V>(p);
+  const Cell q = cell<V, true>(p);
   if (!q.in) return;
   const int64_t own = own_of(p, q.b);
   float mean[V], rstd[V], w[V], bias[V];
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
 template <class T, int V, bool VEC, int ACT>
 __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
-  const Cell q = cell<V>(p);
+  const Cell q = cell<V, false>(p);
   const int64_t end = std::min<int64_t>(q.r1, own_of(p, q.b));
   __shared__ float s_1[256][V + 1], s_2[256][V + 1];
   float s1[V], s2[V];
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p)
     channels<V>(p, q, mean, rstd, w, bias);
     const int64_t at = q.b * p.S * a.C + q.c;
     const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t r = q.r0 + q.ty; r < end; r += q.step) {
       float v[V], g[V];
       load_n<T, V, VEC>(x + r * a.C, V, v);
@@ -232,20 +232,23 @@ __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p)
     s_1[threadIdx.x][c] = s1[c];
     s_2[threadIdx.x][c] = s2[c];
   }
-  __syncthreads();
-  if (q.in && q.ty == 0) {
-    for (int y = 1; y < q.step; ++y)
+  for (int half = p.half; half >= 1; half /= 2) {
+    __syncthreads();
+    const int from = threadIdx.x + half * p.nb;
+    if (q.ty < half && q.ty + half < q.step) {
 #pragma unroll
       for (int c = 0; c < V; ++c) {
-        s1[c] += s_1[y * p.nb + threadIdx.x][c];
-        s2[c] += s_2[y * p.nb + threadIdx.x][c];
+        s_1[threadIdx.x][c] += s_1[from][c];
+        s_2[threadIdx.x][c] += s_2[from][c];
       }
-    float* to = p.part + (q.b * p.blocks + blockIdx.x) * 2 * a.C + q.c;
-#pragma unroll
-    for (int c = 0; c < V; ++c) {
-      to[c] = s1[c];
-      to[a.C + c] = s2[c];
     }
+  }
+  if (q.in && q.ty == 0) {
+#pragma unroll
+    for (int c = 0; c < V; ++c) s1[c] = s_1[threadIdx.x][c], s2[c] = s_2[threadIdx.x][c];
+    float* to = p.part + (q.b * p.blocks + q.block) * 2 * a.C + q.c;
+    store_n<float, V, false>(to, V, s1);
+    store_n<float, V, false>(to + a.C, V, s2);
   }
 }
 
@@ -297,7 +300,7 @@ __global__ void __launch_bounds__(256) norm_param_kernel(const NormParams p) {
 template <class T, int V, bool VEC, int ACT>
 __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
-  const Cell q = cell<V>(p);
+  const Cell q = cell<V, true>(p);
   if (!q.in) return;
   const int64_t own = own_of(p, q.b), cg = a.C / a.G;
   float mean[V], rstd[V], w[V], bias[V], m1[V], m2[V];
@@ -311,7 +314,7 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   const int64_t at = q.b * p.S * a.C + q.c;
   const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
   T* dx = static_cast<T*>(a.dx) + at;
-#pragma unroll 2
+#pragma unroll 4
   for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
     float v[V], g[V];
     load_n<T, V, VEC>(x + r * a.C, r < own ? V : 0, v);
@@ -342,11 +345,11 @@ struct Layout {
   int64_t rows, part, chan, gsum, total;
   int32_t blocks;
 };
-// Blocks of a clip: 4096 over the batch fill the card eight times over; a block walks 32 places at least, so that its sums cost
-// little beside its rows.
+// Blocks of a clip: 2048 over the batch, eight for each compute unit (4096 cost the joining kernels more than they gave the others);
+// a block walks 32 places at least, so that its sums cost little beside its rows.
 Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   Layout l{};
-  int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + 31) / 32, std::max<int64_t>(1, 4096 / std::max<int64_t>(1, B))));
+  int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + 31) / 32, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B))));
   l.rows = std::max<int64_t>(1, (S + n - 1) / n);
   l.blocks = (int32_t)std::max<int64_t>(1, (S + l.rows - 1) / l.rows);
   int64_t at = 0;
@@ -399,6 +402,8 @@ int run(const sed_norm_args* args, bool back, void* stream) {
   p.nv = (int32_t)(vec ? a.C / V : a.C);
   p.nb = std::min(p.nv, 256);
   if ((p.nv + p.nb - 1) / p.nb > 65535) return SED_ERR_CAPACITY;
+  p.half = 0;
+  for (int lanes = 256 / p.nb, h = 1; h < lanes; h *= 2) p.half = h;
   p.blocks = l.blocks;
   p.rows = l.rows;
   float* ws = static_cast<float*>(a.ws);

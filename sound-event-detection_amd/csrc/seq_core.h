@@ -84,12 +84,35 @@ __device__ __forceinline__ void store_n(T* p, int n, const float* in) {
 
 // ---- activations --------------------------------------------------------------------------------------------------------
 
-// act(u) and, where SLOPE, act'(u).
+// The normal distribution's integral up to u, and e = exp(-u^2 / 2).  With x = |u| / sqrt(2) the part beyond |u| is
+// exp(-x^2) erfcx(x) / 2; erfcx(x) is t P(t), t = 1 / (1 + 0.3 x), P a polynomial fitted for the least relative error on
+// 0 <= x <= 10 (iteratively weighted least squares; 4.6e-7 of the value at most as it is evaluated here), half of it taken into
+// the coefficients.  So the far tail keeps its digits, and the slope's exponential is the same one.
+__device__ __forceinline__ float normal_cdf(float u, float& e) {
+  e = exp2_hw(-0.5f * kLog2e * u * u);
+  const float t = rcp_hw(fmaf(0.3f * 0.70710678118654752440f, fabsf(u), 1.0f));
+  float p = 0.5f * -0.1295214593410492f;
+  p = fmaf(p, t, 0.5f * 0.4855561852455139f);
+  p = fmaf(p, t, 0.5f * -0.5122635364532471f);
+  p = fmaf(p, t, 0.5f * 0.547703206539154f);
+  p = fmaf(p, t, 0.5f * -0.09463890641927719f);
+  p = fmaf(p, t, 0.5f * 0.21492087841033936f);
+  p = fmaf(p, t, 0.5f * 0.14834055304527283f);
+  p = fmaf(p, t, 0.5f * 0.17071501910686493f);
+  p = fmaf(p, t, 0.5f * 0.1691880226135254f);
+  const float tail = p * t * e;
+  return u < 0.0f ? tail : 1.0f - tail;  // a NaN stays one through e
+}
+
+// act(u), act'(u)
 template <int ACT>
 __device__ __forceinline__ float act(float u) {
   if constexpr (ACT == SED_ACT_SILU) return u * sigmoid(u);
   if constexpr (ACT == SED_ACT_RELU) return u > 0.0f ? u : (u != u ? u : 0.0f);
-  if constexpr (ACT == SED_ACT_GELU) return u * (0.5f * erfcf(-0.70710678118654752440f * u));
+  if constexpr (ACT == SED_ACT_GELU) {
+    float e;
+    return u * normal_cdf(u, e);
+  }
   return u;
 }
 template <int ACT>
@@ -99,8 +122,11 @@ __device__ __forceinline__ float act_slope(float u) {
     return s * fmaf(u, 1.0f - s, 1.0f);
   }
   if constexpr (ACT == SED_ACT_RELU) return u > 0.0f ? 1.0f : 0.0f;
-  if constexpr (ACT == SED_ACT_GELU)
-    return fmaf(u * 0.39894228040143267794f, exp2_hw(-0.5f * kLog2e * u * u), 0.5f * erfcf(-0.70710678118654752440f * u));
+  if constexpr (ACT == SED_ACT_GELU) {
+    float e;
+    const float cdf = normal_cdf(u, e);
+    return fmaf(u * 0.39894228040143267794f, e, cdf);
+  }
   return 1.0f;
 }
 
