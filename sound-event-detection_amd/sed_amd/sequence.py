@@ -10,8 +10,6 @@ fp16); every output is rounded once.  There is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import torch
 
 from . import _lib as L
@@ -20,24 +18,33 @@ _DTYPES = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.float16: L.F16}
 _ACTIVATIONS = {None: L.ACT_NONE, "silu": L.ACT_SILU, "relu": L.ACT_RELU, "gelu": L.ACT_GELU}
 
 
+# The one-frame forms are called once per frame and layer, so what every call does on the host is kept short: argument structs
+# are filled by position, and a check looks at everything at once and finds out what is wrong only if something is.
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
 def _rows(t):
     """t with a contiguous last axis and rows at most 2^26 elements apart (views of a joint projection are read in place)."""
-    if t is None or ((t.stride(-1) == 1 or t.shape[-1] == 1) and (t.dim() < 3 or t.stride(1) <= 1 << 26)):
+    if t is None:
+        return t
+    st = t.stride()
+    if (st[-1] == 1 or t.shape[-1] == 1) and (len(st) < 3 or st[1] <= 1 << 26):
         return t
     return t.contiguous()
 
 
 def _param(t):
     """A parameter as the kernels read it; its gradient comes back in the parameter's own type."""
-    return None if t is None else t.float().contiguous()
+    if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
+        return t
+    return t.float().contiguous()
 
 
 def _check_x(what, x, dim):
-    if not torch.is_tensor(x) or not x.is_cuda:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise RuntimeError(f"{what}: x is on {getattr(x, 'device', type(x))}; the sequence operators run only on a ROCm device (no CPU path)")
     if x.dtype not in _DTYPES:
         raise TypeError(f"{what}: x is {x.dtype}; fp32, bf16 and fp16 are supported")
@@ -47,19 +54,18 @@ def _check_x(what, x, dim):
 
 def _check(what, name, t, x, shape, dtype=None):
     """t: a tensor of this shape on x's device, of x's type (dtype None), of one type, or of any floating type ('float')."""
-    if not torch.is_tensor(t) or t.device != x.device:
+    if isinstance(t, torch.Tensor) and t.shape == shape and t.device == x.device and (
+            t.is_floating_point() if dtype == "float" else t.dtype is (dtype or x.dtype)):
+        return
+    if not isinstance(t, torch.Tensor) or t.device != x.device:
         raise RuntimeError(f"{what}: {name} has to be a tensor on {x.device}")
-    if dtype == "float":
-        if not t.is_floating_point():
-            raise TypeError(f"{what}: {name} is {t.dtype}; a floating type is needed")
-    elif t.dtype != (dtype or x.dtype):
-        raise TypeError(f"{what}: {name} is {t.dtype}; {dtype or x.dtype} is needed")
     if tuple(t.shape) != tuple(shape):
         raise ValueError(f"{what}: {name} has shape {tuple(t.shape)}; {tuple(shape)} is needed")
+    raise TypeError(f"{what}: {name} is {t.dtype}; {'a floating type' if dtype == 'float' else dtype or x.dtype} is needed")
 
 
 def _check_frames(what, frames, x):
-    if frames is not None and not (torch.is_tensor(frames) and frames.device == x.device and frames.dtype == torch.int32 and
+    if frames is not None and not (isinstance(frames, torch.Tensor) and frames.device == x.device and frames.dtype == torch.int32 and
                                    frames.shape == (x.shape[0],) and frames.is_contiguous()):
         raise TypeError(f"{what}: frames: a contiguous int32 tensor with one entry per clip on x's device")
 
@@ -70,11 +76,12 @@ def _workspace(nbytes, dev):
 
 
 def _call(fn, args, dev, what):
+    stream = torch._C._cuda_getCurrentRawStream(dev.index)
     if torch.cuda.current_device() == dev.index:
-        L.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream), what)
+        L.check(fn(args, stream), what)
     else:
         with torch.cuda.device(dev):
-            L.check(fn(C.byref(args), torch.cuda.current_stream(dev).cuda_stream), what)
+            L.check(fn(args, stream), what)
 
 
 def _no_grad_only(what, *tensors):
@@ -90,20 +97,11 @@ def _wants_grad(*tensors):
 
 
 def _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state):
-    a = L.ScanArgs()
-    a.B, a.L, a.D = x.shape
-    a.G, a.N = B.shape[2], B.shape[3]
-    a.dtype, a.softplus, a.reverse = _DTYPES[x.dtype], int(softplus), int(reverse)
-    a.frames = _ptr(frames)
-    a.x, a.dt, a.z, a.Bm, a.Cm = x.data_ptr(), dt.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr()
-    a.x_b, a.x_t = x.stride(0), x.stride(1)
-    a.dt_b, a.dt_t = dt.stride(0), dt.stride(1)
-    if z is not None:
-        a.z_b, a.z_t = z.stride(0), z.stride(1)
-    a.Bm_b, a.Bm_t, a.Bm_g = B.stride()[:3]
-    a.Cm_b, a.Cm_t, a.Cm_g = Cm.stride()[:3]
-    a.A, a.skip, a.dt_bias, a.h0 = A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(state)
-    return a
+    b, n_frames, d = x.shape
+    xs, ds, zs, bs, cs = x.stride(), dt.stride(), (0, 0) if z is None else z.stride(), B.stride(), Cm.stride()
+    return L.ScanArgs(b, n_frames, d, A.shape[1], B.shape[2], _DTYPES[x.dtype], int(softplus), int(reverse), _ptr(frames),
+                      x.data_ptr(), dt.data_ptr(), _ptr(z), B.data_ptr(), Cm.data_ptr(), xs[0], xs[1], ds[0], ds[1], zs[0], zs[1],
+                      bs[0], bs[1], bs[2], cs[0], cs[1], cs[2], A.data_ptr(), _ptr(D), _ptr(dt_bias), _ptr(state))
 
 
 def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state, want_last, want_saved):
@@ -121,7 +119,7 @@ def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, sta
     if want_saved:
         saved = torch.empty(L.lib.sed_gated_scan_saved_floats(b, n_frames, d, n), dtype=torch.float32, device=dev)
         a.saved = saved.data_ptr()
-    nbytes = L.lib.sed_gated_scan_workspace(C.byref(a), 0)
+    nbytes = L.lib.sed_gated_scan_workspace(a, 0)
     if nbytes:
         ws = _workspace(nbytes, dev)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
@@ -162,7 +160,7 @@ class _GatedScan(torch.autograd.Function):
         a.dy, a.dy_b, a.dy_t, a.dh_last = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
         a.dx, a.ddt, a.dz, a.dB, a.dC = dx.data_ptr(), ddt.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
         a.dA, a.dskip, a.ddt_bias, a.dh0 = dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dstate)
-        nbytes = L.lib.sed_gated_scan_workspace(C.byref(a), 1)
+        nbytes = L.lib.sed_gated_scan_workspace(a, 1)
         ws = _workspace(nbytes, dev)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
         _call(L.lib.sed_gated_scan_backward, a, dev, "sed_gated_scan_backward")
@@ -242,18 +240,11 @@ def gated_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplu
         return y
     x, dt, z, B, C = (_rows(t) for t in (x, dt, z, B, C))
     A, D, dt_bias = _param(A), _param(D), _param(dt_bias)
-    a = L.ScanArgs()
-    a.B, a.D = x.shape
-    a.L, a.G, a.N = 1, g, n
-    a.dtype, a.softplus = _DTYPES[x.dtype], int(softplus)
-    a.x, a.dt, a.Bm, a.Cm, a.A = x.data_ptr(), dt.data_ptr(), B.data_ptr(), C.data_ptr(), A.data_ptr()
-    a.x_b, a.dt_b, a.Bm_b, a.Cm_b = x.stride(0), dt.stride(0), B.stride(0), C.stride(0)
-    if B.dim() == 3:
-        a.Bm_g, a.Cm_g = B.stride(1), C.stride(1)
-    if z is not None:
-        a.z, a.z_b = z.data_ptr(), z.stride(0)
-    a.skip, a.dt_bias = _ptr(D), _ptr(dt_bias)
-    a.y, a.h_last = y.data_ptr(), state.data_ptr()
+    bs, cs = B.stride(), C.stride()
+    wide = len(bs) == 3
+    a = L.ScanArgs(x.shape[0], 1, x.shape[1], n, g, _DTYPES[x.dtype], int(softplus), 0, None, x.data_ptr(), dt.data_ptr(), _ptr(z), B.data_ptr(),
+                   C.data_ptr(), x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, bs[0], 0, bs[1] if wide else 0, cs[0], 0,
+                   cs[1] if wide else 0, A.data_ptr(), _ptr(D), _ptr(dt_bias), None, state.data_ptr(), y.data_ptr())
     _call(L.lib.sed_gated_scan_step, a, x.device, "sed_gated_scan_step")
     return y
 
@@ -262,13 +253,10 @@ def gated_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplu
 
 
 def _conv_args(x, weight, bias, act, frames, reverse, state):
-    a = L.ConvArgs()
-    a.B, a.L, a.D = x.shape
-    a.W = weight.shape[1]
-    a.dtype, a.act, a.reverse = _DTYPES[x.dtype], act, int(reverse)
-    a.frames, a.x, a.x_b, a.x_t = _ptr(frames), x.data_ptr(), x.stride(0), x.stride(1)
-    a.weight, a.bias, a.state = weight.data_ptr(), _ptr(bias), _ptr(state)
-    return a
+    b, n_frames, d = x.shape
+    xs = x.stride()
+    return L.ConvArgs(b, n_frames, d, weight.shape[1], _DTYPES[x.dtype], act, int(reverse), _ptr(frames), x.data_ptr(), xs[0], xs[1],
+                      weight.data_ptr(), _ptr(bias), _ptr(state))
 
 
 def _conv_forward(x, weight, bias, act, frames, reverse, state, want_last):
@@ -370,12 +358,8 @@ def causal_conv_step(state, x, weight, bias=None, activation=None):
     if x.shape[0] == 0:
         return y
     x, weight, bias = _rows(x), _param(weight), _param(bias)
-    a = L.ConvArgs()
-    a.B, a.D = x.shape
-    a.L, a.W = 1, weight.shape[1]
-    a.dtype, a.act = _DTYPES[x.dtype], _ACTIVATIONS[activation]
-    a.x, a.x_b, a.weight, a.bias = x.data_ptr(), x.stride(0), weight.data_ptr(), _ptr(bias)
-    a.y, a.state_out = y.data_ptr(), _ptr(state)
+    a = L.ConvArgs(x.shape[0], 1, x.shape[1], weight.shape[1], _DTYPES[x.dtype], _ACTIVATIONS[activation], 0, None, x.data_ptr(), x.stride(0), 0,
+                   weight.data_ptr(), _ptr(bias), None, y.data_ptr(), _ptr(state))
     _call(L.lib.sed_causal_conv_step, a, x.device, "sed_causal_conv_step")
     return y
 
@@ -383,40 +367,42 @@ def causal_conv_step(state, x, weight, bias=None, activation=None):
 # ---- group norm ---------------------------------------------------------------------------------------------------------
 
 
-def _norm_args(x, shape, groups, weight, bias, act, eps, frames, mean, rstd):
-    a = L.NormArgs()
-    a.B, a.T, a.F, a.C = shape
-    a.G, a.dtype, a.act, a.eps = groups, _DTYPES[x.dtype], act, eps
-    a.frames, a.x, a.weight, a.bias = _ptr(frames), x.data_ptr(), _ptr(weight), _ptr(bias)
-    a.mean, a.rstd = mean.data_ptr(), rstd.data_ptr()
-    return a
+def _norm_args(x, shape, groups, weight, bias, act, eps, frames, stats, y, ws):
+    """stats: mean and rstd, one behind the other; ws: (bytes, tensor) of the workspace."""
+    at = stats.data_ptr()
+    return L.NormArgs(*shape, groups, _DTYPES[x.dtype], act, eps, _ptr(frames), x.data_ptr(), _ptr(weight), _ptr(bias), _ptr(y), at,
+                      at + 4 * shape[0] * groups, None, None, None, None, ws[1].data_ptr(), ws[0])
+
+
+def _norm_workspace(shape, groups, dev):
+    nbytes = L.lib.sed_group_norm_workspace(*shape, groups)
+    return nbytes, _workspace(nbytes, dev)
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, frames):
-    shape = (x.shape[0], x.shape[1], x[0, 0].numel() // x.shape[-1] if x.numel() else 1, x.shape[-1])
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = (torch.empty((shape[0], groups), dtype=torch.float32, device=x.device) for _ in range(2))
-    if x.numel():
-        a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, mean, rstd)
-        nbytes = L.lib.sed_group_norm_workspace(*shape, groups)
-        ws = _workspace(nbytes, x.device)
-        a.ws, a.ws_bytes, a.y = ws.data_ptr(), nbytes, y.data_ptr()
+    n = x.numel()
+    shape = (x.shape[0], x.shape[1], n // (x.shape[0] * x.shape[1] * x.shape[-1]) if n else 1, x.shape[-1])
+    y = torch.empty_like(x)
+    stats = torch.empty(2 * shape[0] * groups, dtype=torch.float32, device=x.device)
+    if n:
+        ws = _norm_workspace(shape, groups, x.device)  # held until the kernels are launched
+        a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, stats, y, ws)
         _call(L.lib.sed_group_norm_forward, a, x.device, "sed_group_norm_forward")
-    return y, mean, rstd, shape
+    return y, stats, shape
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act, frames):
-        y, mean, rstd, shape = _norm_forward(x, groups, weight, bias, eps, act, frames)
-        ctx.save_for_backward(x, weight, bias, frames, mean, rstd)
+        y, stats, shape = _norm_forward(x, groups, weight, bias, eps, act, frames)
+        ctx.save_for_backward(x, weight, bias, frames, stats)
         ctx.rest = (shape, groups, eps, act)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, bias, frames, mean, rstd = ctx.saved_tensors
+        x, weight, bias, frames, stats = ctx.saved_tensors
         shape, groups, eps, act = ctx.rest
         dx, dw, db = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, weight, bias))
         if x.numel() == 0:
@@ -425,11 +411,9 @@ class _GroupNormAct(torch.autograd.Function):
                     t.zero_()
             return dx, dw, db, None, None, None, None
         dy = dy.contiguous()
-        a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, mean, rstd)
+        ws = _norm_workspace(shape, groups, x.device)
+        a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, stats, None, ws)
         a.dy, a.dx, a.dw, a.db = dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
-        nbytes = L.lib.sed_group_norm_workspace(*shape, groups)
-        ws = _workspace(nbytes, x.device)
-        a.ws, a.ws_bytes = ws.data_ptr(), nbytes
         _call(L.lib.sed_group_norm_backward, a, x.device, "sed_group_norm_backward")
         return dx, dw, db, None, None, None, None
 
