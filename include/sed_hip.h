@@ -429,7 +429,7 @@ int sed_causal_conv_step(const sed_conv_args* args, void* stream);
 
 /* y = act((x - mean) * rstd * weight + bias), mean and biased variance over a clip's own frames, F and a group's channels. */
 typedef struct sed_norm_args {
-  int64_t B, T, F, C, G;    /* x is [B][T][F][C], C % G == 0, B <= 65535                           */
+  int64_t B, T, F, C, G;    /* x is [B][T][F][C], C % G == 0, B <= 65535, C <= 2^19                */
   int32_t dtype, act;
   float eps;
   const int32_t* frames;    /* [B] of T, or NULL                                                   */

@@ -128,37 +128,58 @@ __device__ __forceinline__ float block_sum(float v, float* s) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
-// mean and rstd of a (clip, group) out of the blocks' channels.
+// mean and rstd of a (clip, group) out of the blocks' channels: the mean first, then the squares about it, so that neither a far
+// mean nor an odd block costs digits.  HELD: each thread has at most HELD entries and keeps them; 0: they are read twice.
+template <int HELD>
 __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   __shared__ float s[4];
-  const int64_t g = blockIdx.x % a.G, b = blockIdx.x / a.G, cg = a.C / a.G, own = own_of(p, b);
-  const int64_t blocks = (own + p.rows - 1) / p.rows, n = blocks * cg;
+  const int g = blockIdx.x % (int)a.G, b = blockIdx.x / (int)a.G, cg = (int)(a.C / a.G);
+  const int64_t own = own_of(p, b);
+  const int n = (int)((own + p.rows - 1) / p.rows) * cg;  // entries
   const float total = (float)own * (float)cg;
-  const float* part = p.part + b * p.blocks * 2 * a.C + g * cg;
+  const float* part = p.part + (int64_t)b * p.blocks * 2 * a.C + g * cg;
   float mean = 0.0f, var = 0.0f;
   if (own > 0) {
-    // means relative to the first one: their spread is what counts
-    const float k = part[0];
-    float v = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-      const int64_t q = i / cg;
-      const float m = (float)(std::min<int64_t>((q + 1) * p.rows, own) - q * p.rows);
-      v = fmaf(m, part[q * 2 * a.C + i % cg] - k, v);
+    const auto entry = [&](int i, float& count, float& m, float& v) {
+      const int q = i / cg;
+      const float* at = part + (int64_t)q * 2 * a.C + (i - q * cg);
+      count = (float)(std::min<int64_t>((q + 1) * p.rows, own) - q * p.rows);
+      m = at[0];
+      v = at[a.C];
+    };
+    const float k = part[0];  // means relative to the first one: their spread is what counts
+    float w = 0.0f, count[HELD ? HELD : 1], m[HELD ? HELD : 1], v[HELD ? HELD : 1];
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) {
+        count[h] = m[h] = v[h] = 0.0f;
+        if ((int)threadIdx.x + 256 * h < n) entry(threadIdx.x + 256 * h, count[h], m[h], v[h]);
+      }
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) w = fmaf(count[h], m[h] - k, w);
+    } else {
+      for (int i = threadIdx.x; i < n; i += 256) {
+        entry(i, count[0], m[0], v[0]);
+        w = fmaf(count[0], m[0] - k, w);
+      }
     }
-    mean = k + block_sum(v, s) / total;
-    v = 0.0f;
-    for (int64_t i = threadIdx.x; i < n; i += 256) {
-      const int64_t q = i / cg;
-      const float m = (float)(std::min<int64_t>((q + 1) * p.rows, own) - q * p.rows);
-      const float e = part[q * 2 * a.C + i % cg] - mean;
-      v += fmaf(m * e, e, part[q * 2 * a.C + a.C + i % cg]);
+    mean = k + block_sum(w, s) / total;
+    w = 0.0f;
+    if constexpr (HELD > 0) {
+#pragma unroll
+      for (int h = 0; h < HELD; ++h) w += fmaf(count[h] * (m[h] - mean), m[h] - mean, v[h]);
+    } else {
+      for (int i = threadIdx.x; i < n; i += 256) {
+        entry(i, count[0], m[0], v[0]);
+        w += fmaf(count[0] * (m[0] - mean), m[0] - mean, v[0]);
+      }
     }
-    var = block_sum(v, s) / total;
+    var = block_sum(w, s) / total;
   }
   if (threadIdx.x == 0) {
-    a.mean[b * a.G + g] = mean;
-    a.rstd[b * a.G + g] = 1.0f / sqrtf(var + a.eps);
+    a.mean[(int64_t)b * a.G + g] = mean;
+    a.rstd[(int64_t)b * a.G + g] = 1.0f / sqrtf(var + a.eps);
   }
 }
 
@@ -252,33 +273,48 @@ __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p)
   }
 }
 
-// A clip's channels over its blocks, and the group's two means.
+// A clip's channels over its blocks, and the group's two means.  A channel has 256 / cg lanes, which take the blocks in
+// turn; their sums are added in order.
 __global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
-  __shared__ float s[4];
-  const int64_t g = blockIdx.x % a.G, b = blockIdx.x / a.G, cg = a.C / a.G, own = own_of(p, b);
+  __shared__ float s[4], s_1[256], s_2[256];
+  const int g = blockIdx.x % (int)a.G, b = blockIdx.x / (int)a.G, cg = (int)(a.C / a.G);
+  const int wide = std::min(cg, 256), lanes = 256 / wide, lane = threadIdx.x / wide, col = threadIdx.x % wide;
+  const int64_t own = own_of(p, b);
   const float total = (float)own * (float)cg;
   float q1 = 0.0f, q2 = 0.0f;
-  for (int64_t i = threadIdx.x; i < cg; i += 256) {
-    const int64_t c = g * cg + i;
-    const float* part = p.part + b * p.blocks * 2 * a.C + c;
+  for (int i = col; i - col < cg; i += wide) {
+    const int64_t c = (int64_t)g * cg + i;
     float s1 = 0.0f, s2 = 0.0f;
+    if (i < cg && lane < lanes) {
+      const float* part = p.part + (int64_t)b * p.blocks * 2 * a.C + c;
 #pragma unroll 4
-    for (int k = 0; k < p.blocks; ++k) {
-      s1 += part[(int64_t)k * 2 * a.C];
-      s2 += part[(int64_t)k * 2 * a.C + a.C];
+      for (int k = lane; k < p.blocks; k += lanes) {
+        s1 += part[(int64_t)k * 2 * a.C];
+        s2 += part[(int64_t)k * 2 * a.C + a.C];
+      }
     }
-    p.chan[b * 2 * a.C + c] = s1;
-    p.chan[b * 2 * a.C + a.C + c] = s2;
-    const float w = a.weight ? a.weight[c] : 1.0f;
-    q1 = fmaf(w, s1, q1);
-    q2 = fmaf(w, s2, q2);
+    __syncthreads();
+    s_1[threadIdx.x] = s1;
+    s_2[threadIdx.x] = s2;
+    __syncthreads();
+    if (i < cg && lane == 0) {
+      for (int k = 1; k < lanes; ++k) {
+        s1 += s_1[k * wide + col];
+        s2 += s_2[k * wide + col];
+      }
+      p.chan[(int64_t)b * 2 * a.C + c] = s1;
+      p.chan[(int64_t)b * 2 * a.C + a.C + c] = s2;
+      const float w = a.weight ? a.weight[c] : 1.0f;
+      q1 = fmaf(w, s1, q1);
+      q2 = fmaf(w, s2, q2);
+    }
   }
   q1 = block_sum(q1, s);
   q2 = block_sum(q2, s);
   if (threadIdx.x == 0) {
-    p.gsum[(b * a.G + g) * 2] = own > 0 ? q1 / total : 0.0f;
-    p.gsum[(b * a.G + g) * 2 + 1] = own > 0 ? q2 / total : 0.0f;
+    p.gsum[((int64_t)b * a.G + g) * 2] = own > 0 ? q1 / total : 0.0f;
+    p.gsum[((int64_t)b * a.G + g) * 2 + 1] = own > 0 ? q2 / total : 0.0f;
   }
 }
 
@@ -337,7 +373,7 @@ int check_args(const sed_norm_args* a) {
   if (a->dtype != SED_F32 && a->dtype != SED_BF16 && a->dtype != SED_F16) return SED_ERR_BAD_ARG;
   if (a->act < SED_ACT_NONE || a->act > SED_ACT_GELU) return SED_ERR_BAD_ARG;
   if (a->B > 0 && a->T > 0 && (!a->x || !a->mean || !a->rstd)) return SED_ERR_BAD_ARG;
-  if (a->B > 65535) return SED_ERR_CAPACITY;
+  if (a->B > 65535 || a->C > (1 << 19)) return SED_ERR_CAPACITY;
   return SED_OK;
 }
 
@@ -368,7 +404,10 @@ int launch(const NormParams& p, bool back, hipStream_t s) {
   const unsigned groups = (unsigned)(a.B * a.G);
   if (!back) {
     norm_stats_kernel<T, V, VEC><<<grid, 256, 0, s>>>(p);
-    norm_join_kernel<<<groups, 256, 0, s>>>(p);
+    if ((int64_t)p.blocks * (a.C / a.G) <= 8 * 256)
+      norm_join_kernel<8><<<groups, 256, 0, s>>>(p);
+    else
+      norm_join_kernel<0><<<groups, 256, 0, s>>>(p);
     norm_apply_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
   } else {
     norm_grad_sums_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);

@@ -41,6 +41,10 @@ struct ScanParams {
   float* part_d;    // [B * K][2][D]  d skip, d dt_bias
 };
 
+// Up to this many chunks every chunk forms the state in front of it from the ends of the others by itself, which is little work
+// and saves a launch; beyond, chunk_join_kernel does it once for all.
+constexpr int kOwnJoin = 32;
+
 // Tile geometry of one instance.
 template <int NS, int SPLIT>
 struct Geo {
@@ -308,6 +312,28 @@ __device__ __forceinline__ void only_own(const Where& w, int i0, int r, float (&
   for (int c = 0; c < 4; ++c) v[c] = in && (VEC ? w.nc > 0 : c < w.nc) ? v[c] : 0.0f;
 }
 
+// Chunks that have frames of a clip's own.
+template <class G>
+__device__ __forceinline__ int chunks_own(const ScanParams& p, int own) {
+  if (own <= 0) return 0;
+  int k = (int)((int64_t)((own - 1) / G::TT) * p.K / p.nt);
+  while (k < p.K && chunk_begin<G>(p, k) < own) ++k;
+  return k;
+}
+
+// The state behind chunk q from the state h in front of it, its end state from zero and its sum of delta.
+template <class G, int NS, bool VEC>
+__device__ __forceinline__ void pass_chunk(const ScanParams& p, const Where& w, int q, const float (&A2)[4][NS], float (&h)[4][NS]) {
+  const int64_t D = p.a.D, at = (int64_t)w.b * p.K + q;
+  float e[4][NS], s[4];
+  load_plane<NS, VEC>(p.chunk_h + at * G::NP * D, D, w, e);
+  per_channel(p.chunk_s + at * D, w, s);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int n = 0; n < NS; ++n) h[c][n] = fmaf(exp2_hw(A2[c][n] * s[c]), h[c][n], e[c][n]);
+}
+
 // Zero rows of the clip behind its own, this chunk's share of them.
 template <class G, class T, bool VEC>
 __device__ __forceinline__ void clear_rows(const ScanParams& p, const Where& w, void* base) {
@@ -364,15 +390,18 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
     for (int n = 0; n < NS; ++n) A2[c][n] *= kLog2e;
   per_channel(a.dt_bias, w, bias);
   per_channel(a.skip, w, skip);
-  if (!ENDS && p.K > 1) {
+  if (!ENDS && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
-  } else if (!ENDS && a.h0) {
-    load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
   } else {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
+    if (!ENDS && a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
+    if (!ENDS) {
+#pragma unroll 2
+      for (int q = 0; q < w.chunk; ++q) pass_chunk<G, NS, VEC>(p, w, q, A2, h);
+    }
   }
 
   for (int i0 = w.begin; i0 < w.end; i0 += G::TT) {
@@ -453,13 +482,13 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
 }
 
 // The states in front of the chunks, over the chunks in order (BACK: the gradients behind them, from the last).
-// In: every chunk's end state from zero; out, in its place: the state it starts from.  A block has 64 / SEG (channel, state)
+// In: every chunk's end state from zero; out, in its place: the state it starts from.  A block has 256 / SEG (channel, state)
 // pairs next to each other in memory and SEG lanes for each, which take a run of chunks: first the run's own end and sum, then
 // the runs in order (LDS), then the run again from its start, so that a long clip's chunks are not one long chain of loads.
-template <class G, bool BACK, int SEG>
+template <class G, bool BACK>
 __global__ void __launch_bounds__(256) chunk_join_kernel(const ScanParams p) {
   const sed_scan_args& a = p.a;
-  constexpr int NP = G::NP, W = 256 / SEG;
+  constexpr int NP = G::NP, SEG = 16, W = 256 / SEG;
   __shared__ float s_h[SEG][W], s_s[SEG][W];
   const int seg = threadIdx.x / W, lane = threadIdx.x % W;
   const int64_t i = (int64_t)blockIdx.x * W + lane;
@@ -467,11 +496,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ScanParams p) {
   const int64_t d = live ? i % a.D : 0, n = live ? i / a.D % NP : 0, b = live ? i / a.D / NP : 0;
   int own = (int)a.L;
   if (a.frames) own = std::max(0, std::min((int)a.L, a.frames[b]));
-  int k_own = 0;  // chunks with frames of the clip's own
-  if (own > 0) {
-    k_own = (int)((int64_t)((own - 1) / G::TT) * p.K / p.nt);
-    while (k_own < p.K && chunk_begin<G>(p, k_own) < own) ++k_own;
-  }
+  const int k_own = chunks_own<G>(p, own);
   const bool real = n < a.N;
   const float A2 = real ? a.A[d * a.N + n] * kLog2e : 0.0f;
   const float* first = BACK ? a.dh_last : a.h0;
@@ -480,7 +505,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ScanParams p) {
   const int per = (k_own + SEG - 1) / SEG, q0 = seg * per, q1 = live ? std::min(q0 + per, k_own) : 0;
   const auto at = [&](int q) { return (int64_t)(BACK ? k_own - 1 - q : q); };
   // the last chunk of the walk hands nothing on
-  if (SEG > 1) {
+  {
     float h = 0.0f, s = 0.0f;
 #pragma unroll 4
     for (int q = q0; q < std::min(q1, k_own - 1); ++q) {
@@ -609,10 +634,13 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : OCCB) scan_backward_kernel(cons
   }
   __syncthreads();
   // g: exp(delta_{t+1} A) g_{t+1}, what reaches frame t from behind
-  if (!ENDS && tiles && p.K > 1)
+  if (!ENDS && tiles && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
-  else if (!ENDS && a.dh_last && (tiles || w.own == 0))
-    load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
+  } else if (!ENDS && (tiles || w.own == 0)) {
+    if (a.dh_last) load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
+#pragma unroll 2
+    for (int q = chunks_own<G>(p, w.own) - 1; q > w.chunk; --q) pass_chunk<G, NS, VEC>(p, w, q, A2, g);
+  }
 
   // what the lane adds to dB and dC: one of its 2 NS sums, or none
   const int held = sum_index<2 * NS, G::J>(w.j), place = held < 0 ? -1 : held < NS ? w.s * NS + held : G::NP + w.s * NS + held - NS;
@@ -1050,11 +1078,9 @@ bool vector_rows(const sed_scan_args& a, bool back) {
 
 template <class G, bool BACK>
 void launch_join(const ScanParams& p, hipStream_t stream) {
+  if (p.K <= kOwnJoin) return;
   const int64_t n = p.a.B * G::NP * p.a.D;
-  if (p.K <= 16)
-    chunk_join_kernel<G, BACK, 1><<<(unsigned)((n + 255) / 256), 256, 0, stream>>>(p);
-  else
-    chunk_join_kernel<G, BACK, 16><<<(unsigned)((n + 15) / 16), 256, 0, stream>>>(p);
+  chunk_join_kernel<G, BACK><<<(unsigned)((n + 15) / 16), 256, 0, stream>>>(p);
 }
 
 template <int NS, int SPLIT, class T, bool VEC>
