@@ -22,15 +22,13 @@
 
 #include <algorithm>
 
-#ifndef OCCB
-#define OCCB 2
-#endif
 namespace sed {
 namespace {
 
 struct ScanParams {
   sed_scan_args a;
   int32_t nt;       // tiles of frames, ceil(L / TT)
+  int32_t ns;       // states kept of a clip, ceil(L / TS)
   int32_t four;     // N % 4 == 0 and A, h0, dh_last are aligned to 16 bytes
   int32_t K;        // chunks: chunk k has the tiles from k nt / K on
   int32_t tiles;    // channel tiles of a group
@@ -51,7 +49,8 @@ struct Geo {
   static constexpr int NP = NS * SPLIT;       // states, padded
   static constexpr int J = 64 / SPLIT;        // lanes along channels
   static constexpr int CW = 4 * J;            // channels of a wave
-  static constexpr int TT = SPLIT >= 4 ? 8 : 4;  // frames of a tile
+  static constexpr int TT = SPLIT == 16 ? 16 : SPLIT >= 4 ? 8 : 4;  // frames of a tile
+  static constexpr int TS = NP >= 8 ? 8 : 4;  // frames from one kept state to the next, whatever the tile
   static constexpr int TB = 4;                // frames whose states the gradient holds at a time: 16 NS <= 64 registers
   static constexpr int R = TT / SPLIT;        // rows a lane loads
   static constexpr int PB = (TT * NP + 63) / 64;
@@ -207,10 +206,12 @@ struct Step {
 template <int SPLIT>
 __device__ __forceinline__ void put_sums(const float (&v)[4], int s, float* at) {
   if constexpr (SPLIT >= 4) {
-    // rows of 16 lanes: halves of the wave first (channels 0 | 2 and 1 | 3), then neighbouring rows; with SPLIT = 8 the two
-    // halves of a row hold the same channel
-    const float u = fold16(fold32(v[0], v[2]), fold32(v[1], v[3]));
-    at[s / (SPLIT / 4)] = SPLIT == 8 ? u + dpp<kRor8>(u) : u;
+    // rows of 16 lanes: halves of the wave first (channels 0 | 2 and 1 | 3), then neighbouring rows; with SPLIT = 8 and 16 two
+    // and four groups of lanes in a row hold the same channel
+    float u = fold16(fold32(v[0], v[2]), fold32(v[1], v[3]));
+    if (SPLIT >= 8) u += dpp<kRor8>(u);
+    if (SPLIT >= 16) u += dpp<kRor4>(u);
+    at[s / (SPLIT / 4)] = u;
   } else if constexpr (SPLIT == 2) {
     *reinterpret_cast<f32x2*>(at + 2 * s) = f32x2{fold32(v[0], v[2]), fold32(v[1], v[3])};
   } else {
@@ -218,7 +219,12 @@ __device__ __forceinline__ void put_sums(const float (&v)[4], int s, float* at) 
   }
 }
 
+template <bool VEC = false>
 __device__ __forceinline__ void per_channel(const float* from, const Where& w, float (&v)[4]) {
+  if constexpr (VEC) {
+    get4(from + w.cl, v);
+    return;
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c) v[c] = from ? from[w.cl + (c < w.nc ? c : 0)] : 0.0f;
 }
@@ -321,17 +327,34 @@ __device__ __forceinline__ int chunks_own(const ScanParams& p, int own) {
   return k;
 }
 
-// The state behind chunk q from the state h in front of it, its end state from zero and its sum of delta.
+// The state behind `count` chunks from the state h in front of them (their end states from zero and sums of delta): chunks
+// q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.
 template <class G, int NS, bool VEC>
-__device__ __forceinline__ void pass_chunk(const ScanParams& p, const Where& w, int q, const float (&A2)[4][NS], float (&h)[4][NS]) {
-  const int64_t D = p.a.D, at = (int64_t)w.b * p.K + q;
+__device__ __forceinline__ void pass_chunks(const ScanParams& p, const Where& w, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
+  if (count <= 0) return;
+  const int64_t D = p.a.D;
   float e[4][NS], s[4];
-  load_plane<NS, VEC>(p.chunk_h + at * G::NP * D, D, w, e);
-  per_channel(p.chunk_s + at * D, w, s);
+  const auto load = [&](int i) {
+    const int64_t at = (int64_t)w.b * p.K + q + i * step;
+    load_plane<NS, VEC>(p.chunk_h + at * G::NP * D, D, w, e);
+    per_channel<VEC>(p.chunk_s + at * D, w, s);
+  };
+  load(0);
+#pragma unroll 2
+  for (int i = 0; i < count; ++i) {
+    float e1[4][NS], s1[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < 4; ++c) {
+      s1[c] = s[c];
 #pragma unroll
-    for (int n = 0; n < NS; ++n) h[c][n] = fmaf(exp2_hw(A2[c][n] * s[c]), h[c][n], e[c][n]);
+      for (int n = 0; n < NS; ++n) e1[c][n] = e[c][n];
+    }
+    if (i + 1 < count) load(i + 1);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < NS; ++n) h[c][n] = fmaf(exp2_hw(A2[c][n] * s1[c]), h[c][n], e1[c][n]);
+  }
 }
 
 // Zero rows of the clip behind its own, this chunk's share of them.
@@ -348,7 +371,7 @@ __device__ __forceinline__ void clear_rows(const ScanParams& p, const Where& w, 
 
 // ENDS: only the chunk's end state from zero and its sum of delta.  Otherwise the chunk's outputs.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(64, SPLIT == 1 ? 3 : 4) scan_forward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
   const Where w = where<G>(p);
@@ -398,10 +421,7 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
 #pragma unroll
       for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
     if (!ENDS && a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
-    if (!ENDS) {
-#pragma unroll 2
-      for (int q = 0; q < w.chunk; ++q) pass_chunk<G, NS, VEC>(p, w, q, A2, h);
-    }
+    if (!ENDS) pass_chunks<G, NS, VEC>(p, w, 0, 1, w.chunk, A2, h);
   }
 
   for (int i0 = w.begin; i0 < w.end; i0 += G::TT) {
@@ -425,7 +445,6 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
     put_states<G, T>(p, w, i0, bv, &s_B[0][0]);
     if (!ENDS) put_states<G, T>(p, w, i0, cv, &s_C[0][0]);
     if (i0 + G::TT < w.end) fetch(i0 + G::TT);
-    if (!ENDS && a.saved) store_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.nt + i0 / G::TT) * G::NP * a.D, a.D, w, h);
     __syncthreads();
 // a frame's values are read while the frame in front of it is worked on
     const int row = 4 * w.j, state = w.s * NS;
@@ -434,6 +453,8 @@ __global__ void __launch_bounds__(64, NS == 1 ? 3 : 4) scan_forward_kernel(const
 #pragma unroll
     for (int t = 0; t < G::TT; ++t) {
       const Step<NS>& q = f[t % 2];
+      if (!ENDS && a.saved && t % G::TS == 0 && i0 + t < w.own)
+        store_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.ns + (i0 + t) / G::TS) * G::NP * a.D, a.D, w, h);
       if (t + 1 < G::TT) f[(t + 1) % 2].template get<G, true, false, !ENDS>(row, state, t + 1, s_dl[0], s_dx[0], nullptr, s_B[0], s_C[0]);
       float y[4];
 #pragma unroll
@@ -576,7 +597,7 @@ __device__ __forceinline__ int sum_index(int j) {
 
 // ENDS: only the gradient that reaches the frame in front of the chunk from the chunk's own outputs, and the sum of delta.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64, ENDS ? 4 : OCCB) scan_backward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
   Where w = where<G>(p);
@@ -638,8 +659,8 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : OCCB) scan_backward_kernel(cons
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
   } else if (!ENDS && (tiles || w.own == 0)) {
     if (a.dh_last) load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
-#pragma unroll 2
-    for (int q = chunks_own<G>(p, w.own) - 1; q > w.chunk; --q) pass_chunk<G, NS, VEC>(p, w, q, A2, g);
+    const int last = chunks_own<G>(p, w.own) - 1;
+    pass_chunks<G, NS, VEC>(p, w, last, -1, last - w.chunk, A2, g);
   }
 
   // what the lane adds to dB and dC: one of its 2 NS sums, or none
@@ -649,7 +670,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : OCCB) scan_backward_kernel(cons
   // the state in front of a tile
   float h0[ENDS ? 1 : 4][NS];
   const auto plane = [&](int i0) {
-    if constexpr (!ENDS) load_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.nt + i0 / G::TT) * G::NP * a.D, a.D, w, h0);
+    if constexpr (!ENDS) load_plane<NS, VEC>(a.saved + ((int64_t)w.b * p.ns + i0 / G::TT) * G::NP * a.D, a.D, w, h0);
   };
   if (tiles) plane(w.begin + (tiles - 1) * G::TT);
 
@@ -980,30 +1001,31 @@ __global__ void __launch_bounds__(256) scan_step_kernel(const sed_scan_args a) {
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
-// Instance of a state count: NS states a lane, SPLIT lanes a channel.
-struct Shape { int NS, SPLIT, NP, CW, TT; };
-Shape shape_of(int N) {
-  if (N <= 1) return {1, 1, 1, 256, 4};
-  if (N <= 4) return {2, 2, 4, 128, 4};
-  if (N <= 8) return {2, 4, 8, 64, 8};
-#ifndef SH16
-#define SH16 4
-#endif
-  if (N <= 16) return {16 / SH16, SH16, 16, 256 / SH16, 8};
-  return {4, 8, 32, 32, 8};
+// Instance of a state count: NS states a lane, SPLIT lanes a channel.  The thin ones, for the forward pass, have four times the
+// waves with a quarter of the states each (two of eight at 3 and 4 states).
+struct Shape { int NS, SPLIT, NP, CW, TT, TS; };
+Shape shape_of(int N, bool thin) {
+  const auto make = [](int NS, int SPLIT) {
+    const int NP = NS * SPLIT;
+    return Shape{NS, SPLIT, NP, 256 / SPLIT, SPLIT == 16 ? 16 : SPLIT >= 4 ? 8 : 4, NP >= 8 ? 8 : 4};
+  };
+  if (N <= 1) return make(1, 1);
+  if (N <= 4) return thin ? make(1, 4) : make(2, 2);
+  if (N <= 8) return thin ? make(1, 8) : make(2, 4);
+  if (N <= 16) return thin ? make(1, 16) : make(4, 4);
+  return thin ? make(2, 16) : make(4, 8);
 }
 
-#ifndef SED_JOIN
-#define SED_JOIN 4.0
-#endif
 struct Layout {
-  int32_t K, tiles, nt;
+  bool thin;
+  int32_t K, tiles, nt, ns;
   int64_t h, s, bc, pa, pd, total;  // float offsets into the workspace
 };
 
-// Time of `waves` waves of `cost` each on 1024 vector units that hold `most` of them at once: waves share a unit's issue slots
-// (one alone gets 55 % of them, two 79 %, three 86 %, four 90 %, measured on multiply-adds), and a round is over with its last
-// wave.  Clips with lengths of their own: about half the chunks are empty, and the rest is spread as it comes.
+// Time of `waves` waves of `cost` issue slots each on 1024 vector units that hold `most` of them at once, in slots of a full
+// unit (4.4 cycles): waves share a unit's slots (one alone gets 55 % of them, two 79 %, three 86 %, four 90 %, measured on
+// multiply-adds), and a round is over with its last wave.  Clips with lengths of their own: about half the chunks are empty, and
+// the rest is spread as it comes.
 double pass_time(double waves, int most, double cost, bool ragged) {
   static const double together[] = {0.0, 1.82, 2.53, 3.49, 4.44};
   if (ragged) return cost * (0.55 * waves / 1024 * together[most] / most + 1.5 * together[1]);
@@ -1011,35 +1033,43 @@ double pass_time(double waves, int most, double cost, bool ragged) {
   return cost * (double)(n / most) * together[most] + cost * together[n % most];
 }
 
-// Chunks of a clip.  A chunk's frames are walked twice (for its end state, then for its outputs), so a clip stays whole where
-// there are waves enough; else the count that pass_time gives least for, in units of a forward tile: a wave's start costs two
-// tiles, the gradient's tile 3.4 of them, and joining the states two a chunk at most eight waves deep.
-int64_t chunks_of(const sed_scan_args& a, int64_t waves, int64_t nt, bool back) {
-  const double main = back ? 3.4 : 1.0, ends = back ? 0.8 : 0.72;
-  const int occ = back ? OCCB : 4;
-  double best = 0.0;
+// Chunks of a clip, and the time of the passes.  A chunk's frames are walked twice (for its end state, then for its outputs), so
+// a clip stays whole where there are waves enough; else the count that pass_time gives least for.  Slots of a frame: 6 a state
+// and 14 for its sums and loads, 5 and 8 without outputs, 26.5 a state in the gradient, 40 / SPLIT for forming its rows; of a
+// wave's start: 500 (mostly latency); of joining a chunk: 30 a state and 30; of a launch: 1100 (2 us).
+int64_t chunks_of(const sed_scan_args& a, const Shape& s, int64_t waves, int64_t nt, bool back, double& best) {
+  const int n = 4 * s.NS;
+  const double rows = 40.0 / s.SPLIT, main = s.TT * ((back ? 26.5 * n : 6.0 * n + 14) + rows), ends = s.TT * (5.0 * n + 8 + rows);
+  const int occ = back ? 2 : 4;
   int64_t K = 1;
   for (int64_t k = 1; k <= std::max<int64_t>(1, nt / 2) && (k == 1 || waves * k <= 16384); ++k) {
-    const double tiles = (double)((nt + k - 1) / k);
-    double t = pass_time((double)(waves * k), occ, tiles * main + 2.0, a.frames != nullptr);
-    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4, tiles * ends + 2.0, a.frames != nullptr) + SED_JOIN + (double)(waves * k) / 512;
+    const double tiles = (double)((nt + k - 1) / k), join = k > kOwnJoin ? 0.0 : (double)k * (7.5 * n + 30);
+    double t = pass_time((double)(waves * k), occ, tiles * main + 500 + join, a.frames != nullptr);
+    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4, tiles * ends + 500, a.frames != nullptr) + 1100;
+    if (k > kOwnJoin) t += 1100 + 2700;
     if (k == 1 || t < best) best = t, K = k;
   }
   return K;
 }
 
 Layout layout_of(const sed_scan_args& a, bool back) {
-  const Shape s = shape_of(a.N);
   Layout l{};
   const int64_t cg = a.D / a.G;
-  l.tiles = (int32_t)((cg + s.CW - 1) / s.CW);
-  l.nt = (int32_t)((a.L + s.TT - 1) / s.TT);
-#ifdef FK
-  const int64_t K = std::min<int64_t>(back ? BK : FK, std::max(1, l.nt / 2));
-#else
-  const int64_t K = chunks_of(a, a.B * a.G * l.tiles, l.nt, back);
+  Shape s{};
+  double best = 0.0;
+  for (const bool thin : {false, true}) {
+    if (thin && (back || a.N <= 1)) continue;
+    const Shape c = shape_of(a.N, thin);
+    const int32_t tiles = (int32_t)((cg + c.CW - 1) / c.CW), nt = (int32_t)((a.L + c.TT - 1) / c.TT);
+    double t;
+    const int64_t K = chunks_of(a, c, a.B * a.G * tiles, nt, back, t);
+#ifdef FORCE_THIN
+    if (thin != (FORCE_THIN != 0)) continue;
 #endif
-  l.K = (int32_t)K;
+    if (best == 0.0 || t < best) best = t, s = c, l.thin = thin, l.tiles = tiles, l.nt = nt, l.K = (int32_t)K;
+  }
+  l.ns = (int32_t)((a.L + s.TS - 1) / s.TS);
+  const int64_t K = l.K;
   int64_t at = 0;
   const auto take = [&](int64_t n) { const int64_t o = at; at += (n + 63) / 64 * 64; return o; };
   if (K > 1) {
@@ -1083,41 +1113,41 @@ void launch_join(const ScanParams& p, hipStream_t stream) {
   chunk_join_kernel<G, BACK><<<(unsigned)((n + 15) / 16), 256, 0, stream>>>(p);
 }
 
-template <int NS, int SPLIT, class T, bool VEC>
-int launch(const ScanParams& p, bool back, hipStream_t stream) {
+template <int NS, int SPLIT, class T, bool VEC, bool BACK>
+int launch(const ScanParams& p, hipStream_t stream) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
   const int64_t grid = a.B * p.K * a.G * p.tiles, joins = a.B * G::NP * a.D / 16;
   if (grid > 0x7fffffff || joins >= 0x7fffffff) return SED_ERR_CAPACITY;
-  if (!back) {
+  if constexpr (!BACK) {
     if (p.K > 1) {
       scan_forward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
       launch_join<G, false>(p, stream);
     }
     scan_forward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
-    return seq_status(hipGetLastError());
+  } else {
+    const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 63) / 64;
+    if (bc > 0x7fffffff) return SED_ERR_CAPACITY;
+    if (p.K > 1) {
+      scan_backward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
+      launch_join<G, true>(p, stream);
+    }
+    scan_backward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
+    scan_bc_kernel<T><<<(unsigned)bc, 256, 0, stream>>>(p, G::NP);
+    scan_param_kernel<<<(unsigned)pr, 1024, 0, stream>>>(p, G::NP);
   }
-  const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 63) / 64;
-  if (bc > 0x7fffffff) return SED_ERR_CAPACITY;
-  if (p.K > 1) {
-    scan_backward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
-    launch_join<G, true>(p, stream);
-  }
-  scan_backward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
-  scan_bc_kernel<T><<<(unsigned)bc, 256, 0, stream>>>(p, G::NP);
-  scan_param_kernel<<<(unsigned)pr, 1024, 0, stream>>>(p, G::NP);
   return seq_status(hipGetLastError());
 }
 
-template <int NS, int SPLIT, class T>
-int launch_v(const ScanParams& p, bool back, bool vec, hipStream_t s) {
-  return vec ? launch<NS, SPLIT, T, true>(p, back, s) : launch<NS, SPLIT, T, false>(p, back, s);
+template <int NS, int SPLIT, class T, bool BACK>
+int launch_v(const ScanParams& p, bool vec, hipStream_t s) {
+  return vec ? launch<NS, SPLIT, T, true, BACK>(p, s) : launch<NS, SPLIT, T, false, BACK>(p, s);
 }
-template <int NS, int SPLIT>
-int launch_t(const ScanParams& p, bool back, bool vec, hipStream_t s) {
-  if (p.a.dtype == SED_F32) return launch_v<NS, SPLIT, float>(p, back, vec, s);
-  if (p.a.dtype == SED_BF16) return launch_v<NS, SPLIT, bf16>(p, back, vec, s);
-  return launch_v<NS, SPLIT, f16>(p, back, vec, s);
+template <int NS, int SPLIT, bool BACK>
+int launch_t(const ScanParams& p, bool vec, hipStream_t s) {
+  if (p.a.dtype == SED_F32) return launch_v<NS, SPLIT, float, BACK>(p, vec, s);
+  if (p.a.dtype == SED_BF16) return launch_v<NS, SPLIT, bf16, BACK>(p, vec, s);
+  return launch_v<NS, SPLIT, f16, BACK>(p, vec, s);
 }
 
 int run(const sed_scan_args* args, bool back, void* stream) {
@@ -1128,6 +1158,7 @@ int run(const sed_scan_args* args, bool back, void* stream) {
   float* ws = static_cast<float*>(args->ws);
   p.K = l.K;
   p.nt = l.nt;
+  p.ns = l.ns;
   p.four = p.a.N % 4 == 0 && aligned(p.a.A, 16) && aligned(p.a.h0, 16) && aligned(p.a.dh_last, 16);
   p.tiles = l.tiles;
   p.chunk_h = ws + l.h;
@@ -1137,12 +1168,19 @@ int run(const sed_scan_args* args, bool back, void* stream) {
   p.part_d = ws + l.pd;
   const bool vec = vector_rows(p.a, back);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  const Shape sh = shape_of(p.a.N);
-  if (sh.NP == 1) return launch_t<1, 1>(p, back, vec, s);
-  if (sh.NP == 4) return launch_t<2, 2>(p, back, vec, s);
-  if (sh.NP == 8) return launch_t<2, 4>(p, back, vec, s);
-  if (sh.NP == 16) return launch_t<16 / SH16, SH16>(p, back, vec, s);
-  return launch_t<4, 8>(p, back, vec, s);
+  const int NP = shape_of(p.a.N, l.thin).NP;
+  if (back) {
+    if (NP == 1) return launch_t<1, 1, true>(p, vec, s);
+    if (NP == 4) return launch_t<2, 2, true>(p, vec, s);
+    if (NP == 8) return launch_t<2, 4, true>(p, vec, s);
+    if (NP == 16) return launch_t<4, 4, true>(p, vec, s);
+    return launch_t<4, 8, true>(p, vec, s);
+  }
+  if (NP == 1) return launch_t<1, 1, false>(p, vec, s);
+  if (NP == 4) return l.thin ? launch_t<1, 4, false>(p, vec, s) : launch_t<2, 2, false>(p, vec, s);
+  if (NP == 8) return l.thin ? launch_t<1, 8, false>(p, vec, s) : launch_t<2, 4, false>(p, vec, s);
+  if (NP == 16) return l.thin ? launch_t<1, 16, false>(p, vec, s) : launch_t<4, 4, false>(p, vec, s);
+  return l.thin ? launch_t<2, 16, false>(p, vec, s) : launch_t<4, 8, false>(p, vec, s);
 }
 
 template <class T>
@@ -1173,8 +1211,8 @@ int step(const sed_scan_args& a, hipStream_t s) {
 
 extern "C" int64_t sed_gated_scan_saved_floats(int64_t B, int64_t L, int64_t D, int32_t N) {
   if (B < 0 || L < 0 || D < 1 || N < 1 || N > 32) return SED_ERR_BAD_ARG;
-  const sed::Shape s = sed::shape_of(N);
-  return B * ((L + s.TT - 1) / s.TT) * s.NP * D;
+  const sed::Shape s = sed::shape_of(N, false);
+  return B * ((L + s.TS - 1) / s.TS) * s.NP * D;
 }
 
 extern "C" int64_t sed_gated_scan_workspace(const sed_scan_args* a, int32_t backward) {

@@ -146,7 +146,7 @@ template <int CTRL>
 __device__ __forceinline__ float dpp(float x) {
   return __uint_as_float(__builtin_amdgcn_update_dpp(0, __float_as_uint(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128;  // quad_perm [1,0,3,2], [2,3,0,1]; i -> 7 - i in eights; i -> i ^ 8
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kRor8 = 0x128, kRor4 = 0x124;  // quad_perm [1,0,3,2], [2,3,0,1]; i -> 7 - i in eights; i -> i ^ 8; i -> i - 4 in sixteens
 // Sum over the 16 lanes of a row, in every lane of it.
 __device__ __forceinline__ float row_sum(float x) {
   x += dpp<kXor1>(x);
