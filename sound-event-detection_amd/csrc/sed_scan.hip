@@ -5,7 +5,7 @@
 //   y_t[d]     = (sum_n C_t[g,n] h_t[d,n] + skip[d] x_t[d]) * silu(z_t[d])
 //
 // Bound: the vector unit.  A state takes one exp2 and four multiply-adds per frame and no matrix instruction helps, since the
-// decay differs per channel, state and frame.  So the layout serves the vector unit: one wave per workgroup, every lane holds
+// decay differs per channel, state and frame.  So the layout serves the vector unit: a wave works by itself, every lane holds
 // 4 channels x NS states in registers and walks along the frames, SPLIT lanes share a channel's NP = NS * SPLIT states.
 // B and C are then read from LDS once for 4 channels, the sum over states is NS multiply-adds and a few lane exchanges for 4
 // channels at once, and in the gradient the sum over channels is 4 multiply-adds in the lane before any exchange.
@@ -27,10 +27,9 @@ namespace {
 
 struct ScanParams {
   sed_scan_args a;
-  int32_t nt;       // tiles of frames, ceil(L / TT)
   int32_t ns;       // states kept of a clip, ceil(L / TS)
   int32_t four;     // N % 4 == 0 and A, h0, dh_last are aligned to 16 bytes
-  int32_t K;        // chunks: chunk k has the tiles from k nt / K on
+  int32_t K;        // chunks of a clip
   int32_t tiles;    // channel tiles of a group
   float* chunk_h;   // [B][K][NP][D]  end states from zero, then the states in front of the chunks
   float* chunk_s;   // [B][K][D]      sums of delta
@@ -42,6 +41,20 @@ struct ScanParams {
 // Up to this many chunks every chunk forms the state in front of it from the ends of the others by itself, which is little work
 // and saves a launch; beyond, chunk_join_kernel does it once for all.
 constexpr int kOwnJoin = 32;
+
+// Waves of a workgroup.  They work apart from each other (own LDS, no barrier): one workgroup to start for four of them (the
+// forward pass over 16 x 513 x 1536 x 16 takes 113 us so, 121 with one).  The gradient's fp32 tiles take 21 KB of LDS a wave: by
+// fours, only one workgroup would fit.
+template <class T, bool BACK, bool ENDS>
+constexpr int waves_of() { return BACK && !ENDS && sizeof(T) == 4 ? 1 : 4; }
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x / 64); }
+// What a wave's lanes wrote to LDS is there for its other lanes: a wave's LDS operations are carried out in order, so only the
+// compiler has to keep to it.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // Tile geometry of one instance.
 template <int NS, int SPLIT>
@@ -68,31 +81,35 @@ struct Where {
   int flip;        // TT - 1 where the walk goes to earlier rows
 };
 
+// First frame of a clip's chunk k < K: its own tiles in K even parts, so that clips of other lengths have other chunks, but none
+// begins behind the clip's own frames (a clip of fewer than K tiles has empty ones).  Behind the last one: the end.
 template <class G>
-__device__ __forceinline__ int chunk_begin(const ScanParams& p, int k) { return (int)((int64_t)k * p.nt / p.K) * G::TT; }
+__device__ __forceinline__ int chunk_begin(const ScanParams& p, int own, int k) {
+  return std::min((int)((int64_t)k * ((own + G::TT - 1) / G::TT) / p.K) * G::TT, own);
+}
 
-template <class G>
+template <class G, int WAVES>
 __device__ __forceinline__ Where where(const ScanParams& p) {
   Where w;
   const sed_scan_args& a = p.a;
   const unsigned all = p.tiles * a.G;
-  unsigned i = blockIdx.x;
+  unsigned i = blockIdx.x * WAVES + wave_id();
   w.tile = i % all;
   i /= all;
   w.chunk = i % p.K;
-  w.b = i / p.K;
+  w.b = i / p.K;  // B or more in the last workgroup's spare waves, which leave at once
   w.g = w.tile / p.tiles;
   w.flip = a.reverse ? G::TT - 1 : 0;
-  w.s = threadIdx.x / G::J;
+  w.s = threadIdx.x % 64 / G::J;
   w.j = threadIdx.x % G::J;
   const int cg = (int)a.D / a.G, in = (w.tile % p.tiles) * G::CW + 4 * w.j;
   w.c0 = w.g * cg + in;
   w.nc = std::max(0, std::min(4, cg - in));
   w.cl = w.nc ? w.c0 : w.g * cg;
   w.own = (int)a.L;
-  if (a.frames) w.own = std::max(0, std::min((int)a.L, a.frames[w.b]));
-  w.begin = chunk_begin<G>(p, w.chunk);
-  w.end = std::min(chunk_begin<G>(p, w.chunk + 1), w.own);
+  if (a.frames) w.own = std::max(0, std::min((int)a.L, a.frames[std::min<int64_t>(w.b, a.B - 1)]));
+  w.begin = chunk_begin<G>(p, w.own, w.chunk);
+  w.end = chunk_begin<G>(p, w.own, w.chunk + 1);
   return w;
 }
 
@@ -318,15 +335,6 @@ __device__ __forceinline__ void only_own(const Where& w, int i0, int r, float (&
   for (int c = 0; c < 4; ++c) v[c] = in && (VEC ? w.nc > 0 : c < w.nc) ? v[c] : 0.0f;
 }
 
-// Chunks that have frames of a clip's own.
-template <class G>
-__device__ __forceinline__ int chunks_own(const ScanParams& p, int own) {
-  if (own <= 0) return 0;
-  int k = (int)((int64_t)((own - 1) / G::TT) * p.K / p.nt);
-  while (k < p.K && chunk_begin<G>(p, k) < own) ++k;
-  return k;
-}
-
 // The state behind `count` chunks from the state h in front of them (their end states from zero and sums of delta): chunks
 // q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.
 template <class G, int NS, bool VEC>
@@ -361,8 +369,9 @@ __device__ __forceinline__ void pass_chunks(const ScanParams& p, const Where& w,
 template <class G, class T, bool VEC>
 __device__ __forceinline__ void clear_rows(const ScanParams& p, const Where& w, void* base) {
   const float zero[4] = {0, 0, 0, 0};
-  const int stop = std::min(chunk_begin<G>(p, w.chunk + 1), (int)p.a.L);
-  for (int i = std::max(w.begin, w.own) + w.s; i < stop; i += 64 / G::J)
+  const int64_t behind = p.a.L - w.own;
+  const int stop = w.own + (int)(behind * (w.chunk + 1) / p.K);
+  for (int i = w.own + (int)(behind * w.chunk / p.K) + w.s; i < stop; i += 64 / G::J)
     store_n<T, 4, VEC>(static_cast<T*>(base) + ((int64_t)w.b * p.a.L + i) * p.a.D + w.c0, w.nc, zero);
 }
 
@@ -371,17 +380,25 @@ __device__ __forceinline__ void clear_rows(const ScanParams& p, const Where& w, 
 
 // ENDS: only the chunk's end state from zero and its sum of delta.  Otherwise the chunk's outputs.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64, SPLIT == 1 ? 3 : 4) scan_forward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (SPLIT == 1 ? 3 : 4)) scan_forward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
+  constexpr int W = waves_of<T, false, ENDS>();
   const sed_scan_args& a = p.a;
-  const Where w = where<G>(p);
-  __shared__ __attribute__((aligned(16))) float s_dl[G::TT][G::CW], s_dx[G::TT][G::CW], s_y[ENDS ? 1 : G::TT][G::CW];
-  __shared__ __attribute__((aligned(16))) float s_B[G::TT][G::NP], s_C[G::TT][G::NP];
-  if (ENDS && (w.chunk == p.K - 1 || w.begin >= w.own)) return;  // chunk_join_kernel reads no such chunk
+  const Where w = where<G, W>(p);
+  struct Shared {
+    float dl[G::TT][G::CW], dx[G::TT][G::CW], y[ENDS ? 1 : G::TT][G::CW], B[G::TT][G::NP], C[G::TT][G::NP];
+  };
+  __shared__ __attribute__((aligned(16))) Shared shared[W];
+  Shared& sh = shared[wave_id()];
+  auto &s_dl = sh.dl, &s_dx = sh.dx;
+  auto &s_y = sh.y;
+  auto &s_B = sh.B, &s_C = sh.C;
+  if (w.b >= a.B) return;
+  if (ENDS && (w.chunk == p.K - 1 || w.own == 0)) return;  // nothing comes behind it
   if (!ENDS) {
     clear_rows<G, T, VEC>(p, w, a.y);
-    if (w.begin >= w.own) {
-      if (a.h_last && w.own == 0 && w.chunk == 0) {
+    if (w.own == 0) {
+      if (a.h_last && w.chunk == 0) {
         float h[4][NS] = {};
         if (a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
         store_dn<NS>(a.h_last + (int64_t)w.b * a.D * a.N, a.N, w, h);
@@ -445,7 +462,7 @@ __global__ void __launch_bounds__(64, SPLIT == 1 ? 3 : 4) scan_forward_kernel(co
     put_states<G, T>(p, w, i0, bv, &s_B[0][0]);
     if (!ENDS) put_states<G, T>(p, w, i0, cv, &s_C[0][0]);
     if (i0 + G::TT < w.end) fetch(i0 + G::TT);
-    __syncthreads();
+    wave_sync();
 // a frame's values are read while the frame in front of it is worked on
     const int row = 4 * w.j, state = w.s * NS;
     Step<NS> f[2];
@@ -469,7 +486,7 @@ __global__ void __launch_bounds__(64, SPLIT == 1 ? 3 : 4) scan_forward_kernel(co
       if (!ENDS) put_sums<SPLIT>(y, w.s, &s_y[t][4 * w.j]);
       __builtin_amdgcn_sched_barrier(0);
     }
-    __syncthreads();
+    wave_sync();
     if (!ENDS) {
 #pragma unroll
       for (int r = 0; r < G::R; ++r) {
@@ -483,21 +500,21 @@ __global__ void __launch_bounds__(64, SPLIT == 1 ? 3 : 4) scan_forward_kernel(co
         }
         store_row<G, T, VEC>(ry, w, i0, r, y);
       }
-      __syncthreads();
+      wave_sync();
     }
   }
   if (ENDS) {
     store_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
     // every lane of a channel summed its own rows
-    __syncthreads();
+    wave_sync();
     put_sums<SPLIT>(sum, w.s, &s_dl[0][4 * w.j]);
-    __syncthreads();
+    wave_sync();
     if (w.s == 0) {
       float v[4];
       get4(&s_dl[0][4 * w.j], v);
       store_n<float, 4, VEC>(p.chunk_s + ((int64_t)w.b * p.K + w.chunk) * a.D + w.c0, w.nc, v);
     }
-  } else if (a.h_last && w.end == w.own) {
+  } else if (a.h_last && w.chunk == p.K - 1) {
     store_dn<NS>(a.h_last + (int64_t)w.b * a.D * a.N, a.N, w, h);
   }
 }
@@ -517,7 +534,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const ScanParams p) {
   const int64_t d = live ? i % a.D : 0, n = live ? i / a.D % NP : 0, b = live ? i / a.D / NP : 0;
   int own = (int)a.L;
   if (a.frames) own = std::max(0, std::min((int)a.L, a.frames[b]));
-  const int k_own = chunks_own<G>(p, own);
+  const int k_own = own > 0 ? p.K : 0;
   const bool real = n < a.N;
   const float A2 = real ? a.A[d * a.N + n] * kLog2e : 0.0f;
   const float* first = BACK ? a.dh_last : a.h0;
@@ -597,20 +614,31 @@ __device__ __forceinline__ int sum_index(int j) {
 
 // ENDS: only the gradient that reaches the frame in front of the chunk from the chunk's own outputs, and the sum of delta.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 2)) scan_backward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
+  constexpr int W = waves_of<T, true, ENDS>();
   const sed_scan_args& a = p.a;
-  Where w = where<G>(p);
+  Where w = where<G, W>(p);
   constexpr int TX = ENDS ? 1 : G::TT, TB = G::TB;
   constexpr bool EARLY = NS <= 2;  // dC is summed while the states are formed: a multiply-add less, TB * NS registers more
-  // a row's gy and dx make room for the sums S2 and S1 that its frame leaves behind
-  __shared__ __attribute__((aligned(16))) float s_dl[G::TT][G::CW], s_gy[G::TT][G::CW], s_dx[TX][G::CW], s_y[TX][G::CW];
-  __shared__ __attribute__((aligned(16))) float s_B[G::TT][G::NP], s_C[G::TT][G::NP];
-  // the tile's rows and the state in front of it, each lane its own: registers are short
-  __shared__ __attribute__((aligned(16))) T4<T> s_raw[ENDS ? 1 : 4][ENDS ? 1 : G::R][64];
-  __shared__ __attribute__((aligned(16))) float s_h[ENDS ? 1 : NS][ENDS ? 4 : 256], s_ch[2][G::CW];
+  // a row's gy and dx make room for the sums S2 and S1 that its frame leaves behind; raw, h: the tile's rows and the state in
+  // front of it, each lane its own (registers are short); ch: dt_bias and skip
+  struct Shared {
+    float dl[G::TT][G::CW], gy[G::TT][G::CW], dx[TX][G::CW], y[TX][G::CW], B[G::TT][G::NP], C[G::TT][G::NP];
+    T4<T> raw[ENDS ? 1 : 4][ENDS ? 1 : G::R][64];
+    float h[ENDS ? 1 : NS][ENDS ? 4 : 256], ch[2][G::CW];
+  };
+  __shared__ __attribute__((aligned(16))) Shared shared[W];
+  Shared& sh = shared[wave_id()];
+  auto &s_dl = sh.dl, &s_gy = sh.gy;
+  auto &s_dx = sh.dx, &s_y = sh.y;
+  auto &s_B = sh.B, &s_C = sh.C;
+  auto& s_raw = sh.raw;
+  auto& s_h = sh.h;
+  auto& s_ch = sh.ch;
+  if (w.b >= a.B) return;
   float(&s_1)[TX][G::CW] = s_dx;
-  if (ENDS && (w.chunk == 0 || w.begin >= w.own)) return;
+  if (ENDS && (w.chunk == 0 || w.own == 0)) return;
 
   // rows behind the clip's own have no gradient
   if (!ENDS) {
@@ -653,14 +681,13 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
     per_channel(a.skip, w, v);
     put4(v, &s_ch[1][4 * w.j]);
   }
-  __syncthreads();
+  wave_sync();
   // g: exp(delta_{t+1} A) g_{t+1}, what reaches frame t from behind
-  if (!ENDS && tiles && p.K > kOwnJoin) {
+  if (!ENDS && w.own > 0 && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
-  } else if (!ENDS && (tiles || w.own == 0)) {
+  } else if (!ENDS) {
     if (a.dh_last) load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
-    const int last = chunks_own<G>(p, w.own) - 1;
-    pass_chunks<G, NS, VEC>(p, w, last, -1, last - w.chunk, A2, g);
+    if (w.own > 0) pass_chunks<G, NS, VEC>(p, w, p.K - 1, -1, p.K - 1 - w.chunk, A2, g);
   }
 
   // what the lane adds to dB and dC: one of its 2 NS sums, or none
@@ -720,7 +747,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
     put_states<G, T>(p, w, i0, cv, &s_C[0][0]);
     if (!ENDS) put_states<G, T>(p, w, i0, bv, &s_B[0][0]);
     if (k) fetch(i0 - G::TT);
-    __syncthreads();
+    wave_sync();
     int row = 4 * w.j, state = w.s * NS;
     Step<NS> f[2];
     if constexpr (ENDS) {
@@ -819,7 +846,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
         }
       }
     }
-    __syncthreads();
+    wave_sync();
     if constexpr (!ENDS) {
       float bias[4], skip[4];
       get4(&s_ch[0][4 * w.j], bias);
@@ -864,14 +891,14 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
           store_row<G, T, VEC>(wdt, w, i0, r, v);
         }
       }
-      __syncthreads();
+      wave_sync();
     }
   }
-  __syncthreads();
+  wave_sync();
   if (ENDS) {
     store_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
     put_sums<SPLIT>(sum, w.s, &s_dl[0][4 * w.j]);
-    __syncthreads();
+    wave_sync();
     if (w.s == 0) {
       float v[4];
       get4(&s_dl[0][4 * w.j], v);
@@ -883,7 +910,7 @@ __global__ void __launch_bounds__(64, ENDS ? 4 : 2) scan_backward_kernel(const S
   store_plane<NS, VEC>(p.part_a + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, dA);
   put_sums<SPLIT>(dskip, w.s, &s_1[0][4 * w.j]);
   put_sums<SPLIT>(dbias, w.s, &s_gy[0][4 * w.j]);
-  __syncthreads();
+  wave_sync();
   if (w.s == 0) {
     float u[4], v[4];
     get4(&s_1[0][4 * w.j], u);
@@ -1063,9 +1090,6 @@ Layout layout_of(const sed_scan_args& a, bool back) {
     const int32_t tiles = (int32_t)((cg + c.CW - 1) / c.CW), nt = (int32_t)((a.L + c.TT - 1) / c.TT);
     double t;
     const int64_t K = chunks_of(a, c, a.B * a.G * tiles, nt, back, t);
-#ifdef FORCE_THIN
-    if (thin != (FORCE_THIN != 0)) continue;
-#endif
     if (best == 0.0 || t < best) best = t, s = c, l.thin = thin, l.tiles = tiles, l.nt = nt, l.K = (int32_t)K;
   }
   l.ns = (int32_t)((a.L + s.TS - 1) / s.TS);
@@ -1117,22 +1141,24 @@ template <int NS, int SPLIT, class T, bool VEC, bool BACK>
 int launch(const ScanParams& p, hipStream_t stream) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
-  const int64_t grid = a.B * p.K * a.G * p.tiles, joins = a.B * G::NP * a.D / 16;
-  if (grid > 0x7fffffff || joins >= 0x7fffffff) return SED_ERR_CAPACITY;
+  const int64_t waves = a.B * p.K * a.G * p.tiles, joins = a.B * G::NP * a.D / 16;
+  if (waves > 0x7fffffff || joins >= 0x7fffffff) return SED_ERR_CAPACITY;
+  constexpr int WE = waves_of<T, BACK, true>(), WM = waves_of<T, BACK, false>();  // of the ends, of the main pass
+  const unsigned ends = (unsigned)((waves + WE - 1) / WE), main = (unsigned)((waves + WM - 1) / WM);
   if constexpr (!BACK) {
     if (p.K > 1) {
-      scan_forward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
+      scan_forward_kernel<NS, SPLIT, T, VEC, true><<<ends, 64 * WE, 0, stream>>>(p);
       launch_join<G, false>(p, stream);
     }
-    scan_forward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
+    scan_forward_kernel<NS, SPLIT, T, VEC, false><<<main, 64 * WM, 0, stream>>>(p);
   } else {
     const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 63) / 64;
     if (bc > 0x7fffffff) return SED_ERR_CAPACITY;
     if (p.K > 1) {
-      scan_backward_kernel<NS, SPLIT, T, VEC, true><<<(unsigned)grid, 64, 0, stream>>>(p);
+      scan_backward_kernel<NS, SPLIT, T, VEC, true><<<ends, 64 * WE, 0, stream>>>(p);
       launch_join<G, true>(p, stream);
     }
-    scan_backward_kernel<NS, SPLIT, T, VEC, false><<<(unsigned)grid, 64, 0, stream>>>(p);
+    scan_backward_kernel<NS, SPLIT, T, VEC, false><<<main, 64 * WM, 0, stream>>>(p);
     scan_bc_kernel<T><<<(unsigned)bc, 256, 0, stream>>>(p, G::NP);
     scan_param_kernel<<<(unsigned)pr, 1024, 0, stream>>>(p, G::NP);
   }
@@ -1157,7 +1183,6 @@ int run(const sed_scan_args* args, bool back, void* stream) {
   if (l.total > 0 && (!args->ws || args->ws_bytes < l.total * 4 || !aligned(args->ws, 16))) return SED_ERR_CAPACITY;
   float* ws = static_cast<float*>(args->ws);
   p.K = l.K;
-  p.nt = l.nt;
   p.ns = l.ns;
   p.four = p.a.N % 4 == 0 && aligned(p.a.A, 16) && aligned(p.a.h0, 16) && aligned(p.a.dh_last, 16);
   p.tiles = l.tiles;
