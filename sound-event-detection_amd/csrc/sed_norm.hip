@@ -183,19 +183,28 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
   }
 }
 
+// Calls f(channel of the lane, its group) for the lane's V channels in order.
+template <int V, class F>
+__device__ __forceinline__ void each_group(const NormParams& p, const Cell& q, F f) {
+  const int cg = (int)(p.a.C / p.a.G);
+  int g = (int)q.c / cg, left = cg - ((int)q.c - g * cg);
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    f(c, q.b * p.a.G + g);
+    if (--left == 0) ++g, left = cg;
+  }
+}
+
 // mean, scale and shift of a lane's channels: n = (x - mean) rstd, u = n w + bias.
 template <int V>
 __device__ __forceinline__ void channels(const NormParams& p, const Cell& q, float (&mean)[V], float (&rstd)[V], float (&w)[V], float (&bias)[V]) {
   const sed_norm_args& a = p.a;
-  const int64_t cg = a.C / a.G;
-#pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int64_t g = (q.c + c) / cg;
-    mean[c] = a.mean[q.b * a.G + g];
-    rstd[c] = a.rstd[q.b * a.G + g];
+  each_group<V>(p, q, [&](int c, int64_t g) {
+    mean[c] = a.mean[g];
+    rstd[c] = a.rstd[g];
     w[c] = a.weight ? a.weight[q.c + c] : 1.0f;
     bias[c] = a.bias ? a.bias[q.c + c] : 0.0f;
-  }
+  });
 }
 
 template <class T, int V, bool VEC, int ACT>
@@ -211,14 +220,18 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
   const int64_t at = q.b * p.S * a.C + q.c;
   const T* x = static_cast<const T*>(a.x) + at;
   T* y = static_cast<T*>(a.y) + at;
+  const int64_t end = std::min<int64_t>(q.r1, own);
+  int64_t r = q.r0 + q.ty;
 #pragma unroll 4
-  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
+  for (; r < end; r += q.step) {
     float v[V];
-    load_n<T, V, VEC>(x + r * a.C, r < own ? V : 0, v);
+    load_n<T, V, VEC>(x + r * a.C, V, v);
 #pragma unroll
-    for (int c = 0; c < V; ++c) v[c] = r < own ? act<ACT>(fmaf(v[c] - mean[c], w[c], bias[c])) : 0.0f;
+    for (int c = 0; c < V; ++c) v[c] = act<ACT>(fmaf(v[c] - mean[c], w[c], bias[c]));
     store_n<T, V, VEC>(y + r * a.C, V, v);
   }
+  const float zero[V] = {};
+  for (; r < q.r1; r += q.step) store_n<T, V, VEC>(y + r * a.C, V, zero);
 }
 
 template <class T, int V, bool VEC, int ACT>
@@ -338,30 +351,32 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   const Cell q = cell<V, true>(p);
   if (!q.in) return;
-  const int64_t own = own_of(p, q.b), cg = a.C / a.G;
+  const int64_t own = own_of(p, q.b);
   float mean[V], rstd[V], w[V], bias[V], m1[V], m2[V];
   channels<V>(p, q, mean, rstd, w, bias);
-#pragma unroll
-  for (int c = 0; c < V; ++c) {
-    const int64_t g = (q.c + c) / cg;
-    m1[c] = p.gsum[(q.b * a.G + g) * 2];
-    m2[c] = p.gsum[(q.b * a.G + g) * 2 + 1];
-  }
+  each_group<V>(p, q, [&](int c, int64_t g) {
+    m1[c] = p.gsum[g * 2];
+    m2[c] = p.gsum[g * 2 + 1];
+  });
   const int64_t at = q.b * p.S * a.C + q.c;
   const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
   T* dx = static_cast<T*>(a.dx) + at;
+  const int64_t end = std::min<int64_t>(q.r1, own);
+  int64_t r = q.r0 + q.ty;
 #pragma unroll 4
-  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
+  for (; r < end; r += q.step) {
     float v[V], g[V];
-    load_n<T, V, VEC>(x + r * a.C, r < own ? V : 0, v);
-    load_n<T, V, VEC>(dy + r * a.C, r < own ? V : 0, g);
+    load_n<T, V, VEC>(x + r * a.C, V, v);
+    load_n<T, V, VEC>(dy + r * a.C, V, g);
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const float n = (v[c] - mean[c]) * rstd[c], qv = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c])) * w[c];
-      v[c] = r < own ? rstd[c] * (qv - fmaf(n, m2[c], m1[c])) : 0.0f;
+      v[c] = rstd[c] * (qv - fmaf(n, m2[c], m1[c]));
     }
     store_n<T, V, VEC>(dx + r * a.C, V, v);
   }
+  const float zero[V] = {};
+  for (; r < q.r1; r += q.step) store_n<T, V, VEC>(dx + r * a.C, V, zero);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -401,18 +416,18 @@ template <class T, int V, bool VEC, int ACT>
 int launch(const NormParams& p, bool back, hipStream_t s) {
   const sed_norm_args& a = p.a;
   const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb));
-  const unsigned groups = (unsigned)(a.B * a.G);
+  const unsigned groups = (unsigned)(a.B * a.G), threads = (unsigned)((256 / p.nb * p.nb + 63) / 64 * 64);
   if (!back) {
-    norm_stats_kernel<T, V, VEC><<<grid, 256, 0, s>>>(p);
+    norm_stats_kernel<T, V, VEC><<<grid, threads, 0, s>>>(p);
     if ((int64_t)p.blocks * (a.C / a.G) <= 8 * 256)
       norm_join_kernel<8><<<groups, 256, 0, s>>>(p);
     else
       norm_join_kernel<0><<<groups, 256, 0, s>>>(p);
-    norm_apply_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
+    norm_apply_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
   } else {
-    norm_grad_sums_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
+    norm_grad_sums_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
     norm_grad_join_kernel<<<groups, 256, 0, s>>>(p);
-    norm_grad_kernel<T, V, VEC, ACT><<<grid, 256, 0, s>>>(p);
+    norm_grad_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
     if (a.dw || a.db) norm_param_kernel<<<(unsigned)((2 * a.C + 255) / 256), 256, 0, s>>>(p);
   }
   return seq_status(hipGetLastError());
