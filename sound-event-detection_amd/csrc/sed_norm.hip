@@ -20,7 +20,6 @@ struct NormParams {
   int32_t nv, nb;    // vectors of a row, lanes along a row
   int32_t half;      // half the lanes of a channel, rounded up to a power of two
   int32_t blocks;    // blocks a clip is cut into
-  int64_t rows;      // places of a block
   float* part;       // [B][blocks][2][C]: (mean, sum of squares about it), or (sum du, sum du n)
   float* chan;       // [B][2][C]
   float* gsum;       // [B][G][2]: means of q and q n
@@ -32,8 +31,14 @@ __device__ __forceinline__ int64_t own_of(const NormParams& p, int64_t b) {
   return t * a.F;
 }
 
+// First of a clip's n places that block k of its `blocks` takes: even parts, so that clips of other lengths keep every block (and
+// every compute unit) as busy; parts of fixed length would leave the same units without work in clip after clip.
+__device__ __forceinline__ int64_t part_begin(const NormParams& p, int64_t n, int64_t k) {
+  return n < (1 << 20) ? (int64_t)((uint32_t)n * (uint32_t)k / (uint32_t)p.blocks) : n * k / p.blocks;  // blocks <= 2048
+}
+
 struct Cell {
-  int64_t b, block, r0, r1, c;
+  int64_t b, block, r0, r1, z0, z1, c;  // the clip's own places of the block, and the ones behind that it clears
   int ty, step;
   bool in;
 };
@@ -43,8 +48,11 @@ __device__ __forceinline__ Cell cell(const NormParams& p) {
   Cell q;
   q.b = LATE ? p.a.B - 1 - blockIdx.y : blockIdx.y;
   q.block = LATE ? p.blocks - 1 - blockIdx.x : blockIdx.x;
-  q.r0 = q.block * p.rows;
-  q.r1 = std::min<int64_t>(q.r0 + p.rows, p.S);
+  const int64_t own = own_of(p, q.b);
+  q.r0 = part_begin(p, own, q.block);
+  q.r1 = part_begin(p, own, q.block + 1);
+  q.z0 = own + part_begin(p, p.S - own, q.block);
+  q.z1 = own + part_begin(p, p.S - own, q.block + 1);
   const int tx = threadIdx.x % p.nb, v = blockIdx.z * p.nb + tx;
   q.ty = threadIdx.x / p.nb;
   q.step = 256 / p.nb;
@@ -58,7 +66,7 @@ template <class T, int V, bool VEC>
 __global__ void __launch_bounds__(256) norm_stats_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   const Cell q = cell<V, false>(p);
-  const int64_t end = std::min<int64_t>(q.r1, own_of(p, q.b));
+  const int64_t end = q.r1;
   if (q.r0 >= end) return;
   __shared__ float s_m[256][V + 1], s_v[256][V + 1];
   __shared__ int s_n[256];
@@ -136,7 +144,7 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
   __shared__ float s[4];
   const int g = blockIdx.x % (int)a.G, b = blockIdx.x / (int)a.G, cg = (int)(a.C / a.G);
   const int64_t own = own_of(p, b);
-  const int n = (int)((own + p.rows - 1) / p.rows) * cg;  // entries
+  const int n = p.blocks * cg;  // entries
   const float total = (float)own * (float)cg;
   const float* part = p.part + (int64_t)b * p.blocks * 2 * a.C + g * cg;
   float mean = 0.0f, var = 0.0f;
@@ -144,11 +152,11 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
     const auto entry = [&](int i, float& count, float& m, float& v) {
       const int q = i / cg;
       const float* at = part + (int64_t)q * 2 * a.C + (i - q * cg);
-      count = (float)(std::min<int64_t>((q + 1) * p.rows, own) - q * p.rows);
-      m = at[0];
-      v = at[a.C];
+      count = (float)(part_begin(p, own, q + 1) - part_begin(p, own, q));
+      m = count > 0.0f ? at[0] : 0.0f;  // a block without places has written nothing
+      v = count > 0.0f ? at[a.C] : 0.0f;
     };
-    const float k = part[0];  // means relative to the first one: their spread is what counts
+    const float k = part[(int64_t)(p.blocks - 1) * 2 * a.C];  // means relative to one of them (the last block always has places)
     float w = 0.0f, count[HELD ? HELD : 1], m[HELD ? HELD : 1], v[HELD ? HELD : 1];
     if constexpr (HELD > 0) {
 #pragma unroll
@@ -212,7 +220,6 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   const Cell q = cell<V, true>(p);
   if (!q.in) return;
-  const int64_t own = own_of(p, q.b);
   float mean[V], rstd[V], w[V], bias[V];
   channels<V>(p, q, mean, rstd, w, bias);
 #pragma unroll
@@ -220,10 +227,8 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
   const int64_t at = q.b * p.S * a.C + q.c;
   const T* x = static_cast<const T*>(a.x) + at;
   T* y = static_cast<T*>(a.y) + at;
-  const int64_t end = std::min<int64_t>(q.r1, own);
-  int64_t r = q.r0 + q.ty;
 #pragma unroll 4
-  for (; r < end; r += q.step) {
+  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
     float v[V];
     load_n<T, V, VEC>(x + r * a.C, V, v);
 #pragma unroll
@@ -231,14 +236,14 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
     store_n<T, V, VEC>(y + r * a.C, V, v);
   }
   const float zero[V] = {};
-  for (; r < q.r1; r += q.step) store_n<T, V, VEC>(y + r * a.C, V, zero);
+  for (int64_t r = q.z0 + q.ty; r < q.z1; r += q.step) store_n<T, V, VEC>(y + r * a.C, V, zero);
 }
 
 template <class T, int V, bool VEC, int ACT>
 __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   const Cell q = cell<V, false>(p);
-  const int64_t end = std::min<int64_t>(q.r1, own_of(p, q.b));
+  const int64_t end = q.r1;
   __shared__ float s_1[256][V + 1], s_2[256][V + 1];
   float s1[V], s2[V];
 #pragma unroll
@@ -351,7 +356,6 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   const Cell q = cell<V, true>(p);
   if (!q.in) return;
-  const int64_t own = own_of(p, q.b);
   float mean[V], rstd[V], w[V], bias[V], m1[V], m2[V];
   channels<V>(p, q, mean, rstd, w, bias);
   each_group<V>(p, q, [&](int c, int64_t g) {
@@ -361,10 +365,8 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   const int64_t at = q.b * p.S * a.C + q.c;
   const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
   T* dx = static_cast<T*>(a.dx) + at;
-  const int64_t end = std::min<int64_t>(q.r1, own);
-  int64_t r = q.r0 + q.ty;
 #pragma unroll 4
-  for (; r < end; r += q.step) {
+  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
     float v[V], g[V];
     load_n<T, V, VEC>(x + r * a.C, V, v);
     load_n<T, V, VEC>(dy + r * a.C, V, g);
@@ -376,7 +378,7 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
     store_n<T, V, VEC>(dx + r * a.C, V, v);
   }
   const float zero[V] = {};
-  for (; r < q.r1; r += q.step) store_n<T, V, VEC>(dx + r * a.C, V, zero);
+  for (int64_t r = q.z0 + q.ty; r < q.z1; r += q.step) store_n<T, V, VEC>(dx + r * a.C, V, zero);
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------
@@ -393,16 +395,15 @@ int check_args(const sed_norm_args* a) {
 }
 
 struct Layout {
-  int64_t rows, part, chan, gsum, total;
+  int64_t part, chan, gsum, total;
   int32_t blocks;
 };
 // Blocks of a clip: 2048 over the batch, eight for each compute unit (4096 cost the joining kernels more than they gave the others);
 // a block walks 32 places at least, so that its sums cost little beside its rows.
 Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   Layout l{};
-  int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + 31) / 32, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B))));
-  l.rows = std::max<int64_t>(1, (S + n - 1) / n);
-  l.blocks = (int32_t)std::max<int64_t>(1, (S + l.rows - 1) / l.rows);
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + 31) / 32, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B))));
+  l.blocks = (int32_t)n;
   int64_t at = 0;
   const auto take = [&](int64_t k) { const int64_t o = at; at += (k + 63) / 64 * 64; return o; };
   l.part = take(B * l.blocks * 2 * C);
@@ -459,7 +460,6 @@ int run(const sed_norm_args* args, bool back, void* stream) {
   p.half = 0;
   for (int lanes = 256 / p.nb, h = 1; h < lanes; h *= 2) p.half = h;
   p.blocks = l.blocks;
-  p.rows = l.rows;
   float* ws = static_cast<float*>(a.ws);
   p.part = ws + l.part;
   p.chan = ws + l.chan;

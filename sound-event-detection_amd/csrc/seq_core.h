@@ -85,21 +85,20 @@ __device__ __forceinline__ void store_n(T* p, int n, const float* in) {
 // ---- activations --------------------------------------------------------------------------------------------------------
 
 // The normal distribution's integral up to u, and e = exp(-u^2 / 2).  With x = |u| / sqrt(2) the part beyond |u| is
-// exp(-x^2) erfcx(x) / 2; erfcx(x) is t P(t), t = 1 / (1 + 0.3 x), P a polynomial fitted for the least relative error on
-// 0 <= x <= 10 (iteratively weighted least squares; 4.6e-7 of the value at most as it is evaluated here), half of it taken into
+// exp(-x^2) erfcx(x) / 2; erfcx(x) is t P(t), t = 1 / (1 + 0.6 x), P a polynomial fitted for the least relative error on
+// 0 <= x <= 10 (iteratively weighted least squares; 5.2e-7 of the value at most as it is evaluated here), half of it taken into
 // the coefficients.  So the far tail keeps its digits, and the slope's exponential is the same one.
 __device__ __forceinline__ float normal_cdf(float u, float& e) {
   e = exp2_hw(-0.5f * kLog2e * u * u);
-  const float t = rcp_hw(fmaf(0.3f * 0.70710678118654752440f, fabsf(u), 1.0f));
-  float p = 0.5f * -0.1295214593410492f;
-  p = fmaf(p, t, 0.5f * 0.4855561852455139f);
-  p = fmaf(p, t, 0.5f * -0.5122635364532471f);
-  p = fmaf(p, t, 0.5f * 0.547703206539154f);
-  p = fmaf(p, t, 0.5f * -0.09463890641927719f);
-  p = fmaf(p, t, 0.5f * 0.21492087841033936f);
-  p = fmaf(p, t, 0.5f * 0.14834055304527283f);
-  p = fmaf(p, t, 0.5f * 0.17071501910686493f);
-  p = fmaf(p, t, 0.5f * 0.1691880226135254f);
+  const float t = rcp_hw(fmaf(0.6f * 0.70710678118654752440f, fabsf(u), 1.0f));
+  float p = 0.5f * -0.09207959473133087f;
+  p = fmaf(p, t, 0.5f * 0.41193491220474243f);
+  p = fmaf(p, t, 0.5f * -0.6444382667541504f);
+  p = fmaf(p, t, 0.5f * 0.2837556004524231f);
+  p = fmaf(p, t, 0.5f * 0.07341824471950531f);
+  p = fmaf(p, t, 0.5f * 0.2915993928909302f);
+  p = fmaf(p, t, 0.5f * 0.33724936842918396f);
+  p = fmaf(p, t, 0.5f * 0.3385600745677948f);
   const float tail = p * t * e;
   return u < 0.0f ? tail : 1.0f - tail;  // a NaN stays one through e
 }
