@@ -399,10 +399,11 @@ struct Layout {
   int32_t blocks;
 };
 // Blocks of a clip: 2048 over the batch, eight for each compute unit (4096 cost the joining kernels more than they gave the others);
-// a block walks 32 places at least, so that its sums cost little beside its rows.
+// a block walks 32 places and 4096 values at least, so that its sums cost little beside its rows.
 Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   Layout l{};
-  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + 31) / 32, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B))));
+  const int64_t least = std::max<int64_t>(32, 4096 / C);
+  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + least - 1) / least, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B))));
   l.blocks = (int32_t)n;
   int64_t at = 0;
   const auto take = [&](int64_t k) { const int64_t o = at; at += (k + 63) / 64 * 64; return o; };

@@ -1049,31 +1049,36 @@ struct Layout {
   int64_t h, s, bc, pa, pd, total;  // float offsets into the workspace
 };
 
-// Time of `waves` waves of `cost` issue slots each on 1024 vector units that hold `most` of them at once, in slots of a full
-// unit (4.4 cycles): waves share a unit's slots (one alone gets 55 % of them, two 79 %, three 86 %, four 90 %, measured on
-// multiply-adds), and a round is over with its last wave.  Clips with lengths of their own: about half the chunks are empty, and
-// the rest is spread as it comes.
-double pass_time(double waves, int most, double cost, bool ragged) {
+// Time of `waves` waves on 1024 vector units that hold `most` of them at once, in issue slots of a full unit (4.4 cycles): a wave
+// takes `fixed` slots and `work`, or half of that on average where clips have lengths of their own.  Waves share a unit's slots
+// (one alone gets 55 % of them, two 79 %, three 86 %, four 90 %, measured on multiply-adds), and a round is over with its last
+// wave; waves of different lengths fill each other's gaps up to the last ones.
+double pass_time(double waves, int most, double fixed, double work, bool ragged) {
   static const double together[] = {0.0, 1.82, 2.53, 3.49, 4.44};
-  if (ragged) return cost * (0.55 * waves / 1024 * together[most] / most + 1.5 * together[1]);
+  if (ragged) {
+    const double mean = fixed + 0.5 * work;
+    return std::max((fixed + work) * together[1], mean * (waves / 1024 * together[most] / most + 0.5 * together[most]));
+  }
   const int64_t n = (int64_t)((waves + 1023) / 1024);
-  return cost * (double)(n / most) * together[most] + cost * together[n % most];
+  return (fixed + work) * ((double)(n / most) * together[most] + together[n % most]);
 }
 
 // Chunks of a clip, and the time of the passes.  A chunk's frames are walked twice (for its end state, then for its outputs), so
 // a clip stays whole where there are waves enough; else the count that pass_time gives least for.  Slots of a frame: 6 a state
 // and 14 for its sums and loads, 5 and 8 without outputs, 26.5 a state in the gradient, 40 / SPLIT for forming its rows; of a
-// wave's start: 500 (mostly latency); of joining a chunk: 30 a state and 30; of a launch: 1100 (2 us).
+// wave's start: 500 (mostly latency); of joining a chunk: 7.5 a state and 30; of a launch: 1100 (2 us); of a chunk's states in a
+// joining launch: 0.1 a state (12 bytes of traffic).
 int64_t chunks_of(const sed_scan_args& a, const Shape& s, int64_t waves, int64_t nt, bool back, double& best) {
   const int n = 4 * s.NS;
   const double rows = 40.0 / s.SPLIT, main = s.TT * ((back ? 26.5 * n : 6.0 * n + 14) + rows), ends = s.TT * (5.0 * n + 8 + rows);
   const int occ = back ? 2 : 4;
+  const bool ragged = a.frames != nullptr;
   int64_t K = 1;
-  for (int64_t k = 1; k <= std::max<int64_t>(1, nt / 2) && (k == 1 || waves * k <= 16384); ++k) {
+  for (int64_t k = 1; k <= std::max<int64_t>(1, nt / 2) && (k == 1 || waves * k <= 16384); k += k < 32 ? 1 : k / 8) {
     const double tiles = (double)((nt + k - 1) / k), join = k > kOwnJoin ? 0.0 : (double)k * (7.5 * n + 30);
-    double t = pass_time((double)(waves * k), occ, tiles * main + 500 + join, a.frames != nullptr);
-    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4, tiles * ends + 500, a.frames != nullptr) + 1100;
-    if (k > kOwnJoin) t += 1100 + 2700;
+    double t = pass_time((double)(waves * k), occ, 500 + join, tiles * main, ragged);
+    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4, 500, tiles * ends, ragged) + 1100;
+    if (k > kOwnJoin) t += 1100 + 2700 + 0.1 * n * (double)(waves * k);
     if (k == 1 || t < best) best = t, K = k;
   }
   return K;

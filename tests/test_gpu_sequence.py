@@ -127,6 +127,33 @@ def test_scan_many_waves_stay_whole():
     _scan_case(260, 20, 256, 1, 16, torch.bfloat16, seed=3, frames=[(7 * i) % 21 for i in range(260)], reverse=True)
 
 
+@pytest.mark.parametrize("nb,n,d,ns,frames", ((1, 70, 5, 3, None), (3, 1200, 5, 3, (1200, 2, 700)), (260, 9, 257, 3, None), (3, 1200, 5, 8, (3, 1200, 41)),
+                                              (260, 9, 512, 8, None), (100, 9, 511, 16, None), (3, 1200, 12, 16, (1200, 0, 99)), (2, 2000, 130, 16, (1999, 1)),
+                                              (3, 1200, 6, 32, (5, 640, 1200)), (520, 20, 31, 32, None), (2, 1500, 9, 1, (1500, 17))))
+def test_scan_instances_and_chunks(nb, n, d, ns, frames):
+    """Few waves and many, so that every instance runs, and long clips in more chunks than a short clip beside them has tiles."""
+    _scan_case(nb, n, d, 1, ns, torch.float32, seed=n + ns, frames=frames, state=True, reverse=n % 100 == 0)
+
+
+@pytest.mark.parametrize("nb,n,d,ns,frames", ((32, 600, 255, 16, None), (2, 2000, 768, 16, (1201, 2000)), (40, 300, 260, 8, None), (32, 300, 255, 32, None)))
+def test_scan_large_batches_clip_by_clip(nb, n, d, ns, frames):
+    """Batches in which every wave is full and clips are cut: two of the clips against the restatement of those alone."""
+    import sed_amd
+    dev, ref, rng = _scan_inputs(nb, n, d, 1, ns, torch.bfloat16, ns, state=True, frames=frames)
+    dy, rdy = _rounded(rng.standard_normal((nb, n, d)), torch.bfloat16)
+    leaves = {k: t.requires_grad_(True) for k, t in dev.items() if k != "frames"}
+    args = dict(dev)
+    y, last = sed_amd.gated_scan(*(args.pop(k) for k in ("x", "dt", "A", "B", "C")), **args, softplus=True, return_state=True)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
+    per_clip = ("x", "dt", "B", "C", "z", "state", "frames")
+    for b in (0, nb - 1):
+        o = S.scan(**{k: (v[b:b + 1] if k in per_clip else v) for k, v in ref.items()}, use_softplus=True, dy=rdy[b:b + 1])
+        _close(y[b:b + 1], o["y"][0], _scan_bound(o, "y", nb, n, d), "y")
+        _close(last[b:b + 1], o["last"][0], _scan_bound(o, "last", nb, n, d), "last")
+        for k in per_clip[:-1]:
+            _close(grads[k][b:b + 1], o[NAMES[k]][0], _scan_bound(o, NAMES[k], nb, n, d), NAMES[k])
+
+
 def test_scan_rows_behind_are_neither_read_nor_kept():
     import sed_amd
     dev, _, rng = _scan_inputs(3, 40, 64, 1, 16, torch.bfloat16, 7, frames=[40, 13, 0])
