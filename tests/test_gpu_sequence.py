@@ -143,7 +143,8 @@ def test_scan_large_batches_clip_by_clip(nb, n, d, ns, frames):
     dy, rdy = _rounded(rng.standard_normal((nb, n, d)), torch.bfloat16)
     leaves = {k: t.requires_grad_(True) for k, t in dev.items() if k != "frames"}
     args = dict(dev)
-    y, last = sed_amd.gated_scan(*(args.pop(k) for k in ("x", "dt", "A", "B", "C")), **args, softplus=True, return_state=True)
+    base = [args.pop(k) for k in ("x", "dt", "A", "B", "C")]
+    y, last = sed_amd.gated_scan(*base, **args, softplus=True, return_state=True)
     grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)))
     per_clip = ("x", "dt", "B", "C", "z", "state", "frames")
     for b in (0, nb - 1):
