@@ -3,8 +3,12 @@
 # usage: resource_usage.sh [file.hip] [extra hipcc flags]
 f=${1:-sed_frontend.hip}
 shift
-# the decoders and the resampler are built without fp contraction, as in the Makefile
-case "$f" in *sed_frontend.hip) nc= ;; *) nc=-ffp-contract=off ;; esac
+# flags per file as in the Makefile: the decoders and the resampler without fp contraction, the sequence operators without packed fp32
+case "$f" in
+  *sed_frontend.hip) nc= ;;
+  *sed_scan.hip|*sed_conv.hip|*sed_norm.hip) nc="-Xclang -target-feature -Xclang -packed-fp32-ops" ;;
+  *) nc=-ffp-contract=off ;;
+esac
 /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -I../../include $nc "$@" -c "$f" -o /dev/null \
   -Rpass-analysis=kernel-resource-usage 2>&1 | python3 -c '
 import re, subprocess, sys

@@ -7,6 +7,12 @@
 // meets there (a far mean costs no precision), joined per channel, then per group with the exact formula for joined means.
 // The gradient needs two sums a group, sum q and sum q n (q = du w, n the normalised value), which follow from the channels'
 // sums of du and du n: those are the bias' and the weight's gradients at the same time.
+// Two walks over a map are what a grid without a barrier can do: the second one goes backwards, so that what the memory-side
+// cache still holds is read from there.
+//
+// Measured (MI355X): 32 x 1001 x 64 x 64 bf16 SiLU (262 MB a map): statistics 59 us (4.4 TB/s), output 92 us (5.7 TB/s), the
+// gradient's sums 129 us (4.1 TB/s), the gradient 149 us (5.3 TB/s); a 1 GiB copy reaches 5.1.  Four walks of 8 clips each were no
+// faster than one of 32.  64 x 862 x 768 GELU with lengths of their own: 37 us for the output (vector unit: 24 slots a value).
 #include "seq_core.h"
 
 #include <algorithm>
