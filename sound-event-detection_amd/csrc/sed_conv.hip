@@ -354,7 +354,7 @@ template <class T, int V, int WM>
 int launch(const ConvParams& p, bool back, hipStream_t s) {
   const sed_conv_args& a = p.a;
   const int64_t grid = a.B * p.runs * p.nw;
-  if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
+  if (!grid_fits(grid, 64)) return SED_ERR_CAPACITY;
   const unsigned n = (unsigned)grid;
   if (!back) {
     if (a.act == SED_ACT_SILU)
@@ -375,7 +375,7 @@ template <class T, int V, int WM>
 int launch_step(const sed_conv_args& a, hipStream_t s) {
   const int nv = (int)(a.D / V);
   const int64_t grid = (a.B * nv + 255) / 256;
-  if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
+  if (!grid_fits(grid, 256)) return SED_ERR_CAPACITY;
   if (a.act == SED_ACT_SILU)
     conv_step_kernel<T, V, (V > 1), WM, SED_ACT_SILU><<<(unsigned)grid, 256, 0, s>>>(a, nv);
   else
@@ -398,7 +398,7 @@ int go(const ConvParams& p, Kind kind, int V, hipStream_t s) {
   int rc = V == 4 ? go_w<T, 4>(p, kind, s) : go_w<T, 1>(p, kind, s);
   if (rc != SED_OK || kind == STEP || a.W == 1) return rc;
   const int64_t grid = (a.B * (a.W - 1) * a.D + 255) / 256;
-  if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
+  if (!grid_fits(grid, 256)) return SED_ERR_CAPACITY;
   if (kind == FORWARD && a.state_out) conv_state_kernel<T><<<(unsigned)grid, 256, 0, s>>>(a);
   if (kind == BACKWARD && a.dstate) {
     if (a.act == SED_ACT_SILU)

@@ -458,7 +458,7 @@ int run(const sed_norm_args* args, bool back, void* stream) {
   p.S = a.T * a.F;
   const Layout l = layout_of(a.B, p.S, a.C, a.G);
   if (!a.ws || a.ws_bytes < l.total * 4 || !aligned(a.ws, 16)) return SED_ERR_CAPACITY;
-  if (a.B * a.G > 0x7fffffff) return SED_ERR_CAPACITY;
+  if (!grid_fits(a.B * a.G, 256)) return SED_ERR_CAPACITY;
   const int V = a.dtype == SED_F32 ? 4 : 8;
   const bool vec = a.C % V == 0 && aligned(a.x, 16) && aligned(a.y, 16) && aligned(a.dy, 16) && aligned(a.dx, 16);
   p.nv = (int32_t)(vec ? a.C / V : a.C);

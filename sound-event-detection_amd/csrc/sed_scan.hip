@@ -1153,7 +1153,7 @@ int launch(const ScanParams& p, hipStream_t stream) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
   const int64_t waves = a.B * p.K * a.G * p.tiles, joins = a.B * G::NP * a.D / 16;
-  if (waves > 0x7fffffff || joins >= 0x7fffffff) return SED_ERR_CAPACITY;
+  if (!grid_fits(waves + 4, 64) || !grid_fits(joins + 1, 256)) return SED_ERR_CAPACITY;
   constexpr int WE = waves_of<T, BACK, true>(), WM = waves_of<T, BACK, false>();  // of the ends, of the main pass
   const unsigned ends = (unsigned)((waves + WE - 1) / WE), main = (unsigned)((waves + WM - 1) / WM);
   if constexpr (!BACK) {
@@ -1164,7 +1164,7 @@ int launch(const ScanParams& p, hipStream_t stream) {
     scan_forward_kernel<NS, SPLIT, T, VEC, false><<<main, 64 * WM, 0, stream>>>(p);
   } else {
     const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 63) / 64;
-    if (bc > 0x7fffffff) return SED_ERR_CAPACITY;
+    if (!grid_fits(bc, 256)) return SED_ERR_CAPACITY;
     if (p.K > 1) {
       scan_backward_kernel<NS, SPLIT, T, VEC, true><<<ends, 64 * WE, 0, stream>>>(p);
       launch_join<G, true>(p, stream);
@@ -1224,7 +1224,7 @@ int step(const sed_scan_args& a, hipStream_t s) {
   const bool four = a.N % 4 == 0 && aligned(a.h_last, 16) && aligned(a.A, 16);
   const int need = four ? a.N / 4 : a.N, SP = need <= 1 ? 1 : need <= 2 ? 2 : need <= 4 ? 4 : 8;
   const int64_t grid = (a.B * a.D * SP + 255) / 256;
-  if (grid > 0x7fffffff) return SED_ERR_CAPACITY;
+  if (!grid_fits(grid, 256)) return SED_ERR_CAPACITY;
   const unsigned n = (unsigned)grid;
 #define SED_STEP(Q, S) scan_step_kernel<T, Q, S><<<n, 256, 0, s>>>(a)
   if (four) {

@@ -161,6 +161,9 @@ __device__ __forceinline__ float wave_sum(float x) {
   return fold32(x, x);
 }
 
+// A launch has fewer than 2^32 threads along an axis.
+inline bool grid_fits(int64_t blocks, int threads) { return blocks <= (int64_t)(0xffffffffu / (unsigned)threads); }
+
 inline int seq_status(hipError_t e) { return e == hipSuccess ? SED_OK : SED_ERR_HIP - (int)e; }
 
 }  // namespace sed

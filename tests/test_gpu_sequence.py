@@ -583,6 +583,68 @@ def test_replayed_graphs_follow_eager_calls(op):
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_replayed_steps_follow_eager_steps():
+    """One frame of both one-frame forms in a graph: every replay moves the states on by a frame, as eager calls do."""
+    import sed_amd
+    dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(4)
+    r = lambda *s: torch.randn(s, generator=g, device=dev)  # noqa: E731
+    A, w = -torch.rand(24, 16, generator=g, device=dev) * 3, r(24, 4)
+    frame = {"x": r(5, 24).bfloat16(), "dt": (r(5, 24) - 2).bfloat16(), "B": r(5, 16).bfloat16(), "C": r(5, 16).bfloat16()}
+    states = [[r(5, 3, 24).bfloat16(), r(5, 24, 16)] for _ in range(2)]
+    states[1] = [t.clone() for t in states[0]]
+
+    def call(v, s):
+        x = sed_amd.causal_conv_step(s[0], v["x"], w, activation="silu")
+        return sed_amd.gated_scan_step(s[1], x, v["dt"], A, v["B"], v["C"], softplus=True)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(frame, [t.clone() for t in states[0]])
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(frame, states[0])
+    for _ in range(4):
+        for t in frame.values():
+            t.copy_(r(*t.shape))
+        want = call(frame, states[1])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and all(torch.equal(a, b) for a, b in zip(*states))
+
+
+def test_lengths_out_of_range_are_clamped():
+    import sed_amd
+    dev = _dev()
+    x, A, bc, w = torch.randn(3, 20, 8, device=dev), -torch.rand(8, 4, device=dev), torch.randn(3, 20, 4, device=dev), torch.randn(8, 4, device=dev)
+    odd, even = (torch.tensor(v, dtype=torch.int32, device=dev) for v in ([-7, 2 ** 31 - 1, 5], [0, 20, 5]))
+    for call in (lambda f: sed_amd.gated_scan(x, x, A, bc, bc, softplus=True, frames=f), lambda f: sed_amd.causal_conv(x, w, frames=f),
+                 lambda f: sed_amd.group_norm_act(x, 2, frames=f)):
+        assert torch.equal(call(odd), call(even))
+
+
+def test_parameters_of_another_type():
+    """bf16 parameters are read as the fp32 values they hold; their gradients are the fp32 ones, rounded to bf16."""
+    import sed_amd
+    dev = _dev()
+    x, bc = torch.randn(2, 40, 16, device=dev), torch.randn(2, 40, 8, device=dev)
+    small = {"A": -torch.rand(16, 8, device=dev), "D": torch.randn(16, device=dev), "dt_bias": torch.randn(16, device=dev) - 2,
+             "w": torch.randn(16, 4, device=dev), "b": torch.randn(16, device=dev)}
+    got = []
+    for t in (torch.bfloat16, torch.float32):
+        p = {k: v.bfloat16().to(t).requires_grad_(True) for k, v in small.items()}
+        y = sed_amd.gated_scan(x, x, p["A"], bc, bc, D=p["D"], dt_bias=p["dt_bias"], softplus=True)
+        y = y + sed_amd.causal_conv(x, p["w"], p["b"], activation="silu") + sed_amd.group_norm_act(x, 4, p["D"], p["b"], activation="silu")
+        got.append([y.detach(), *torch.autograd.grad(y.sum(), list(p.values()))])
+    assert torch.equal(got[0][0], got[1][0])
+    for k, (a, b) in zip(small, zip(got[0][1:], got[1][1:])):
+        assert a.dtype == torch.bfloat16
+        if k in ("A", "dt_bias", "w"):  # D and b add two gradients, each rounded
+            assert torch.equal(a, b.bfloat16()), k
+
+
 def test_two_streams_and_repeated_calls_agree():
     import sed_amd
     dev = _dev()
