@@ -368,6 +368,14 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
     m1[c] = p.gsum[g * 2];
     m2[c] = p.gsum[g * 2 + 1];
   });
+  // dx = rstd (du w - m1 - n m2)
+  float wr[V];
+#pragma unroll
+  for (int c = 0; c < V; ++c) {
+    wr[c] = w[c] * rstd[c];
+    m1[c] *= rstd[c];
+    m2[c] *= rstd[c];
+  }
   const int64_t at = q.b * p.S * a.C + q.c;
   const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
   T* dx = static_cast<T*>(a.dx) + at;
@@ -378,8 +386,8 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
     load_n<T, V, VEC>(dy + r * a.C, V, g);
 #pragma unroll
     for (int c = 0; c < V; ++c) {
-      const float n = (v[c] - mean[c]) * rstd[c], qv = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c])) * w[c];
-      v[c] = rstd[c] * (qv - fmaf(n, m2[c], m1[c]));
+      const float n = (v[c] - mean[c]) * rstd[c], du = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c]));
+      v[c] = fmaf(-n, m2[c], fmaf(du, wr[c], -m1[c]));
     }
     store_n<T, V, VEC>(dx + r * a.C, V, v);
   }
