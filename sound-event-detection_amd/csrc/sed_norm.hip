@@ -11,7 +11,7 @@
 // cache still holds is read from there.
 //
 // Measured (MI355X): 32 x 1001 x 64 x 64 bf16 SiLU (262 MB a map): statistics 59 us (4.4 TB/s), output 92 us (5.7 TB/s), the
-// gradient's sums 129 us (4.1 TB/s), the gradient 149 us (5.3 TB/s); a 1 GiB copy reaches 5.1.  Four walks of 8 clips each were no
+// gradient's sums 122 us (4.3 TB/s), the gradient 137 us (5.7 TB/s); a 1 GiB copy reaches 5.1.  Four walks of 8 clips each were no
 // faster than one of 32.  64 x 862 x 768 GELU with lengths of their own: 37 us for the output (vector unit: 24 slots a value).
 #include "seq_core.h"
 
@@ -197,6 +197,39 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
   }
 }
 
+// Rows of both maps that a gradient's lane has on the way at once.  Two where a row takes the most registers (gelu, 8 channels): there
+// four leave three waves a vector unit and are 1.5 % slower (32 x 1001 x 64 x 64 bf16, forward and gradient).  Four elsewhere: fp32
+// gelu 869 us against 896 with two, bf16 SiLU 435 against 442 with the compiler's own order.
+template <int ACT>
+constexpr int grad_rows(int channels) { return ACT == SED_ACT_GELU && channels == 8 ? 2 : 4; }
+
+// Walks rows [r, end) in steps, ROWS of them loaded from both maps before the first is worked on (then one after another: worked
+// on together they would take more registers than keep four waves a vector unit).
+template <class T, int V, int ROWS, class F>
+__device__ __forceinline__ void walk_two(const T* x, const T* y, int64_t r, int64_t end, int step, int64_t C, F f) {
+  typedef T vt __attribute__((ext_vector_type(V)));
+  const auto one = [&](const vt& a, const vt& b, int64_t at) {
+    float u[V], v[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) u[c] = (float)a[c], v[c] = (float)b[c];
+    f(u, v, at);
+  };
+  for (; r + (ROWS - 1) * step < end; r += ROWS * step) {
+    vt a[ROWS], b[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      a[k] = *reinterpret_cast<const vt*>(x + (r + k * step) * C);
+      b[k] = *reinterpret_cast<const vt*>(y + (r + k * step) * C);
+    }
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      __builtin_amdgcn_sched_barrier(0);
+      one(a[k], b[k], r + k * step);
+    }
+  }
+  for (; r < end; r += step) one(*reinterpret_cast<const vt*>(x + r * C), *reinterpret_cast<const vt*>(y + r * C), r);
+}
+
 // Calls f(channel of the lane, its group) for the lane's V channels in order.
 template <int V, class F>
 __device__ __forceinline__ void each_group(const NormParams& p, const Cell& q, F f) {
@@ -259,18 +292,14 @@ __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p)
     channels<V>(p, q, mean, rstd, w, bias);
     const int64_t at = q.b * p.S * a.C + q.c;
     const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
-#pragma unroll 4
-    for (int64_t r = q.r0 + q.ty; r < end; r += q.step) {
-      float v[V], g[V];
-      load_n<T, V, VEC>(x + r * a.C, V, v);
-      load_n<T, V, VEC>(dy + r * a.C, V, g);
+    walk_two<T, V, grad_rows<ACT>(V)>(x, dy, q.r0 + q.ty, end, q.step, a.C, [&](const float(&v)[V], const float(&g)[V], int64_t) {
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const float n = (v[c] - mean[c]) * rstd[c], du = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c]));
         s1[c] += du;
         s2[c] = fmaf(du, n, s2[c]);
       }
-    }
+    });
   }
 #pragma unroll
   for (int c = 0; c < V; ++c) {
@@ -379,18 +408,15 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   const int64_t at = q.b * p.S * a.C + q.c;
   const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
   T* dx = static_cast<T*>(a.dx) + at;
-#pragma unroll 4
-  for (int64_t r = q.r0 + q.ty; r < q.r1; r += q.step) {
-    float v[V], g[V];
-    load_n<T, V, VEC>(x + r * a.C, V, v);
-    load_n<T, V, VEC>(dy + r * a.C, V, g);
+  walk_two<T, V, grad_rows<ACT>(V)>(x, dy, q.r0 + q.ty, q.r1, q.step, a.C, [&](const float(&v)[V], const float(&g)[V], int64_t r) {
+    float d[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) {
       const float n = (v[c] - mean[c]) * rstd[c], du = g[c] * act_slope<ACT>(fmaf(n, w[c], bias[c]));
-      v[c] = fmaf(-n, m2[c], fmaf(du, wr[c], -m1[c]));
+      d[c] = fmaf(-n, m2[c], fmaf(du, wr[c], -m1[c]));
     }
-    store_n<T, V, VEC>(dx + r * a.C, V, v);
-  }
+    store_n<T, V, VEC>(dx + r * a.C, V, d);
+  });
   const float zero[V] = {};
   for (int64_t r = q.z0 + q.ty; r < q.z1; r += q.step) store_n<T, V, VEC>(dx + r * a.C, V, zero);
 }
