@@ -7,7 +7,7 @@
 // window of WM rows, the weights and, in the gradient, the sums of its V channels in registers.  Rows come WM at a time, the
 // next WM on their way while WM are worked on.  A row is read once but for the WM - 1 in front of a run (and behind it, in the
 // gradient).  WM is W rounded up to 2, 4 or 8: the weights in front are zero.  V = 4 where rows allow it and there are channels
-// enough for a wave, else 1.  The weight gradient is summed per lane over its run, written once per run and added over the runs
+// enough for a wave (2 of them at a time in the gradient of more than 4 taps), else 1.  The weight gradient is summed per lane over its run, written once per run and added over the runs
 // in a fixed order.  Sums are fp32 and every output is rounded once.
 //
 // Measured (MI355X): 16 x 4096 x 1536 bf16, 4 taps with SiLU: forward 79 us for 403 MB (5.1 TB/s, what a 1 GiB copy reaches),
@@ -350,23 +350,31 @@ int run_frames(int64_t B, int64_t L, int64_t nw, bool back) {
 }
 int64_t waves_along(int64_t D, int V) { return (D / V + 63) / 64; }
 
+// The gradient's lane takes 2 channels in place of 4 where more than 4 taps would leave no room for them (254 registers, one wave a
+// vector unit, fp32 with 36 of them spilt).  16 x 4096 x 1536 with 8 taps: bf16 276 us with 4, 248 with 2, 312 with 1; fp32 402, 319, 324.
+constexpr int back_vector(int V, int taps) { return V == 4 && taps > 4 ? 2 : V; }
+
 template <class T, int V, int WM>
-int launch(const ConvParams& p, bool back, hipStream_t s) {
+int launch_forward(const ConvParams& p, hipStream_t s) {
   const sed_conv_args& a = p.a;
   const int64_t grid = a.B * p.runs * p.nw;
   if (!grid_fits(grid, 64)) return SED_ERR_CAPACITY;
-  const unsigned n = (unsigned)grid;
-  if (!back) {
-    if (a.act == SED_ACT_SILU)
-      conv_forward_kernel<T, V, WM, SED_ACT_SILU><<<n, 64, 0, s>>>(p);
-    else
-      conv_forward_kernel<T, V, WM, SED_ACT_NONE><<<n, 64, 0, s>>>(p);
-    return seq_status(hipGetLastError());
-  }
   if (a.act == SED_ACT_SILU)
-    conv_backward_kernel<T, V, WM, SED_ACT_SILU><<<n, 64, 0, s>>>(p);
+    conv_forward_kernel<T, V, WM, SED_ACT_SILU><<<(unsigned)grid, 64, 0, s>>>(p);
   else
-    conv_backward_kernel<T, V, WM, SED_ACT_NONE><<<n, 64, 0, s>>>(p);
+    conv_forward_kernel<T, V, WM, SED_ACT_NONE><<<(unsigned)grid, 64, 0, s>>>(p);
+  return seq_status(hipGetLastError());
+}
+
+template <class T, int V, int WM>
+int launch_backward(const ConvParams& p, hipStream_t s) {
+  const sed_conv_args& a = p.a;
+  const int64_t grid = a.B * p.runs * p.nw;
+  if (!grid_fits(grid, 64)) return SED_ERR_CAPACITY;
+  if (a.act == SED_ACT_SILU)
+    conv_backward_kernel<T, V, WM, SED_ACT_SILU><<<(unsigned)grid, 64, 0, s>>>(p);
+  else
+    conv_backward_kernel<T, V, WM, SED_ACT_NONE><<<(unsigned)grid, 64, 0, s>>>(p);
   conv_param_kernel<<<(unsigned)(((a.W + 1) * a.D + 63) / 64), 1024, 0, s>>>(p);
   return seq_status(hipGetLastError());
 }
@@ -385,11 +393,18 @@ int launch_step(const sed_conv_args& a, hipStream_t s) {
 
 enum Kind { FORWARD, BACKWARD, STEP };
 
+template <class T, int V, int WM>
+int go_kind(const ConvParams& p, Kind kind, hipStream_t s) {
+  if (kind == STEP) return launch_step<T, V, WM>(p.a, s);
+  if (kind == FORWARD) return launch_forward<T, V, WM>(p, s);
+  return launch_backward<T, back_vector(V, WM), WM>(p, s);
+}
+
 template <class T, int V>
 int go_w(const ConvParams& p, Kind kind, hipStream_t s) {
-  if (p.a.W <= 2) return kind == STEP ? launch_step<T, V, 2>(p.a, s) : launch<T, V, 2>(p, kind == BACKWARD, s);
-  if (p.a.W <= 4) return kind == STEP ? launch_step<T, V, 4>(p.a, s) : launch<T, V, 4>(p, kind == BACKWARD, s);
-  return kind == STEP ? launch_step<T, V, 8>(p.a, s) : launch<T, V, 8>(p, kind == BACKWARD, s);
+  if (p.a.W <= 2) return go_kind<T, V, 2>(p, kind, s);
+  if (p.a.W <= 4) return go_kind<T, V, 4>(p, kind, s);
+  return go_kind<T, V, 8>(p, kind, s);
 }
 
 template <class T>
@@ -413,7 +428,7 @@ int run(const sed_conv_args* args, Kind kind, void* stream) {
   ConvParams p{};
   p.a = *args;
   const int V = vector_of(p.a);
-  p.nw = (int32_t)waves_along(p.a.D, V);
+  p.nw = (int32_t)waves_along(p.a.D, kind == BACKWARD ? back_vector(V, p.a.W) : V);
   p.TL = run_frames(p.a.B, p.a.L, p.nw, kind == BACKWARD);
   p.runs = (p.a.L + p.TL - 1) / p.TL;
   if (kind == BACKWARD) {
@@ -432,7 +447,7 @@ int run(const sed_conv_args* args, Kind kind, void* stream) {
 extern "C" int64_t sed_causal_conv_workspace(int64_t B, int64_t L, int64_t D, int32_t W) {
   if (B < 0 || L < 0 || D < 1 || W < 1 || W > 8) return SED_ERR_BAD_ARG;
   int64_t most = 0;
-  for (const int V : {1, 4}) {
+  for (const int V : {1, sed::back_vector(4, W)}) {
     if (D % V) continue;
     const int TL = sed::run_frames(B, L, sed::waves_along(D, V), true);
     most = std::max<int64_t>(most, 4 * B * ((L + TL - 1) / TL) * (W + 1) * D);

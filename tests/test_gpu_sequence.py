@@ -351,6 +351,41 @@ def test_conv_sizes(nb, n, d, W, dtype):
     _conv_case(nb, n, d, W, DTYPES[dtype], seed=n + d, state=n % 2 == 0)
 
 
+@pytest.mark.parametrize("dtype", ("fp32", "bf16", "fp16"))
+@pytest.mark.parametrize("nb,n,d,W", ((2, 97, 256, 4), (1, 200, 260, 3), (1, 65, 516, 2), (2, 130, 260, 8), (1, 70, 256, 5), (1, 9, 256, 1), (3, 1, 768, 7)))
+def test_conv_rows_of_whole_vectors(nb, n, d, W, dtype):
+    _conv_case(nb, n, d, W, DTYPES[dtype], seed=n + d, state=n % 2 == 0)
+    _conv_case(nb, n, d, W, DTYPES[dtype], seed=n + d + 1, state=True, reverse=True, silu=False, frames=[n - n // 3, 0, n][:nb])
+
+
+@pytest.mark.parametrize("d,W,dtype", ((1, 4, torch.float32), (1, 6, torch.bfloat16), (256, 4, torch.bfloat16), (256, 8, torch.bfloat16), (256, 8, torch.float32)))
+def test_conv_batches_that_fill_the_card(d, W, dtype):
+    """Runs of the longest kind (2100 clips of two): all clips but two are zeros, so that those two are the weights' gradient."""
+    import sed_amd
+    nb, n, pick = 2100, 70, [3, 2099]
+    rng = np.random.default_rng(d + W)
+    x, rx = _rounded(rng.standard_normal((2, n, d)), dtype)
+    dy, rdy = _rounded(rng.standard_normal((2, n, d)), dtype)
+    w, rw = _rounded(rng.standard_normal((d, W)), torch.float32)
+    b, rb = _rounded(rng.standard_normal(d), torch.float32)
+    bx, bdy = (torch.zeros(nb, n, d, dtype=dtype, device=_dev()) for _ in range(2))
+    bx[pick], bdy[pick] = x, dy
+    fr = torch.full((nb,), n, dtype=torch.int32, device=_dev())
+    fr[3] = 67
+    leaves = [t.requires_grad_(True) for t in (bx, w, b)]
+    y = sed_amd.causal_conv(bx, w, b, activation="silu", frames=fr)
+    o = S.conv(rx, rw, rb, True, [67, n], False, None, rdy, None)
+    few, many = U * (2 * W + 32), U * (2 * W + 150 + 2 * n / 8)  # as in every case: a zero clip adds nothing to a sum
+    _close(y[pick], o["y"][0], few * o["y"][1], "y")
+    dx, dw, db = torch.autograd.grad(y, leaves, bdy)
+    _close(dx[pick], o["dx"][0], 2 * few * o["dx"][1], "dx")
+    _close(dw, o["dw"][0], many * o["dw"][1], "dw")
+    _close(db, o["db"][0], many * o["db"][1], "db")
+    rest = torch.ones(nb, dtype=torch.bool)
+    rest[pick] = False
+    assert (dx[rest.to(dx.device)] == 0).all()
+
+
 @pytest.mark.parametrize("reverse", (False, True))
 def test_conv_own_lengths(reverse):
     for dtype in (torch.float32, torch.bfloat16):
@@ -442,6 +477,14 @@ def _norm_case(shape, groups, dtype, act="silu", seed=0, affine=True, frames=Non
                                           ((1, 33, 40), 40), ((2, 9, 3, 2, 6), 2), ((1, 70, 2064), 3), ((1, 5, 4104), 2), ((1, 400, 257), 1), ((2, 130, 64), 32)))
 def test_norm_sizes(shape, groups, dtype):
     _norm_case(shape, groups, DTYPES[dtype], act=(None, "silu", "gelu")[sum(shape) % 3], seed=sum(shape))
+
+
+@pytest.mark.parametrize("act", (None, "silu", "gelu"))
+@pytest.mark.parametrize("shape,groups", (((1, 700, 1, 256), 8), ((2, 433, 3, 64), 8), ((1, 1501, 2064), 3), ((1, 901, 33), 3)))
+def test_norm_long_walks(shape, groups, act):
+    """Blocks whose lanes meet many rows: whole batches of rows, a rest behind them, and blocks of uneven parts."""
+    for dtype in (torch.float32, torch.bfloat16):
+        _norm_case(shape, groups, dtype, act=act, seed=7, frames=[shape[1] - 5, 2][:shape[0]] if shape[3:] else None)
 
 
 @pytest.mark.parametrize("act", (None, "silu", "relu", "gelu"))
