@@ -127,6 +127,13 @@ def test_scan_many_waves_stay_whole():
     _scan_case(260, 20, 256, 1, 16, torch.bfloat16, seed=3, frames=[(7 * i) % 21 for i in range(260)], reverse=True)
 
 
+@pytest.mark.parametrize("nb", (2, 63, 64, 65, 130))
+def test_scan_orders_of_clips(nb):
+    """Every clip is walked once whatever the order of lengths: equal ones, none, rising and falling, past the ends, more than 64 clips."""
+    for k, frames in enumerate(([9] * nb, [0] * nb, list(range(nb)), list(range(nb, 0, -1)), [(29 * i) % 47 - 3 for i in range(nb)])):
+        _scan_case(nb, 41, 4, 1, (1, 4, 8, 16, 17)[k], torch.float32, seed=k, frames=frames, reverse=k % 2 == 0, state=True)
+
+
 @pytest.mark.parametrize("nb,n,d,ns,frames", ((1, 70, 5, 3, None), (3, 1200, 5, 3, (1200, 2, 700)), (260, 9, 257, 3, None), (3, 1200, 5, 8, (3, 1200, 41)),
                                               (260, 9, 512, 8, None), (100, 9, 511, 16, None), (3, 1200, 12, 16, (1200, 0, 99)), (2, 2000, 130, 16, (1999, 1)),
                                               (3, 1200, 6, 32, (5, 640, 1200)), (520, 20, 31, 32, None), (2, 1500, 9, 1, (1500, 17))))
