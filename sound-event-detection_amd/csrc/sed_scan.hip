@@ -22,7 +22,7 @@
 //
 // Measured (MI355X, bf16, N = 16): 16 x 513 x 1536 forward 111 us in one pass of thin waves (134 in chunks of wide ones), 1.8e12
 // states of a frame a second; its gradient 202 us and 54 us for the chunks' ends: 26.5 vector instructions a state and
-// frame, of which 16 are the formulas', the vector units issuing 76 % of the time.  64 clips of up to 1024 x 768: 218 us.
+// frame, of which 16 are the formulas', the vector units issuing 76 % of the time.  64 clips of up to 1024 x 768: 167 us.
 // 512 streams x 1536 x 16, one frame: 25 us for 107 MB (4.2 TB/s; a 1 GiB copy reaches 5.1).
 #include "seq_core.h"
 
