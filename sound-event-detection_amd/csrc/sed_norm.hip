@@ -10,8 +10,8 @@
 // Two walks over a map are what a grid without a barrier can do: the second one goes backwards, so that what the memory-side
 // cache still holds is read from there.
 //
-// Measured (MI355X): 32 x 1001 x 64 x 64 bf16 SiLU (262 MB a map): statistics 59 us (4.4 TB/s), output 92 us (5.7 TB/s), the
-// gradient's sums 122 us (4.3 TB/s), the gradient 137 us (5.7 TB/s); a 1 GiB copy reaches 5.1.  Four walks of 8 clips each were no
+// Measured (MI355X): 32 x 1001 x 64 x 64 bf16 SiLU (262 MB a map): statistics 59 us (4.4 TB/s), output 93 us (5.6 TB/s), the
+// gradient's sums 115 us (4.6 TB/s), the gradient 136 us (5.8 TB/s); a 1 GiB copy reaches 5.1.  Four walks of 8 clips each were no
 // faster than one of 32.  64 x 862 x 768 GELU with lengths of their own: 37 us for the output (vector unit: 24 slots a value).
 #include "seq_core.h"
 
@@ -26,6 +26,7 @@ struct NormParams {
   int32_t nv, nb;    // vectors of a row, lanes along a row
   int32_t half;      // half the lanes of a channel, rounded up to a power of two
   int32_t blocks;    // blocks a clip is cut into
+  int32_t late;      // the same for the second walk
   float* part;       // [B][blocks][2][C]: (mean, sum of squares about it), or (sum du, sum du n)
   float* chan;       // [B][2][C]
   float* gsum;       // [B][G][2]: means of q and q n
@@ -37,10 +38,10 @@ __device__ __forceinline__ int64_t own_of(const NormParams& p, int64_t b) {
   return t * a.F;
 }
 
-// First of a clip's n places that block k of its `blocks` takes: even parts, so that clips of other lengths keep every block (and
+// First of a clip's n places that block k of `blocks` takes: even parts, so that clips of other lengths keep every block (and
 // every compute unit) as busy; parts of fixed length would leave the same units without work in clip after clip.
-__device__ __forceinline__ int64_t part_begin(const NormParams& p, int64_t n, int64_t k) {
-  return n < (1 << 20) ? (int64_t)((uint32_t)n * (uint32_t)k / (uint32_t)p.blocks) : n * k / p.blocks;  // blocks <= 2048
+__device__ __forceinline__ int64_t part_begin(int blocks, int64_t n, int64_t k) {
+  return n < (1 << 18) ? (int64_t)((uint32_t)n * (uint32_t)k / (uint32_t)blocks) : n * k / blocks;  // blocks <= 8192
 }
 
 struct Cell {
@@ -53,12 +54,13 @@ template <int V, bool LATE>
 __device__ __forceinline__ Cell cell(const NormParams& p) {
   Cell q;
   q.b = LATE ? p.a.B - 1 - blockIdx.y : blockIdx.y;
-  q.block = LATE ? p.blocks - 1 - blockIdx.x : blockIdx.x;
+  const int blocks = LATE ? p.late : p.blocks;
+  q.block = LATE ? blocks - 1 - blockIdx.x : blockIdx.x;
   const int64_t own = own_of(p, q.b);
-  q.r0 = part_begin(p, own, q.block);
-  q.r1 = part_begin(p, own, q.block + 1);
-  q.z0 = own + part_begin(p, p.S - own, q.block);
-  q.z1 = own + part_begin(p, p.S - own, q.block + 1);
+  q.r0 = part_begin(blocks, own, q.block);
+  q.r1 = part_begin(blocks, own, q.block + 1);
+  q.z0 = own + part_begin(blocks, p.S - own, q.block);
+  q.z1 = own + part_begin(blocks, p.S - own, q.block + 1);
   const int tx = threadIdx.x % p.nb, v = blockIdx.z * p.nb + tx;
   q.ty = threadIdx.x / p.nb;
   q.step = 256 / p.nb;
@@ -158,7 +160,7 @@ __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
     const auto entry = [&](int i, float& count, float& m, float& v) {
       const int q = i / cg;
       const float* at = part + (int64_t)q * 2 * a.C + (i - q * cg);
-      count = (float)(part_begin(p, own, q + 1) - part_begin(p, own, q));
+      count = (float)(part_begin(p.blocks, own, q + 1) - part_begin(p.blocks, own, q));
       m = count > 0.0f ? at[0] : 0.0f;  // a block without places has written nothing
       v = count > 0.0f ? at[a.C] : 0.0f;
     };
@@ -436,15 +438,18 @@ int check_args(const sed_norm_args* a) {
 
 struct Layout {
   int64_t part, chan, gsum, total;
-  int32_t blocks;
+  int32_t blocks, late;
 };
 // Blocks of a clip: 2048 over the batch, eight for each compute unit (4096 cost the joining kernels more than they gave the others);
-// a block walks 32 places and 4096 values at least, so that its sums cost little beside its rows.
+// a block walks 32 places and 4096 values at least, so that its sums cost little beside its rows.  The second walk leaves no sums:
+// 8192 blocks, which end closer together (32 x 1001 x 64 x 64 forward and gradient: 435 us with 2048, 429 with 4096, 423 with 8192,
+// 450 with 16384; fewer than 32 places each: 64 clips of up to 862 x 768 in 72 us, 57 with 32).
 Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   Layout l{};
   const int64_t least = std::max<int64_t>(32, 4096 / C);
-  const int64_t n = std::max<int64_t>(1, std::min<int64_t>((S + least - 1) / least, std::max<int64_t>(1, 2048 / std::max<int64_t>(1, B))));
-  l.blocks = (int32_t)n;
+  const auto blocks = [&](int64_t most) { return (int32_t)std::max<int64_t>(1, std::min<int64_t>((S + least - 1) / least, most / std::max<int64_t>(1, B))); };
+  l.blocks = blocks(2048);
+  l.late = blocks(8192);
   int64_t at = 0;
   const auto take = [&](int64_t k) { const int64_t o = at; at += (k + 63) / 64 * 64; return o; };
   l.part = take(B * l.blocks * 2 * C);
@@ -457,7 +462,7 @@ Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
 template <class T, int V, bool VEC, int ACT>
 int launch(const NormParams& p, bool back, hipStream_t s) {
   const sed_norm_args& a = p.a;
-  const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb));
+  const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb)), late((unsigned)p.late, grid.y, grid.z);
   const unsigned groups = (unsigned)(a.B * a.G), threads = (unsigned)((256 / p.nb * p.nb + 63) / 64 * 64);
   if (!back) {
     norm_stats_kernel<T, V, VEC><<<grid, threads, 0, s>>>(p);
@@ -465,11 +470,11 @@ int launch(const NormParams& p, bool back, hipStream_t s) {
       norm_join_kernel<8><<<groups, 256, 0, s>>>(p);
     else
       norm_join_kernel<0><<<groups, 256, 0, s>>>(p);
-    norm_apply_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
+    norm_apply_kernel<T, V, VEC, ACT><<<late, threads, 0, s>>>(p);
   } else {
     norm_grad_sums_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
     norm_grad_join_kernel<<<groups, 256, 0, s>>>(p);
-    norm_grad_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
+    norm_grad_kernel<T, V, VEC, ACT><<<late, threads, 0, s>>>(p);
     if (a.dw || a.db) norm_param_kernel<<<(unsigned)((2 * a.C + 255) / 256), 256, 0, s>>>(p);
   }
   return seq_status(hipGetLastError());
@@ -501,6 +506,7 @@ int run(const sed_norm_args* args, bool back, void* stream) {
   p.half = 0;
   for (int lanes = 256 / p.nb, h = 1; h < lanes; h *= 2) p.half = h;
   p.blocks = l.blocks;
+  p.late = l.late;
   float* ws = static_cast<float*>(a.ws);
   p.part = ws + l.part;
   p.chan = ws + l.chan;
