@@ -76,6 +76,14 @@ struct Geo {
   static_assert(R * SPLIT == TT, "");
 };
 
+// LDS that a wave of the main passes takes (the gradient keeps rows of elements of `size` bytes there), and its waves on a vector unit.
+constexpr int lds_of(int NS, int SPLIT, int NP, int TT, bool back, int size) {
+  const int cw = 256 / SPLIT;
+  if (!back) return 4 * (3 * TT * cw + 2 * TT * NP);
+  return 4 * (4 * TT * cw + 2 * TT * NP + NS * 256 + 2 * cw) + 4 * (TT / SPLIT) * 64 * 4 * size;
+}
+constexpr int per_unit(int SPLIT, bool back) { return back ? 2 : SPLIT == 1 ? 3 : 4; }
+
 // Where a wave works.
 struct Where {
   int b, chunk, g, s, j;
@@ -401,7 +409,7 @@ __device__ __forceinline__ void clear_rows(const ScanParams& p, const Where& w, 
 
 // ENDS: only the chunk's end state from zero and its sum of delta.  Otherwise the chunk's outputs.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (SPLIT == 1 ? 3 : 4)) scan_forward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(SPLIT, false))) scan_forward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   constexpr int W = waves_of<T, false, ENDS>();
   const sed_scan_args& a = p.a;
@@ -409,6 +417,7 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (SPLIT == 1
   struct Shared {
     float dl[G::TT][G::CW], dx[G::TT][G::CW], y[ENDS ? 1 : G::TT][G::CW], B[G::TT][G::NP], C[G::TT][G::NP];
   };
+  static_assert(ENDS || sizeof(Shared) == lds_of(NS, SPLIT, G::NP, G::TT, false, sizeof(T)), "");
   __shared__ __attribute__((aligned(16))) Shared shared[W];
   Shared& sh = shared[wave_id()];
   auto &s_dl = sh.dl, &s_dx = sh.dx;
@@ -635,7 +644,7 @@ __device__ __forceinline__ int sum_index(int j) {
 
 // ENDS: only the gradient that reaches the frame in front of the chunk from the chunk's own outputs, and the sum of delta.
 template <int NS, int SPLIT, class T, bool VEC, bool ENDS>
-__global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 2)) scan_backward_kernel(const ScanParams p) {
+__global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : per_unit(SPLIT, true))) scan_backward_kernel(const ScanParams p) {
   using G = Geo<NS, SPLIT>;
   constexpr int W = waves_of<T, true, ENDS>();
   const sed_scan_args& a = p.a;
@@ -649,6 +658,7 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
     T4<T> raw[ENDS ? 1 : 4][ENDS ? 1 : G::R][64];
     float h[ENDS ? 1 : NS][ENDS ? 4 : 256], ch[2][G::CW];
   };
+  static_assert(ENDS || sizeof(Shared) == lds_of(NS, SPLIT, G::NP, G::TT, true, sizeof(T)), "");
   __shared__ __attribute__((aligned(16))) Shared shared[W];
   Shared& sh = shared[wave_id()];
   auto &s_dl = sh.dl, &s_gy = sh.gy;
@@ -1070,18 +1080,26 @@ struct Layout {
   int64_t h, s, bc, pa, pd, total;  // float offsets into the workspace
 };
 
-// Time of `waves` waves on 1024 vector units that hold `most` of them at once, in issue slots of a full unit (4.4 cycles): a wave
+// Waves of the main pass that the card holds at once.  The gradient of 16 states in fp32 is the one that LDS keeps from its two a vector
+// unit (7 a compute unit): taken for 8, the last waves ran alone (1 x 16385 x 384: 230 us, 186 so; 16 x 513 x 1536: 365, 323).
+int resident(const Shape& s, bool back, int size) {
+  const int group = back && size == 4 ? 1 : 4, fit = 160 * 1024 / (group * lds_of(s.NS, s.SPLIT, s.NP, s.TT, back, size));
+  return 256 * std::min(4 * per_unit(s.SPLIT, back), group * std::max(1, fit));
+}
+
+// Time of `waves` waves on 1024 vector units that hold `held` of them at once, in issue slots of a full unit (4.4 cycles): a wave
 // takes `fixed` slots and `work`, or half of that on average where clips have lengths of their own.  Waves share a unit's slots
 // (one alone gets 55 % of them, two 79 %, three 86 %, four 90 %, measured on multiply-adds), and a round is over with its last
 // wave; waves of different lengths fill each other's gaps up to the last ones.
-double pass_time(double waves, int most, double fixed, double work, bool ragged) {
+double pass_time(double waves, int held, double fixed, double work, bool ragged) {
   static const double together[] = {0.0, 1.82, 2.53, 3.49, 4.44};
+  const int most = (held + 1023) / 1024;
   if (ragged) {
     const double mean = fixed + 0.5 * work;
-    return std::max((fixed + work) * together[1], mean * (waves / 1024 * together[most] / most + 0.5 * together[most]));
+    return std::max((fixed + work) * together[1], mean * (waves / held * together[most] + 0.5 * together[most]));
   }
-  const int64_t n = (int64_t)((waves + 1023) / 1024);
-  return (fixed + work) * ((double)(n / most) * together[most] + together[n % most]);
+  const int64_t rounds = (int64_t)waves / held, rest = (int64_t)waves % held;
+  return (fixed + work) * ((double)rounds * together[most] + together[(rest + 1023) / 1024]);
 }
 
 // Chunks of a clip, and the time of the passes.  A chunk's frames are walked twice (for its end state, then for its outputs), so
@@ -1092,16 +1110,19 @@ double pass_time(double waves, int most, double fixed, double work, bool ragged)
 int64_t chunks_of(const sed_scan_args& a, const Shape& s, int64_t waves, int64_t nt, bool back, double& best) {
   const int n = 4 * s.NS;
   const double rows = 40.0 / s.SPLIT, main = s.TT * ((back ? 26.5 * n : 6.0 * n + 14) + rows), ends = s.TT * (5.0 * n + 8 + rows);
-  const int occ = back ? 2 : 4;
+  const int held = resident(s, back, a.dtype == SED_F32 ? 4 : 2);
   const bool ragged = a.frames != nullptr;
+  const int64_t most = std::max<int64_t>(1, nt / 2);
   int64_t K = 1;
-  for (int64_t k = 1; k <= std::max<int64_t>(1, nt / 2) && (k == 1 || waves * k <= 16384); k += k < 32 ? 1 : k / 8) {
+  const auto look = [&](int64_t k) {
     const double tiles = (double)((nt + k - 1) / k), join = k > kOwnJoin ? 0.0 : (double)k * (7.5 * n + 30);
-    double t = pass_time((double)(waves * k), occ, 500 + join, tiles * main, ragged);
-    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4, 500, tiles * ends, ragged) + 1100;
+    double t = pass_time((double)(waves * k), held, 500 + join, tiles * main, ragged);
+    if (k > 1) t += pass_time((double)(waves * (k - 1)), 4096, 500, tiles * ends, ragged) + 1100;
     if (k > kOwnJoin) t += 1100 + 2700 + 0.1 * n * (double)(waves * k);
     if (k == 1 || t < best) best = t, K = k;
-  }
+  };
+  for (int64_t k = 1; k <= most && (k == 1 || waves * k <= 16384); k += k < 32 ? 1 : k / 8) look(k);
+  if (held / waves > 1) look(std::min(most, held / waves));  // as many as fill the card once
   return K;
 }
 
