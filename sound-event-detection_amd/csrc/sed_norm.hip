@@ -8,7 +8,7 @@
 // The gradient needs two sums a group, sum q and sum q n (q = du w, n the normalised value), which follow from the channels'
 // sums of du and du n: those are the bias' and the weight's gradients at the same time.
 // Two walks over a map are what a grid without a barrier can do: the second one goes backwards, so that what the memory-side
-// cache still holds is read from there.
+// cache still holds is read from there.  Groups small enough for one workgroup's registers are read once, in one launch.
 //
 // Measured (MI355X): 32 x 1001 x 64 x 64 bf16 SiLU (262 MB a map): statistics 59 us (4.4 TB/s), output 93 us (5.6 TB/s), the
 // gradient's sums 115 us (4.6 TB/s), the gradient 136 us (5.8 TB/s); a 1 GiB copy reaches 5.1.  Four walks of 8 clips each were no
@@ -144,27 +144,95 @@ __device__ __forceinline__ float block_sum(float v, float* s) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
+constexpr int kBlocks = 2048;  // of a clip at most, in the walk that leaves sums
+
+// Joins the blocks of a clip per channel, 16 channels a workgroup and a thread for every 64th block, all of which it holds: into the
+// first block's place, or the gradient's sums into `chan`.  For clips of more blocks and channels a group than one workgroup
+// joins in passing (1 x 1001 x 64 x 256 in one group: 1936 us by norm_join_kernel alone).
+template <bool BACK>
+__global__ void __launch_bounds__(1024) norm_channel_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  constexpr int W = 16, H = 1024 / W, HELD = kBlocks / H;
+  __shared__ float s_1[H][W + 1], s_2[H][W + 1];
+  const int lane = threadIdx.x % W, row = threadIdx.x / W;
+  const int64_t b = blockIdx.y, at = (int64_t)blockIdx.x * W + lane, c = std::min(at, a.C - 1), own = own_of(p, b);
+  float* part = p.part + b * p.blocks * 2 * a.C + c;
+  // sums over the rows, in pairs
+  const auto all = [&](float (&s)[H][W + 1], float v) {
+    s[row][lane] = v;
+    for (int half = H / 2; half >= 1; half /= 2) {
+      __syncthreads();
+      if (row < half) s[row][lane] += s[row + half][lane];
+    }
+    __syncthreads();
+    return s[0][lane];
+  };
+  float m[HELD], v[HELD], s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int k = row + h * H;
+    m[h] = v[h] = 0.0f;
+    if (k < p.blocks) {
+      m[h] = part[(int64_t)k * 2 * a.C];
+      v[h] = part[(int64_t)k * 2 * a.C + a.C];
+    }
+  }
+  if constexpr (BACK) {
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      s1 += m[h];
+      s2 += v[h];
+    }
+    s1 = all(s_1, s1);
+    s2 = all(s_2, s2);
+    if (row == 0 && at < a.C) {
+      p.chan[b * 2 * a.C + c] = s1;
+      p.chan[b * 2 * a.C + a.C + c] = s2;
+    }
+  } else {
+    if (own <= 0) return;
+    const float first = part[(int64_t)(p.blocks - 1) * 2 * a.C];  // the last block always has places
+    float n[HELD];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+      const int k = row + h * H;
+      n[h] = k < p.blocks ? (float)(part_begin(p.blocks, own, k + 1) - part_begin(p.blocks, own, k)) : 0.0f;
+      if (n[h] > 0.0f) s1 = fmaf(n[h], m[h] - first, s1);  // a block without places has written nothing
+    }
+    const float mean = first + all(s_1, s1) / (float)own;
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (n[h] > 0.0f) s2 += fmaf(n[h] * (m[h] - mean), m[h] - mean, v[h]);
+    s2 = all(s_2, s2);
+    if (row == 0 && at < a.C) {
+      part[0] = mean;
+      part[a.C] = s2;
+    }
+  }
+}
+
 // mean and rstd of a (clip, group) out of the blocks' channels: the mean first, then the squares about it, so that neither a far
-// mean nor an odd block costs digits.  HELD: each thread has at most HELD entries and keeps them; 0: they are read twice.
-template <int HELD>
+// mean nor an odd block costs digits.  HELD: each thread has at most HELD entries and keeps them; 0: they are read twice.  JOINED: the
+// blocks are joined already.
+template <int HELD, bool JOINED>
 __global__ void __launch_bounds__(256) norm_join_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   __shared__ float s[4];
   const int g = blockIdx.x % (int)a.G, b = blockIdx.x / (int)a.G, cg = (int)(a.C / a.G);
   const int64_t own = own_of(p, b);
-  const int n = p.blocks * cg;  // entries
+  const int n = JOINED ? cg : p.blocks * cg;  // entries
   const float total = (float)own * (float)cg;
   const float* part = p.part + (int64_t)b * p.blocks * 2 * a.C + g * cg;
   float mean = 0.0f, var = 0.0f;
   if (own > 0) {
     const auto entry = [&](int i, float& count, float& m, float& v) {
-      const int q = i / cg;
+      const int q = JOINED ? 0 : i / cg;
       const float* at = part + (int64_t)q * 2 * a.C + (i - q * cg);
-      count = (float)(part_begin(p.blocks, own, q + 1) - part_begin(p.blocks, own, q));
+      count = JOINED ? (float)own : (float)(part_begin(p.blocks, own, q + 1) - part_begin(p.blocks, own, q));
       m = count > 0.0f ? at[0] : 0.0f;  // a block without places has written nothing
       v = count > 0.0f ? at[a.C] : 0.0f;
     };
-    const float k = part[(int64_t)(p.blocks - 1) * 2 * a.C];  // means relative to one of them (the last block always has places)
+    const float k = part[JOINED ? 0 : (int64_t)(p.blocks - 1) * 2 * a.C];  // means relative to one of them (the last block always has places)
     float w = 0.0f, count[HELD ? HELD : 1], m[HELD ? HELD : 1], v[HELD ? HELD : 1];
     if constexpr (HELD > 0) {
 #pragma unroll
@@ -280,6 +348,89 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(const NormParams p) {
   for (int64_t r = q.z0 + q.ty; r < q.z1; r += q.step) store_n<T, V, VEC>(y + r * a.C, V, zero);
 }
 
+// A (clip, group) whose values fit into a workgroup's registers: read once, its statistics taken there, written.  Lanes along the
+// group's channels, V of them each, then along the places; the sums are relative to the group's first value, the squares to the
+// mean that they give, and what that mean is off by is put right in both.  Groups of a clip lie side by side in memory: workgroups
+// are counted so that an XCD has whole clips and its L2 the lines that two groups share.  Bound by latency or, in large batches, by
+// HBM: 1 x 101 x 64 x 32 fp32 11 us (three launches of the walks: 13), 512 x 100 x 256 bf16 18 us (41), 2000 x 200 x 256 bf16 in 8
+// groups 99 us for 410 MB, 4.1 TB/s (145).
+template <class T, int V, int HELD, int ACT>
+__global__ void __launch_bounds__(1024) norm_whole_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  typedef T vt __attribute__((ext_vector_type(V)));
+  __shared__ float s[2][16];
+  const unsigned item = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  if (item >= a.B * a.G) return;
+  const int b = item / (unsigned)a.G, g = item % (unsigned)a.G, cg = (int)(a.C / a.G);
+  const int nv = cg / V, tx = threadIdx.x % nv, ty = threadIdx.x / nv, step = blockDim.x / nv, waves = (blockDim.x + 63) / 64;
+  const int own = (int)own_of(p, b), mine = ty < step ? own : 0;  // places; of this lane
+  const int64_t c = g * cg + tx * V, at = b * p.S * a.C + c;
+  const T* x = static_cast<const T*>(a.x) + at;
+  T* y = static_cast<T*>(a.y) + at;
+  vt v[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int r = ty + h * step;
+    if (r < mine) v[h] = *reinterpret_cast<const vt*>(x + r * a.C);
+  }
+  float w[V], bias[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    w[i] = a.weight ? a.weight[c + i] : 1.0f;
+    bias[i] = a.bias ? a.bias[c + i] : 0.0f;
+  }
+  const auto all = [&](float t, float* to) {
+    t = wave_sum(t);
+    if (threadIdx.x % 64 == 0) to[threadIdx.x / 64] = t;
+    __syncthreads();
+    t = 0.0f;
+    for (int i = 0; i < waves; ++i) t += to[i];
+    return t;
+  };
+  const float k = own > 0 ? (float)static_cast<const T*>(a.x)[b * p.S * a.C + g * cg] : 0.0f;
+  const float inv = own > 0 ? 1.0f / ((float)own * (float)cg) : 0.0f;
+  float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h)
+    if (ty + h * step < mine)
+#pragma unroll
+      for (int i = 0; i < V; ++i) s1 += (float)v[h][i] - k;
+  float mean = fmaf(all(s1, s[0]), inv, k);
+  s1 = 0.0f;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h)
+    if (ty + h * step < mine)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float e = (float)v[h][i] - mean;
+        s1 += e;
+        s2 = fmaf(e, e, s2);
+      }
+  __syncthreads();
+  const float off = all(s1, s[0]) * inv, var = fmaf(all(s2, s[1]), inv, -off * off);
+  mean += off;
+  const float rstd = 1.0f / sqrtf(std::max(var, 0.0f) + a.eps);
+  if (threadIdx.x == 0) {
+    a.mean[item] = mean;
+    a.rstd[item] = rstd;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] *= rstd;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int r = ty + h * step;
+    if (r < mine) {
+      float u[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) u[i] = act<ACT>(fmaf((float)v[h][i] - mean, w[i], bias[i]));
+      store_n<T, V, true>(y + r * a.C, V, u);
+    }
+  }
+  const float zero[V] = {};
+  if (ty < step)
+    for (int64_t r = own + ty; r < p.S; r += step) store_n<T, V, true>(y + r * a.C, V, zero);
+}
+
 template <class T, int V, bool VEC, int ACT>
 __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
@@ -329,7 +480,8 @@ __global__ void __launch_bounds__(256) norm_grad_sums_kernel(const NormParams p)
 }
 
 // A clip's channels over its blocks, and the group's two means.  A channel has 256 / cg lanes, which take the blocks in
-// turn; their sums are added in order.
+// turn; their sums are added in order.  JOINED: the channels' sums are there already.
+template <bool JOINED>
 __global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormParams p) {
   const sed_norm_args& a = p.a;
   __shared__ float s[4], s_1[256], s_2[256];
@@ -341,7 +493,7 @@ __global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormParams p)
   for (int i = col; i - col < cg; i += wide) {
     const int64_t c = (int64_t)g * cg + i;
     float s1 = 0.0f, s2 = 0.0f;
-    if (i < cg && lane < lanes) {
+    if (!JOINED && i < cg && lane < lanes) {
       const float* part = p.part + (int64_t)b * p.blocks * 2 * a.C + c;
 #pragma unroll 4
       for (int k = lane; k < p.blocks; k += lanes) {
@@ -349,17 +501,25 @@ __global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormParams p)
         s2 += part[(int64_t)k * 2 * a.C + a.C];
       }
     }
-    __syncthreads();
-    s_1[threadIdx.x] = s1;
-    s_2[threadIdx.x] = s2;
-    __syncthreads();
+    if (!JOINED) {
+      __syncthreads();
+      s_1[threadIdx.x] = s1;
+      s_2[threadIdx.x] = s2;
+      __syncthreads();
+    }
     if (i < cg && lane == 0) {
-      for (int k = 1; k < lanes; ++k) {
-        s1 += s_1[k * wide + col];
-        s2 += s_2[k * wide + col];
+      float* chan = p.chan + (int64_t)b * 2 * a.C + c;
+      if (JOINED) {
+        s1 = chan[0];
+        s2 = chan[a.C];
+      } else {
+        for (int k = 1; k < lanes; ++k) {
+          s1 += s_1[k * wide + col];
+          s2 += s_2[k * wide + col];
+        }
+        chan[0] = s1;
+        chan[a.C] = s2;
       }
-      p.chan[(int64_t)b * 2 * a.C + c] = s1;
-      p.chan[(int64_t)b * 2 * a.C + a.C + c] = s2;
       const float w = a.weight ? a.weight[c] : 1.0f;
       q1 = fmaf(w, s1, q1);
       q2 = fmaf(w, s2, q2);
@@ -448,7 +608,7 @@ Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   Layout l{};
   const int64_t least = std::max<int64_t>(32, 4096 / C);
   const auto blocks = [&](int64_t most) { return (int32_t)std::max<int64_t>(1, std::min<int64_t>((S + least - 1) / least, most / std::max<int64_t>(1, B))); };
-  l.blocks = blocks(2048);
+  l.blocks = blocks(kBlocks);
   l.late = blocks(8192);
   int64_t at = 0;
   const auto take = [&](int64_t k) { const int64_t o = at; at += (k + 63) / 64 * 64; return o; };
@@ -459,21 +619,70 @@ Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   return l;
 }
 
+// Threads of norm_whole_kernel for lanes of V channels and `held` rows, or 0 where it does not fit or is slower: 8 rows a lane (more
+// registers, more code) beyond a workgroup a compute unit (64 x 862 x 768 bf16: 71 us, the walks 68; 16 x 101 x 64 x 32 fp32 15 us, 17);
+// pieces of lines under 32 bytes in maps beyond 64 MB (fp32, 4 channels a group: 106 MB 62 us, the walks 57; 212 MB 146, 116; but 33
+// MB 23, 28).  Many groups: as few threads as hold one, so that a compute unit has several; else all, for the shortest way through.
+int whole_threads(const NormParams& p, int V, int held) {
+  const sed_norm_args& a = p.a;
+  const int64_t cg = a.C / a.G, nv = cg / V, items = a.B * a.G;
+  if (cg % V || nv > 1024 || p.S > held * (1024 / nv)) return 0;
+  if (held > 4 && items > 256) return 0;
+  const int64_t size = a.dtype == SED_F32 ? 4 : 2;
+  if (cg * size < 32 && a.B * p.S * a.C * size > (64 << 20)) return 0;
+  int threads = 1024;
+  if (items >= 512)
+    while (threads > 256 && nv <= threads / 2 && p.S <= held * (threads / 2 / nv)) threads /= 2;
+  return (int)std::min<int64_t>(threads, (p.S * nv + 63) / 64 * 64);
+}
+
+template <class T, int V, int HELD, int ACT>
+int launch_whole(const NormParams& p, int threads, hipStream_t s) {
+  const int64_t grid = (p.a.B * p.a.G + 7) / 8 * 8;
+  if (!grid_fits(grid, threads)) return SED_ERR_CAPACITY;
+  norm_whole_kernel<T, V, HELD, ACT><<<(unsigned)grid, threads, 0, s>>>(p);
+  return seq_status(hipGetLastError());
+}
+
 template <class T, int V, bool VEC, int ACT>
 int launch(const NormParams& p, bool back, hipStream_t s) {
   const sed_norm_args& a = p.a;
+  if constexpr (VEC) {
+    if (!back) {
+      if (const int n = whole_threads(p, V, 4)) return launch_whole<T, V, 4, ACT>(p, n, s);
+      if (const int n = whole_threads(p, V, 8)) return launch_whole<T, V, 8, ACT>(p, n, s);
+      if constexpr (V == 8) {
+        if (const int n = whole_threads(p, 4, 4)) return launch_whole<T, 4, 4, ACT>(p, n, s);
+        if (const int n = whole_threads(p, 4, 8)) return launch_whole<T, 4, 8, ACT>(p, n, s);
+      }
+    }
+  }
   const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb)), late((unsigned)p.late, grid.y, grid.z);
+  // more blocks and channels a group than a workgroup joins in 8 steps: a launch of its own for the blocks
+  const int64_t cg = a.C / a.G;
+  const bool far = p.blocks * cg > 8 * 256, many = far && p.blocks > 1;
+  const dim3 channels((unsigned)((a.C + 15) / 16), grid.y);
   const unsigned groups = (unsigned)(a.B * a.G), threads = (unsigned)((256 / p.nb * p.nb + 63) / 64 * 64);
   if (!back) {
     norm_stats_kernel<T, V, VEC><<<grid, threads, 0, s>>>(p);
-    if ((int64_t)p.blocks * (a.C / a.G) <= 8 * 256)
-      norm_join_kernel<8><<<groups, 256, 0, s>>>(p);
-    else
-      norm_join_kernel<0><<<groups, 256, 0, s>>>(p);
+    if (!far) {
+      norm_join_kernel<8, false><<<groups, 256, 0, s>>>(p);
+    } else {
+      if (many) norm_channel_kernel<false><<<channels, 1024, 0, s>>>(p);
+      if (cg <= 8 * 256)
+        norm_join_kernel<8, true><<<groups, 256, 0, s>>>(p);
+      else
+        norm_join_kernel<0, true><<<groups, 256, 0, s>>>(p);
+    }
     norm_apply_kernel<T, V, VEC, ACT><<<late, threads, 0, s>>>(p);
   } else {
     norm_grad_sums_kernel<T, V, VEC, ACT><<<grid, threads, 0, s>>>(p);
-    norm_grad_join_kernel<<<groups, 256, 0, s>>>(p);
+    if (!many) {
+      norm_grad_join_kernel<false><<<groups, 256, 0, s>>>(p);
+    } else {
+      norm_channel_kernel<true><<<channels, 1024, 0, s>>>(p);
+      norm_grad_join_kernel<true><<<groups, 256, 0, s>>>(p);
+    }
     norm_grad_kernel<T, V, VEC, ACT><<<late, threads, 0, s>>>(p);
     if (a.dw || a.db) norm_param_kernel<<<(unsigned)((2 * a.C + 255) / 256), 256, 0, s>>>(p);
   }

@@ -494,6 +494,24 @@ def test_norm_long_walks(shape, groups, act):
         _norm_case(shape, groups, dtype, act=act, seed=7, frames=[shape[1] - 5, 2][:shape[0]] if shape[3:] else None)
 
 
+@pytest.mark.parametrize("dtype", ("fp32", "bf16", "fp16"))
+@pytest.mark.parametrize("shape,groups", (((1, 1, 8), 1), ((2, 1, 1, 4), 1), ((3, 7, 24), 1), ((1, 101, 3, 32), 8), ((2, 33, 96), 2), ((600, 3, 16), 2),
+                                          ((1, 4, 4096), 1), ((1, 9, 6156), 3), ((1, 8, 4104), 2), ((130, 40, 16), 4), ((5, 257, 48), 1), ((1, 2049, 4), 1)))
+def test_norm_groups_held_whole(shape, groups, dtype):
+    """Groups that one workgroup holds, at the ends of what it holds, with lengths of their own and without."""
+    n = shape[1]
+    _norm_case(shape, groups, DTYPES[dtype], act="silu", seed=sum(shape), frames=[(n, 0, 1, n - 1, n + 3, -1)[i % 6] for i in range(shape[0])])
+    _norm_case(shape, groups, DTYPES[dtype], act=None, seed=n, mean=100.0 if dtype == "fp32" else 3.0, affine=n % 2 == 0)
+
+
+@pytest.mark.parametrize("shape,groups", (((1, 2000, 64), 1), ((1, 300, 1200), 1), ((2, 700, 520), 1), ((1, 150, 3, 2052), 1), ((1, 6000, 40), 2)))
+def test_norm_groups_of_many_blocks(shape, groups):
+    """Blocks and channels a group that are joined by a launch of their own; clips that leave blocks without a place."""
+    for dtype in (torch.float32, torch.bfloat16):
+        _norm_case(shape, groups, dtype, act="silu", seed=sum(shape))
+        _norm_case(shape, groups, dtype, act=None, seed=3, frames=[5, shape[1]][:shape[0]], mean=10.0)
+
+
 @pytest.mark.parametrize("act", (None, "silu", "relu", "gelu"))
 @pytest.mark.parametrize("affine", (True, False))
 def test_norm_activations(act, affine):
