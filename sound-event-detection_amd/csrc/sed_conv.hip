@@ -261,33 +261,17 @@ __global__ void __launch_bounds__(256) conv_state_grad_kernel(const sed_conv_arg
   static_cast<T*>(a.dstate)[q] = rounded<T>(s);
 }
 
-// dw [D][W] and db [D] out of the runs' sums [rows][W + 1][D], a thread for every 4th row, added in order.
-__global__ void __launch_bounds__(1024) conv_param_kernel(const ConvParams p) {
+// dw [D][W] and db [D] out of the runs' sums [rows][W + 1][D].
+__global__ void __launch_bounds__(1024) conv_param_kernel(const ConvParams p, int64_t rows, int64_t step) {
   const sed_conv_args& a = p.a;
-  __shared__ float s[16][64];
-  const int64_t cols = (int64_t)(a.W + 1) * a.D, c = (int64_t)blockIdx.x * 64 + threadIdx.x % 64;
-  const int ty = threadIdx.x / 64;
-  const int64_t rows = a.B * p.runs;
-  float v[4] = {0, 0, 0, 0};
-  if (c < cols) {
-    int64_t r = ty;
-    for (; r + 48 < rows; r += 64)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += p.part[(r + 16 * k) * cols + c];
-    for (; r < rows; r += 16) v[0] += p.part[r * cols + c];
-  }
-  s[ty][threadIdx.x % 64] = (v[0] + v[1]) + (v[2] + v[3]);
-  __syncthreads();
-  if (ty == 0 && c < cols) {
-    float t = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 16; ++k) t += s[k][threadIdx.x];
-    const int64_t k = c / a.D, d = c % a.D;
-    if (k < a.W)
-      a.dw[d * a.W + k] = t;
-    else if (a.db)
-      a.db[d] = t;
-  }
+  const int64_t cols = (int64_t)(a.W + 1) * a.D, c = (int64_t)blockIdx.x * kColumns + threadIdx.x % kColumns;
+  const float t = column_sum(p.part + c, rows, step, c < cols);
+  if (threadIdx.x >= kColumns || c >= cols) return;
+  const int64_t k = c / a.D, d = c % a.D;
+  if (k < a.W)
+    a.dw[d * a.W + k] = t;
+  else if (a.db)
+    a.db[d] = t;
 }
 
 // One frame: the state moves up by a row in place.  A thread owns V channels of a stream.
@@ -375,7 +359,10 @@ int launch_backward(const ConvParams& p, hipStream_t s) {
     conv_backward_kernel<T, V, WM, SED_ACT_SILU><<<(unsigned)grid, 64, 0, s>>>(p);
   else
     conv_backward_kernel<T, V, WM, SED_ACT_NONE><<<(unsigned)grid, 64, 0, s>>>(p);
-  conv_param_kernel<<<(unsigned)(((a.W + 1) * a.D + 63) / 64), 1024, 0, s>>>(p);
+  const int64_t cols = (a.W + 1) * a.D;
+  int64_t rows = a.B * p.runs, step = cols;
+  fold_rows(p.part, rows, step, cols, s);
+  conv_param_kernel<<<(unsigned)((cols + kColumns - 1) / kColumns), 1024, 0, s>>>(p, rows, step);
   return seq_status(hipGetLastError());
 }
 

@@ -533,14 +533,12 @@ __global__ void __launch_bounds__(256) norm_grad_join_kernel(const NormParams p)
   }
 }
 
-// dw and db: the clips' channels, added in order.
-__global__ void __launch_bounds__(256) norm_param_kernel(const NormParams p) {
+// dw and db: the clips' channels.
+__global__ void __launch_bounds__(1024) norm_param_kernel(const NormParams p, int64_t rows, int64_t step) {
   const sed_norm_args& a = p.a;
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= 2 * a.C) return;
-  float v = 0.0f;
-#pragma unroll 4
-  for (int64_t b = 0; b < a.B; ++b) v += p.chan[b * 2 * a.C + c];
+  const int64_t c = (int64_t)blockIdx.x * kColumns + threadIdx.x % kColumns;
+  const float v = column_sum(p.chan + c, rows, step, c < 2 * a.C);
+  if (threadIdx.x >= kColumns || c >= 2 * a.C) return;
   if (c < a.C) {
     if (a.db) a.db[c] = v;
   } else if (a.dw) {
@@ -684,7 +682,11 @@ int launch(const NormParams& p, bool back, hipStream_t s) {
       norm_grad_join_kernel<true><<<groups, 256, 0, s>>>(p);
     }
     norm_grad_kernel<T, V, VEC, ACT><<<late, threads, 0, s>>>(p);
-    if (a.dw || a.db) norm_param_kernel<<<(unsigned)((2 * a.C + 255) / 256), 256, 0, s>>>(p);
+    if (a.dw || a.db) {
+      int64_t rows = a.B, step = 2 * a.C;
+      fold_rows(p.chan, rows, step, 2 * a.C, s);
+      norm_param_kernel<<<(unsigned)((2 * a.C + kColumns - 1) / kColumns), 1024, 0, s>>>(p, rows, step);
+    }
   }
   return seq_status(hipGetLastError());
 }

@@ -971,31 +971,14 @@ __global__ void __launch_bounds__(256) scan_bc_kernel(const ScanParams p, int NP
   static_cast<T*>(e < NP ? a.dB : a.dC)[((b * a.L + t) * a.G + g) * a.N + n] = (T)v;
 }
 
-// dA [D][N], d skip and d dt_bias [D]: sums over clips and chunks; dA's partial sums lie [NP][D].  A block has 64 columns and
-// 16 lanes for each, which take every 16th row; they are added in order.
-__global__ void __launch_bounds__(1024) scan_param_kernel(const ScanParams p, int NP) {
+// dA [D][N], d skip and d dt_bias [D]: sums over clips and chunks; dA's partial sums lie [NP][D].
+__global__ void __launch_bounds__(1024) scan_param_kernel(const ScanParams p, int64_t rows_a, int64_t step_a, int64_t rows_d, int64_t step_d) {
   const sed_scan_args& a = p.a;
-  __shared__ float s[16][64];
-  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x % 64, rows = a.B * p.K;
-  const int ty = threadIdx.x / 64;
-  const int64_t d = i % a.D, n = i / a.D;
+  const int64_t i = (int64_t)blockIdx.x * kColumns + threadIdx.x % kColumns, d = i % a.D, n = i / a.D;
   const bool live = n < a.N + 2;
-  float v[4] = {0, 0, 0, 0};
-  if (live) {
-    const float* q = n < a.N ? p.part_a + n * a.D + d : p.part_d + (n - a.N) * a.D + d;
-    const int64_t step = n < a.N ? (int64_t)NP * a.D : 2 * a.D;
-    int64_t r = ty;
-    for (; r + 48 < rows; r += 64)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] += q[(r + 16 * k) * step];
-    for (; r < rows; r += 16) v[0] += q[r * step];
-  }
-  s[ty][threadIdx.x % 64] = (v[0] + v[1]) + (v[2] + v[3]);
-  __syncthreads();
-  if (ty != 0 || !live) return;
-  float sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 16; ++k) sum += s[k][threadIdx.x];
+  const float* q = n < a.N ? p.part_a + n * a.D + d : p.part_d + (n - a.N) * a.D + d;
+  const float sum = column_sum(q, n < a.N ? rows_a : rows_d, n < a.N ? step_a : step_d, live);
+  if (threadIdx.x >= kColumns || !live) return;
   if (n < a.N)
     a.dA[d * a.N + n] = sum;
   else if (n == a.N) {
@@ -1122,7 +1105,7 @@ int64_t chunks_of(const sed_scan_args& a, const Shape& s, int64_t waves, int64_t
     if (k == 1 || t < best) best = t, K = k;
   };
   for (int64_t k = 1; k <= most && (k == 1 || waves * k <= 16384); k += k < 32 ? 1 : k / 8) look(k);
-  if (held / waves > 1) look(std::min(most, held / waves));  // as many as fill the card once
+  if (waves > 0 && held / waves > 1) look(std::min(most, held / waves));  // as many as fill the card once
   return K;
 }
 
@@ -1199,15 +1182,18 @@ int launch(const ScanParams& p, hipStream_t stream) {
     }
     scan_forward_kernel<NS, SPLIT, T, VEC, false><<<main, 64 * WM, 0, stream>>>(p);
   } else {
-    const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + 63) / 64;
-    if (!grid_fits(bc, 256)) return SED_ERR_CAPACITY;
+    const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + kColumns - 1) / kColumns;
+    if (!grid_fits(bc, 256) || !grid_fits(pr, 1024)) return SED_ERR_CAPACITY;
     if (p.K > 1) {
       scan_backward_kernel<NS, SPLIT, T, VEC, true><<<ends, 64 * WE, 0, stream>>>(p);
       launch_join<G, true>(p, stream);
     }
     scan_backward_kernel<NS, SPLIT, T, VEC, false><<<main, 64 * WM, 0, stream>>>(p);
     scan_bc_kernel<T><<<(unsigned)bc, 256, 0, stream>>>(p, G::NP);
-    scan_param_kernel<<<(unsigned)pr, 1024, 0, stream>>>(p, G::NP);
+    int64_t rows_a = a.B * p.K, step_a = G::NP * a.D, rows_d = rows_a, step_d = 2 * a.D;
+    fold_rows(p.part_a, rows_a, step_a, a.N * a.D, stream);
+    fold_rows(p.part_d, rows_d, step_d, 2 * a.D, stream);
+    scan_param_kernel<<<(unsigned)pr, 1024, 0, stream>>>(p, rows_a, step_a, rows_d, step_d);
   }
   return seq_status(hipGetLastError());
 }

@@ -3,6 +3,7 @@
 #pragma once
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
 
 #include "sed_hip.h"
@@ -159,6 +160,53 @@ __device__ __forceinline__ float wave_sum(float x) {
   x = row_sum(x);
   x = fold16(x, x);
   return fold32(x, x);
+}
+
+// Sum of a column of `rows` values that lie `step` apart, for kColumns columns of a workgroup of 1024 threads: 16 threads a column
+// take every 16th row, 8 of them on the way at once, and are added in order.  All threads call it; the sum is there for the first
+// kColumns.
+constexpr int kColumns = 64;
+__device__ __forceinline__ float column_sum(const float* q, int64_t rows, int64_t step, bool live) {
+  constexpr int H = 1024 / kColumns;
+  __shared__ float s[H][kColumns];
+  const int col = threadIdx.x % kColumns, row = threadIdx.x / kColumns;
+  float v[8] = {};
+  int64_t r = row;
+  if (live) {
+    for (; r + 7 * H < rows; r += 8 * H)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[k] += q[(r + k * H) * step];
+#pragma unroll
+    for (int k = 0; k < 7; ++k) {  // every load is in bounds, so none waits for another's condition
+      const float t = q[std::min(r + k * H, rows - 1) * step];
+      v[k] += r + k * H < rows ? t : 0.0f;
+    }
+  }
+  s[row][col] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+  __syncthreads();
+  float sum = 0.0f;
+  if (row == 0)
+#pragma unroll
+    for (int k = 0; k < H; ++k) sum += s[k][col];
+  return sum;
+}
+
+// Sums parts of `per` rows into the first row of each.
+static __global__ void __launch_bounds__(1024) fold_rows_kernel(float* base, int64_t rows, int64_t step, int64_t cols, int64_t per) {
+  const int64_t c = (int64_t)blockIdx.x * kColumns + threadIdx.x % kColumns, r0 = blockIdx.y * per;
+  float* q = base + r0 * step + c;
+  const float sum = column_sum(q, std::min(per, rows - r0), step, c < cols);
+  if (threadIdx.x < kColumns && c < cols) *q = sum;  // behind column_sum's barrier nobody reads this part any more
+}
+// Many rows of few columns would keep a few workgroups busy for long: parts of them are summed in place first, and rows and step
+// become those of the parts' sums (65536 rows of 80 columns: 360 us in one go).
+inline void fold_rows(float* base, int64_t& rows, int64_t& step, int64_t cols, hipStream_t s) {
+  const int64_t wide = (cols + kColumns - 1) / kColumns, most = std::min<int64_t>(rows / 256, 1024 / wide);
+  if (rows <= 2048 || most < 2) return;
+  const int64_t per = (rows + most - 1) / most, parts = (rows + per - 1) / per;
+  fold_rows_kernel<<<dim3((unsigned)wide, (unsigned)parts), 1024, 0, s>>>(base, rows, step, cols, per);
+  rows = parts;
+  step *= per;
 }
 
 // A launch has fewer than 2^32 threads along an axis.

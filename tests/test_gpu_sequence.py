@@ -127,6 +127,16 @@ def test_scan_many_waves_stay_whole():
     _scan_case(260, 20, 256, 1, 16, torch.bfloat16, seed=3, frames=[(7 * i) % 21 for i in range(260)], reverse=True)
 
 
+def test_parameter_gradients_of_many_clips():
+    """More clips than one pass over their sums takes, a last part of other size among them."""
+    _scan_case(2053, 3, 4, 1, 4, torch.float32, seed=11)
+    _scan_case(4999, 1, 6, 2, 3, torch.bfloat16, seed=12)
+    _conv_case(2050, 2, 5, 4, torch.float32, seed=13)
+    _conv_case(5001, 1, 72, 2, torch.bfloat16, seed=14)
+    _norm_case((2051, 2, 8), 2, torch.float32, seed=15)
+    _norm_case((4500, 3, 40), 5, torch.bfloat16, seed=16)
+
+
 @pytest.mark.parametrize("nb", (2, 63, 64, 65, 130))
 def test_scan_orders_of_clips(nb):
     """Every clip is walked once whatever the order of lengths: equal ones, none, rising and falling, past the ends, more than 64 clips."""

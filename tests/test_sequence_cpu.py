@@ -150,3 +150,19 @@ def test_python_entry_points_refuse_cpu_tensors():
         sed_amd.causal_conv_step(torch.zeros(1, 3, 8), x[:, 0], torch.zeros(8, 4))
     with pytest.raises(RuntimeError, match="no CPU path"):
         sed_amd.group_norm_act(x, 2)
+
+
+def test_workspaces_of_empty_and_of_large_calls():
+    """Host arithmetic only: no clip, no frame, one wave and more waves than the card holds; never negative, never less for a gradient."""
+    from ctypes import byref
+    from sed_amd import _lib as L
+    for B in (0, 1, 2, 63, 5000):
+        for n in (0, 1, 9, 700, 100000):
+            for N in (1, 4, 8, 16, 17):
+                for dtype in (L.F32, L.BF16):
+                    for ragged in (None, 16):
+                        a = L.ScanArgs(B=B, L=n, D=96, N=N, G=1, dtype=dtype, frames=ragged)
+                        forward, back = L.lib.sed_gated_scan_workspace(byref(a), 0), L.lib.sed_gated_scan_workspace(byref(a), 1)
+                        assert forward >= 0 and back >= 4 * B * n * 2 * N
+            assert L.lib.sed_causal_conv_workspace(B, n, 96, 4) >= 0
+            assert L.lib.sed_group_norm_workspace(B, n, 3, 96, 8) >= 0
