@@ -581,6 +581,115 @@ __global__ void __launch_bounds__(256) norm_grad_kernel(const NormParams p) {
   for (int64_t r = q.z0 + q.ty; r < q.z1; r += q.step) store_n<T, V, VEC>(dx + r * a.C, V, zero);
 }
 
+// The gradient of such a group in one launch: both maps' rows are read once; the channels' sums of du and du n go over the places in
+// pairs through LDS, their weighted sums over the channels to all.  512 x 100 x 256 bf16 42 us (four launches of the walks 66), 2000 x 200 x 256 bf16 in 8 groups 178 us
+// for 614 MB (232).
+template <class T, int V, int HELD, int ACT>
+__global__ void __launch_bounds__(1024) norm_whole_grad_kernel(const NormParams p) {
+  const sed_norm_args& a = p.a;
+  typedef T vt __attribute__((ext_vector_type(V)));
+  extern __shared__ float sums[];  // [threads][V + 1]
+  __shared__ float s[2][16];
+  const unsigned item = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  if (item >= a.B * a.G) return;
+  const int b = item / (unsigned)a.G, g = item % (unsigned)a.G, cg = (int)(a.C / a.G);
+  const int nv = cg / V, tx = threadIdx.x % nv, ty = threadIdx.x / nv, step = blockDim.x / nv, waves = (blockDim.x + 63) / 64;
+  const int own = (int)own_of(p, b), mine = ty < step ? own : 0;
+  const int64_t c = g * cg + tx * V, at = b * p.S * a.C + c;
+  const T *x = static_cast<const T*>(a.x) + at, *dy = static_cast<const T*>(a.dy) + at;
+  T* dx = static_cast<T*>(a.dx) + at;
+  vt v[HELD], e[HELD];
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int r = ty + h * step;
+    if (r < mine) {
+      v[h] = *reinterpret_cast<const vt*>(x + r * a.C);
+      e[h] = *reinterpret_cast<const vt*>(dy + r * a.C);
+    }
+  }
+  const float mean = a.mean[item], rstd = a.rstd[item];
+  float w[V], s1[V], s2[V], du[HELD][V];
+  {
+    float bias[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      w[i] = a.weight ? a.weight[c + i] : 1.0f;
+      bias[i] = a.bias ? a.bias[c + i] : 0.0f;
+      s1[i] = s2[i] = 0.0f;
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (ty + h * step < mine)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float n = ((float)v[h][i] - mean) * rstd;
+          du[h][i] = (float)e[h][i] * act_slope<ACT>(fmaf(n, w[i], bias[i]));
+          s1[i] += du[h][i];
+          s2[i] = fmaf(du[h][i], n, s2[i]);
+        }
+  }
+  // over the places: lane (tx, 0) gets its channels' sums
+  float(*const rows)[V + 1] = reinterpret_cast<float(*)[V + 1]>(sums);
+  const auto over_places = [&](float (&t)[V]) {
+    int half = 1;
+    while (2 * half < step) half *= 2;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) rows[threadIdx.x][i] = t[i];
+    for (; half >= 1; half /= 2) {
+      __syncthreads();
+      if (ty < half && ty + half < step)
+#pragma unroll
+        for (int i = 0; i < V; ++i) rows[threadIdx.x][i] += rows[threadIdx.x + half * nv][i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) t[i] = rows[threadIdx.x][i];
+  };
+  over_places(s1);
+  over_places(s2);
+  float q1 = 0.0f, q2 = 0.0f;
+  if (ty == 0) {
+    float* chan = p.chan + (int64_t)b * 2 * a.C + c;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      chan[i] = s1[i];
+      chan[a.C + i] = s2[i];
+      q1 = fmaf(w[i], s1[i], q1);
+      q2 = fmaf(w[i], s2[i], q2);
+    }
+  }
+  q1 = wave_sum(q1);
+  q2 = wave_sum(q2);
+  if (threadIdx.x % 64 == 0) {
+    s[0][threadIdx.x / 64] = q1;
+    s[1][threadIdx.x / 64] = q2;
+  }
+  __syncthreads();
+  q1 = q2 = 0.0f;
+  for (int i = 0; i < waves; ++i) {
+    q1 += s[0][i];
+    q2 += s[1][i];
+  }
+  const float scale = own > 0 ? rstd / ((float)own * (float)cg) : 0.0f;
+  q1 *= scale;
+  q2 *= scale;
+#pragma unroll
+  for (int i = 0; i < V; ++i) w[i] *= rstd;
+#pragma unroll
+  for (int h = 0; h < HELD; ++h) {
+    const int r = ty + h * step;
+    if (r < mine) {
+      float d[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) d[i] = fmaf(-((float)v[h][i] - mean) * rstd, q2, fmaf(du[h][i], w[i], -q1));
+      store_n<T, V, true>(dx + r * a.C, V, d);
+    }
+  }
+  const float zero[V] = {};
+  if (ty < step)
+    for (int64_t r = own + ty; r < p.S; r += step) store_n<T, V, true>(dx + r * a.C, V, zero);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------
 
 bool aligned(const void* p, int64_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
@@ -617,17 +726,18 @@ Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
   return l;
 }
 
-// Threads of norm_whole_kernel for lanes of V channels and `held` rows, or 0 where it does not fit or is slower: 8 rows a lane (more
-// registers, more code) beyond a workgroup a compute unit (64 x 862 x 768 bf16: 71 us, the walks 68; 16 x 101 x 64 x 32 fp32 15 us, 17);
-// pieces of lines under 32 bytes in maps beyond 64 MB (fp32, 4 channels a group: 106 MB 62 us, the walks 57; 212 MB 146, 116; but 33
-// MB 23, 28).  Many groups: as few threads as hold one, so that a compute unit has several; else all, for the shortest way through.
-int whole_threads(const NormParams& p, int V, int held) {
+// Threads of norm_whole_kernel (BACK: of norm_whole_grad_kernel) for lanes of V channels and `held` rows, or 0 where it does not fit
+// or is slower: 8 rows a lane (more registers, more code) beyond a workgroup a compute unit (64 x 862 x 768 bf16: 71 us, the walks 68;
+// 16 x 101 x 64 x 32 fp32 15 us, 17); pieces of lines under 32 bytes where more than 96 MB are read (4 channels a group of 256 x 101 x
+// 32 x 32: fp32 62 us, the walks 57, bf16 gradient 106, 73; but 64 x 125 x 16 x 64 fp32 23, 28 and gradient 37, 44).  Many groups: as
+// few threads as hold one, so that a compute unit has several; else all, for the shortest way through.
+int whole_threads(const NormParams& p, int V, int held, bool back) {
   const sed_norm_args& a = p.a;
   const int64_t cg = a.C / a.G, nv = cg / V, items = a.B * a.G;
   if (cg % V || nv > 1024 || p.S > held * (1024 / nv)) return 0;
   if (held > 4 && items > 256) return 0;
   const int64_t size = a.dtype == SED_F32 ? 4 : 2;
-  if (cg * size < 32 && a.B * p.S * a.C * size > (64 << 20)) return 0;
+  if (cg * size < 32 && a.B * p.S * a.C * size * (back ? 2 : 1) > (96 << 20)) return 0;
   int threads = 1024;
   if (items >= 512)
     while (threads > 256 && nv <= threads / 2 && p.S <= held * (threads / 2 / nv)) threads /= 2;
@@ -642,17 +752,39 @@ int launch_whole(const NormParams& p, int threads, hipStream_t s) {
   return seq_status(hipGetLastError());
 }
 
+int launch_param(const NormParams& p, hipStream_t s) {
+  const sed_norm_args& a = p.a;
+  if (a.dw || a.db) {
+    int64_t rows = a.B, step = 2 * a.C;
+    fold_rows(p.chan, rows, step, 2 * a.C, s);
+    norm_param_kernel<<<(unsigned)((2 * a.C + kColumns - 1) / kColumns), 1024, 0, s>>>(p, rows, step);
+  }
+  return seq_status(hipGetLastError());
+}
+
+template <class T, int V, int ACT>
+int launch_whole_grad(const NormParams& p, int threads, hipStream_t s) {
+  const int64_t grid = (p.a.B * p.a.G + 7) / 8 * 8;
+  if (!grid_fits(grid, threads)) return SED_ERR_CAPACITY;
+  norm_whole_grad_kernel<T, V, 4, ACT><<<(unsigned)grid, threads, threads * (V + 1) * 4, s>>>(p);
+  return launch_param(p, s);
+}
+
 template <class T, int V, bool VEC, int ACT>
 int launch(const NormParams& p, bool back, hipStream_t s) {
   const sed_norm_args& a = p.a;
   if constexpr (VEC) {
     if (!back) {
-      if (const int n = whole_threads(p, V, 4)) return launch_whole<T, V, 4, ACT>(p, n, s);
-      if (const int n = whole_threads(p, V, 8)) return launch_whole<T, V, 8, ACT>(p, n, s);
+      if (const int n = whole_threads(p, V, 4, false)) return launch_whole<T, V, 4, ACT>(p, n, s);
+      if (const int n = whole_threads(p, V, 8, false)) return launch_whole<T, V, 8, ACT>(p, n, s);
       if constexpr (V == 8) {
-        if (const int n = whole_threads(p, 4, 4)) return launch_whole<T, 4, 4, ACT>(p, n, s);
-        if (const int n = whole_threads(p, 4, 8)) return launch_whole<T, 4, 8, ACT>(p, n, s);
+        if (const int n = whole_threads(p, 4, 4, false)) return launch_whole<T, 4, 4, ACT>(p, n, s);
+        if (const int n = whole_threads(p, 4, 8, false)) return launch_whole<T, 4, 8, ACT>(p, n, s);
       }
+    } else {
+      if (const int n = whole_threads(p, V, 4, true)) return launch_whole_grad<T, V, ACT>(p, n, s);
+      if constexpr (V == 8)
+        if (const int n = whole_threads(p, 4, 4, true)) return launch_whole_grad<T, 4, ACT>(p, n, s);
     }
   }
   const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb)), late((unsigned)p.late, grid.y, grid.z);
@@ -682,11 +814,7 @@ int launch(const NormParams& p, bool back, hipStream_t s) {
       norm_grad_join_kernel<true><<<groups, 256, 0, s>>>(p);
     }
     norm_grad_kernel<T, V, VEC, ACT><<<late, threads, 0, s>>>(p);
-    if (a.dw || a.db) {
-      int64_t rows = a.B, step = 2 * a.C;
-      fold_rows(p.chan, rows, step, 2 * a.C, s);
-      norm_param_kernel<<<(unsigned)((2 * a.C + kColumns - 1) / kColumns), 1024, 0, s>>>(p, rows, step);
-    }
+    return launch_param(p, s);
   }
   return seq_status(hipGetLastError());
 }

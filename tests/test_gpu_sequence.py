@@ -514,6 +514,14 @@ def test_norm_groups_held_whole(shape, groups, dtype):
     _norm_case(shape, groups, DTYPES[dtype], act=None, seed=n, mean=100.0 if dtype == "fp32" else 3.0, affine=n % 2 == 0)
 
 
+@pytest.mark.parametrize("act", (None, "silu", "gelu"))
+@pytest.mark.parametrize("shape,groups,frames", (((3, 9000, 32), 4, (9000, 5, 4501)), ((1, 8300, 16), 2, None), ((2, 900, 3, 30), 6, (1, 900)), ((20, 1100, 128), 4, None)))
+def test_norm_groups_walked_twice(shape, groups, frames, act):
+    """Groups beyond one workgroup, whole vectors and single channels, with blocks that have no place and blocks of many rows."""
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        _norm_case(shape, groups, dtype, act=act, seed=17, frames=frames)
+
+
 @pytest.mark.parametrize("shape,groups", (((1, 2000, 64), 1), ((1, 300, 1200), 1), ((2, 700, 520), 1), ((1, 150, 3, 2052), 1), ((1, 6000, 40), 2)))
 def test_norm_groups_of_many_blocks(shape, groups):
     """Blocks and channels a group that are joined by a launch of their own; clips that leave blocks without a place."""
