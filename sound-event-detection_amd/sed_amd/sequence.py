@@ -36,6 +36,11 @@ def _rows(t):
     return t.contiguous()
 
 
+def _new(t):
+    """An output of t's shape and type, contiguous whatever t's strides."""
+    return None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _param(t):
     """A parameter as the kernels read it; its gradient comes back in the parameter's own type."""
     if t is None or (t.dtype is torch.float32 and t.is_contiguous()):
@@ -70,9 +75,9 @@ def _check_frames(what, frames, x):
         raise TypeError(f"{what}: frames: a contiguous int32 tensor with one entry per clip on x's device")
 
 
-def _workspace(nbytes, dev):
+def _workspace(nbytes, x):
     L.check(nbytes, "workspace")
-    return torch.empty(max(int(nbytes), 16), dtype=torch.uint8, device=dev)
+    return x.new_empty(max(int(nbytes), 16), dtype=torch.uint8)
 
 
 def _call(fn, args, dev, what):
@@ -108,8 +113,8 @@ def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, sta
     b, n_frames, d = x.shape
     n = B.shape[3]
     dev = x.device
-    y = torch.empty((b, n_frames, d), dtype=x.dtype, device=dev)
-    last = torch.empty((b, d, n), dtype=torch.float32, device=dev) if want_last else None
+    y = _new(x)
+    last = x.new_empty((b, d, n), dtype=torch.float32) if want_last else None
     saved = None
     if b == 0 or n_frames == 0:
         if want_last:
@@ -117,11 +122,11 @@ def _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, sta
         return y, last, saved
     a = _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state)
     if want_saved:
-        saved = torch.empty(L.lib.sed_gated_scan_saved_floats(b, n_frames, d, n), dtype=torch.float32, device=dev)
+        saved = x.new_empty(L.lib.sed_gated_scan_saved_floats(b, n_frames, d, n), dtype=torch.float32)
         a.saved = saved.data_ptr()
     nbytes = L.lib.sed_gated_scan_workspace(a, 0)
     if nbytes:
-        ws = _workspace(nbytes, dev)
+        ws = _workspace(nbytes, x)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
     a.y, a.h_last = y.data_ptr(), _ptr(last)
     _call(L.lib.sed_gated_scan_forward, a, dev, "sed_gated_scan_forward")
@@ -144,8 +149,7 @@ class _GatedScan(torch.autograd.Function):
         softplus, reverse = ctx.flags
         b, n_frames, d = x.shape
         dev = x.device
-        new = lambda t, dtype=None: None if t is None else torch.empty(t.shape, dtype=dtype or t.dtype, device=dev)  # noqa: E731
-        dx, ddt, dA, dB, dC, dD, dz, dbias, dstate = (new(t) for t in (x, dt, A, B, Cm, D, z, dt_bias, state))
+        dx, ddt, dA, dB, dC, dD, dz, dbias, dstate = (_new(t) for t in (x, dt, A, B, Cm, D, z, dt_bias, state))
         if b == 0 or n_frames == 0:
             for t in (dA, dD, dbias, dstate):
                 if t is not None:
@@ -161,7 +165,7 @@ class _GatedScan(torch.autograd.Function):
         a.dx, a.ddt, a.dz, a.dB, a.dC = dx.data_ptr(), ddt.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
         a.dA, a.dskip, a.ddt_bias, a.dh0 = dA.data_ptr(), _ptr(dD), _ptr(dbias), _ptr(dstate)
         nbytes = L.lib.sed_gated_scan_workspace(a, 1)
-        ws = _workspace(nbytes, dev)
+        ws = _workspace(nbytes, x)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
         _call(L.lib.sed_gated_scan_backward, a, dev, "sed_gated_scan_backward")
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None
@@ -235,7 +239,7 @@ def gated_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplu
     if not state.is_contiguous():
         raise ValueError(f"{what}: state is updated in place and has to be contiguous")
     _no_grad_only(what, state, x, dt, A, B, C, D, z, dt_bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _new(x)
     if x.shape[0] == 0:
         return y
     x, dt, z, B, C = (_rows(t) for t in (x, dt, z, B, C))
@@ -261,8 +265,8 @@ def _conv_args(x, weight, bias, act, frames, reverse, state):
 
 def _conv_forward(x, weight, bias, act, frames, reverse, state, want_last):
     b, n_frames, d = x.shape
-    y = torch.empty((b, n_frames, d), dtype=x.dtype, device=x.device)
-    last = torch.empty((b, weight.shape[1] - 1, d), dtype=x.dtype, device=x.device) if want_last else None
+    y = _new(x)
+    last = x.new_empty((b, weight.shape[1] - 1, d)) if want_last else None
     if b == 0 or n_frames == 0:
         if want_last:
             last.zero_() if state is None else last.copy_(state)
@@ -289,7 +293,7 @@ class _CausalConv(torch.autograd.Function):
         act, reverse = ctx.flags
         b, n_frames, d = x.shape
         dev = x.device
-        dx, dw, db, dstate = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (x, weight, bias, state))
+        dx, dw, db, dstate = (_new(t) for t in (x, weight, bias, state))
         if b == 0 or n_frames == 0:
             for t in (dw, db, dstate):
                 if t is not None:
@@ -303,7 +307,7 @@ class _CausalConv(torch.autograd.Function):
         a.dy, a.dy_b, a.dy_t, a.dstate_out = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
         a.dx, a.dw, a.db, a.dstate = dx.data_ptr(), dw.data_ptr(), _ptr(db), _ptr(dstate)
         nbytes = L.lib.sed_causal_conv_workspace(b, n_frames, d, weight.shape[1])
-        ws = _workspace(nbytes, dev)
+        ws = _workspace(nbytes, x)
         a.ws, a.ws_bytes = ws.data_ptr(), nbytes
         _call(L.lib.sed_causal_conv_backward, a, dev, "sed_causal_conv_backward")
         return dx, dw, db, dstate, None, None, None, None
@@ -354,7 +358,7 @@ def causal_conv_step(state, x, weight, bias=None, activation=None):
     if not state.is_contiguous():
         raise ValueError(f"{what}: state is updated in place and has to be contiguous")
     _no_grad_only(what, state, x, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = _new(x)
     if x.shape[0] == 0:
         return y
     x, weight, bias = _rows(x), _param(weight), _param(bias)
@@ -374,18 +378,18 @@ def _norm_args(x, shape, groups, weight, bias, act, eps, frames, stats, y, ws):
                       at + 4 * shape[0] * groups, None, None, None, None, ws[1].data_ptr(), ws[0])
 
 
-def _norm_workspace(shape, groups, dev):
+def _norm_workspace(shape, groups, x):
     nbytes = L.lib.sed_group_norm_workspace(*shape, groups)
-    return nbytes, _workspace(nbytes, dev)
+    return nbytes, _workspace(nbytes, x)
 
 
 def _norm_forward(x, groups, weight, bias, eps, act, frames):
     n = x.numel()
     shape = (x.shape[0], x.shape[1], n // (x.shape[0] * x.shape[1] * x.shape[-1]) if n else 1, x.shape[-1])
     y = torch.empty_like(x)
-    stats = torch.empty(2 * shape[0] * groups, dtype=torch.float32, device=x.device)
+    stats = x.new_empty(2 * shape[0] * groups, dtype=torch.float32)
     if n:
-        ws = _norm_workspace(shape, groups, x.device)  # held until the kernels are launched
+        ws = _norm_workspace(shape, groups, x)  # held until the kernels are launched
         a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, stats, y, ws)
         _call(L.lib.sed_group_norm_forward, a, x.device, "sed_group_norm_forward")
     return y, stats, shape
@@ -404,14 +408,14 @@ class _GroupNormAct(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, frames, stats = ctx.saved_tensors
         shape, groups, eps, act = ctx.rest
-        dx, dw, db = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=x.device) for t in (x, weight, bias))
+        dx, dw, db = (_new(t) for t in (x, weight, bias))
         if x.numel() == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
             return dx, dw, db, None, None, None, None
         dy = dy.contiguous()
-        ws = _norm_workspace(shape, groups, x.device)
+        ws = _norm_workspace(shape, groups, x)
         a = _norm_args(x, shape, groups, weight, bias, act, eps, frames, stats, None, ws)
         a.dy, a.dx, a.dw, a.db = dy.data_ptr(), dx.data_ptr(), _ptr(dw), _ptr(db)
         _call(L.lib.sed_group_norm_backward, a, x.device, "sed_group_norm_backward")
