@@ -741,13 +741,13 @@ int whole_threads(const NormParams& p, int V, int held, bool back) {
   int threads = 1024;
   if (items >= 512)
     while (threads > 256 && nv <= threads / 2 && p.S <= held * (threads / 2 / nv)) threads /= 2;
-  return (int)std::min<int64_t>(threads, (p.S * nv + 63) / 64 * 64);
+  threads = (int)std::min<int64_t>(threads, (p.S * nv + 63) / 64 * 64);
+  return grid_fits(items + 7, threads) ? threads : 0;
 }
 
 template <class T, int V, int HELD, int ACT>
 int launch_whole(const NormParams& p, int threads, hipStream_t s) {
   const int64_t grid = (p.a.B * p.a.G + 7) / 8 * 8;
-  if (!grid_fits(grid, threads)) return SED_ERR_CAPACITY;
   norm_whole_kernel<T, V, HELD, ACT><<<(unsigned)grid, threads, 0, s>>>(p);
   return seq_status(hipGetLastError());
 }
@@ -765,7 +765,6 @@ int launch_param(const NormParams& p, hipStream_t s) {
 template <class T, int V, int ACT>
 int launch_whole_grad(const NormParams& p, int threads, hipStream_t s) {
   const int64_t grid = (p.a.B * p.a.G + 7) / 8 * 8;
-  if (!grid_fits(grid, threads)) return SED_ERR_CAPACITY;
   norm_whole_grad_kernel<T, V, 4, ACT><<<(unsigned)grid, threads, threads * (V + 1) * 4, s>>>(p);
   return launch_param(p, s);
 }
