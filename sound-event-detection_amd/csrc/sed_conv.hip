@@ -6,13 +6,14 @@
 // TL frames of one clip: which rows it meets and where they lie is the same for all its lanes (scalar work), a lane keeps the
 // window of WM rows, the weights and, in the gradient, the sums of its V channels in registers.  Rows come WM at a time, the
 // next WM on their way while WM are worked on.  A row is read once but for the WM - 1 in front of a run (and behind it, in the
-// gradient).  WM is W rounded up to 2, 4 or 8: the weights in front are zero.  V = 4 where rows allow it and there are channels
-// enough for a wave (2 of them at a time in the gradient of more than 4 taps), else 1.  The weight gradient is summed per lane over its run, written once per run and added over the runs
-// in a fixed order.  Sums are fp32 and every output is rounded once.
+// gradient).  WM is W, or 2 for 1 and 8 for 5 to 8.  V = 4 where rows allow it and there are channels enough for a wave (2 in the
+// gradient of more than 4 taps), else 1.  The weight gradient is summed per lane over its run, written once per run and added over
+// the runs in a fixed order.  Sums are fp32 and every output is rounded once.
 //
 // Measured (MI355X): 16 x 4096 x 1536 bf16, 4 taps with SiLU: forward 79 us for 403 MB (5.1 TB/s, what a 1 GiB copy reaches),
-// gradient 150 us for 604 MB (4.0 TB/s); runs of 16 / 32 / 64 frames forward: 84 / 79 / 80 us, of 32 / 64 / 128 in the gradient
-// with its weight sums: 164 / 162 / 167 us.  A thread per 8 channels with its own row addresses took 168 and 407 us.
+// gradient 142 us for 604 MB (4.3 TB/s; 150 with a condition at every load, 145 with registers for four waves a vector unit); runs
+// of 16 / 32 / 64 frames forward: 84 / 79 / 80 us, of 32 / 64 / 128 in the gradient with its weight sums: 164 / 162 / 167 us at the
+// time.  A thread per 8 channels with its own row addresses took 168 and 407 us.
 #include "seq_core.h"
 
 #include <algorithm>
@@ -60,6 +61,15 @@ __device__ __forceinline__ void load_weights(const sed_conv_args& a, int64_t d, 
   }
 }
 
+// acc + w x for tap m of WM, of which the first WM - W are none of the call's: what lies in front of its window, an infinity say, stays
+// out (its weight of zero would make a NaN of it).  An instance for 2 taps is called with 1 or 2, for 8 with 5 to 8.
+template <int WM>
+__device__ __forceinline__ float tap(const sed_conv_args& a, int m, float w, float x, float acc) {
+  constexpr int pads = WM == 2 ? 1 : WM == 8 ? 3 : 0;
+  const float sum = fmaf(w, x, acc);
+  return m < pads && m < WM - a.W ? acc : sum;
+}
+
 template <class T, int V>
 using Vec = T __attribute__((ext_vector_type(V)));
 
@@ -95,12 +105,14 @@ __device__ __forceinline__ Vec<T, V> row_at(const sed_conv_args& a, const Run& r
   if (!p) return Vec<T, V>{};
   return *reinterpret_cast<const Vec<T, V>*>(reinterpret_cast<const char*>(p) + (uint32_t)r.d * (uint32_t)sizeof(T));
 }
+// Row i >= 0 of the walk out of the rows `p` of a clip, the last own one in place of those behind it: loads without a condition, which
+// the caller's arithmetic leaves out.
 template <class T, int V>
-__device__ __forceinline__ Vec<T, V> dy_at(const sed_conv_args& a, const Run& r, int64_t i) {
-  if (i >= r.own) return Vec<T, V>{};
-  const T* p = static_cast<const T*>(a.dy) + r.b * a.dy_b + row_of(a, r.own, i) * a.dy_t;
-  return *reinterpret_cast<const Vec<T, V>*>(reinterpret_cast<const char*>(p) + (uint32_t)r.d * (uint32_t)sizeof(T));
+__device__ __forceinline__ Vec<T, V> row_in(const sed_conv_args& a, const Run& r, const void* p, int64_t step, int64_t i) {
+  const int64_t row = row_of(a, r.own, std::max<int64_t>(0, std::min(i, r.own - 1)));
+  return *reinterpret_cast<const Vec<T, V>*>(static_cast<const char*>(p) + row * step * (int64_t)sizeof(T) + (uint32_t)r.d * (uint32_t)sizeof(T));
 }
+
 template <class T, int V>
 __device__ __forceinline__ void put_row(const sed_conv_args& a, const Run& r, void* base, int64_t i, const float (&v)[V]) {
   T* p = static_cast<T*>(base) + (r.b * a.L + row_of(a, r.own, i)) * a.D;
@@ -111,10 +123,16 @@ template <class T, int V, int WM, int ACT>
 __global__ void __launch_bounds__(64) conv_forward_kernel(const ConvParams p) {
   const sed_conv_args& a = p.a;
   const Run r = run_of<V>(p);
+  const T* x = static_cast<const T*>(a.x) + r.b * a.x_b;
+  if (r.i0 >= r.own) {  // nothing of the clip's own: rows of zeros
+    const float zero[V] = {};
+    for (int64_t i = r.i0; i < r.i1; ++i) put_row<T, V>(a, r, a.y, i, zero);
+    return;
+  }
   float w[WM][V], bias[V], win[WM][V];
   Vec<T, V> next[WM];
 #pragma unroll
-  for (int k = 0; k < WM; ++k) next[k] = row_at<T, V>(a, r, r.i0 + k);
+  for (int k = 0; k < WM; ++k) next[k] = row_in<T, V>(a, r, x, a.x_t, r.i0 + k);
 #pragma unroll
   for (int k = 1; k < WM; ++k) {  // row i lies in win[(i - i0) % WM]
     const Vec<T, V> v = row_at<T, V>(a, r, r.i0 - WM + k);
@@ -128,7 +146,7 @@ __global__ void __launch_bounds__(64) conv_forward_kernel(const ConvParams p) {
     for (int k = 0; k < WM; ++k) in[k] = next[k];
     if (i + WM < r.i1) {
 #pragma unroll
-      for (int k = 0; k < WM; ++k) next[k] = row_at<T, V>(a, r, i + WM + k);
+      for (int k = 0; k < WM; ++k) next[k] = row_in<T, V>(a, r, x, a.x_t, i + WM + k);
     }
 #pragma unroll
     for (int k = 0; k < WM; ++k) {
@@ -138,7 +156,7 @@ __global__ void __launch_bounds__(64) conv_forward_kernel(const ConvParams p) {
         win[k][c] = (float)in[k][c];
         float u = bias[c];
 #pragma unroll
-        for (int m = 0; m < WM; ++m) u = fmaf(w[m][c], win[(k + 1 + m) % WM][c], u);
+        for (int m = 0; m < WM; ++m) u = tap<WM>(a, m, w[m][c], win[(k + 1 + m) % WM][c], u);
         y[c] = i + k < r.own ? act<ACT>(u) : 0.0f;
       }
       if (i + k < r.i1) put_row<T, V>(a, r, a.y, i + k, y);
@@ -154,10 +172,11 @@ __global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
   const Run r = run_of<V>(p);
   float w[WM][V], bias[V], win[WM][V], du[WM][V], dw[WM][V], db[V];
   Vec<T, V> nx[WM], ny[WM];
+  const T *x = static_cast<const T*>(a.x) + r.b * a.x_b, *g = static_cast<const T*>(a.dy) + r.b * a.dy_b;
 #pragma unroll
   for (int k = 0; k < WM; ++k) {
-    nx[k] = row_at<T, V>(a, r, r.i0 + k);
-    ny[k] = dy_at<T, V>(a, r, r.i0 + k);
+    nx[k] = row_in<T, V>(a, r, x, a.x_t, r.i0 + k);
+    ny[k] = row_in<T, V>(a, r, g, a.dy_t, r.i0 + k);
   }
 #pragma unroll
   for (int k = 1; k < WM; ++k) {
@@ -172,23 +191,27 @@ __global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
 #pragma unroll
     for (int k = 0; k < WM; ++k) dw[k][c] = du[k][c] = 0.0f;
   }
-  for (int64_t i = r.i0; i < r.i1 + WM - 1; i += WM) {
+  const float zero[V] = {};
+  const int64_t none = std::max(r.i0, r.own);  // rows behind the clip's own: zeros
+  for (int64_t i = none; i < r.i1; ++i) put_row<T, V>(a, r, a.dx, i, zero);
+  const int64_t last = std::min(r.i1, r.own);
+  for (int64_t i = r.i0; i < last + WM - 1 && r.i0 < last; i += WM) {
     Vec<T, V> in[WM], dy[WM];
 #pragma unroll
     for (int k = 0; k < WM; ++k) {
       in[k] = nx[k];
       dy[k] = ny[k];
     }
-    if (i + WM < r.i1 + WM - 1) {
+    if (i + WM < last + WM - 1) {
 #pragma unroll
       for (int k = 0; k < WM; ++k) {
-        nx[k] = row_at<T, V>(a, r, i + WM + k);
-        ny[k] = dy_at<T, V>(a, r, i + WM + k);
+        nx[k] = row_in<T, V>(a, r, x, a.x_t, i + WM + k);
+        ny[k] = row_in<T, V>(a, r, g, a.dy_t, i + WM + k);
       }
     }
 #pragma unroll
     for (int k = 0; k < WM; ++k) {
-      const bool counts = i + k < r.i1;  // rows behind the clip's own have dy = 0
+      const bool counts = i + k < last;
       const int64_t at = i + k - (WM - 1);
       float dx[V];
 #pragma unroll
@@ -196,7 +219,7 @@ __global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
         win[k][c] = (float)in[k][c];
         float u = bias[c];
 #pragma unroll
-        for (int m = 0; m < WM; ++m) u = fmaf(w[m][c], win[(k + 1 + m) % WM][c], u);
+        for (int m = 0; m < WM; ++m) u = tap<WM>(a, m, w[m][c], win[(k + 1 + m) % WM][c], u);
         du[k][c] = i + k < r.own ? (float)dy[k][c] * act_slope<ACT>(u) : 0.0f;
       }
       if (counts) {
@@ -207,17 +230,16 @@ __global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
           for (int m = 0; m < WM; ++m) dw[m][c] = fmaf(du[k][c], win[(k + 1 + m) % WM][c], dw[m][c]);
         }
       }
-      if (at >= r.i0 && at < r.i1) {
+      if (at >= r.i0 && at < last) {
         // row i + k - (WM - 1): du of that row and of the WM - 1 behind it
 #pragma unroll
         for (int c = 0; c < V; ++c) {
           dx[c] = 0.0f;
 #pragma unroll
-          for (int j = 0; j < WM; ++j) dx[c] = fmaf(w[WM - 1 - j][c], du[(k + 1 + j) % WM][c], dx[c]);
-          if (at >= r.own) dx[c] = 0.0f;
+          for (int j = 0; j < WM; ++j) dx[c] = tap<WM>(a, WM - 1 - j, w[WM - 1 - j][c], du[(k + 1 + j) % WM][c], dx[c]);
         }
         const int64_t late = at - (r.own - (a.W - 1));  // row of the state that the call returned
-        if (a.dstate_out && late >= 0 && at < r.own) {
+        if (a.dstate_out && late >= 0) {
           const T* e = static_cast<const T*>(a.dstate_out) + (r.b * (a.W - 1) + late) * a.D + r.d;
 #pragma unroll
           for (int c = 0; c < V; ++c) dx[c] += (float)e[c];
@@ -390,7 +412,8 @@ int go_kind(const ConvParams& p, Kind kind, hipStream_t s) {
 template <class T, int V>
 int go_w(const ConvParams& p, Kind kind, hipStream_t s) {
   if (p.a.W <= 2) return go_kind<T, V, 2>(p, kind, s);
-  if (p.a.W <= 4) return go_kind<T, V, 4>(p, kind, s);
+  if (p.a.W == 3) return go_kind<T, V, 3>(p, kind, s);
+  if (p.a.W == 4) return go_kind<T, V, 4>(p, kind, s);
   return go_kind<T, V, 8>(p, kind, s);
 }
 

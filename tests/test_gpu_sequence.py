@@ -411,6 +411,37 @@ def test_conv_own_lengths(reverse):
     _conv_case(2, 20, 16, 4, torch.float32, reverse=reverse, last=False)
 
 
+@pytest.mark.parametrize("W", range(1, 9))
+@pytest.mark.parametrize("d", (3, 256))
+def test_conv_infinities_reach_their_window_only(W, d):
+    import sed_amd
+    dev = _dev()
+    g = torch.Generator(device=dev).manual_seed(W)
+    x, dy = (torch.randn(2, 90, d, generator=g, device=dev) for _ in range(2))
+    w = torch.randn(d, W, generator=g, device=dev)
+    got = []
+    for bad in (False, True):
+        v, e = x.clone(), dy.clone()
+        if bad:
+            v[0, 40], e[1, 30] = float("inf"), float("nan")
+        v.requires_grad_(True)
+        y = sed_amd.causal_conv(v, w, activation=None)
+        got.append([y, *torch.autograd.grad(y, [v], e)])
+    clean, dirty = got
+    away = torch.ones(90, dtype=torch.bool, device=dev)
+    away[40:40 + W] = False
+    assert torch.equal(clean[0][0][away], dirty[0][0][away]) and torch.equal(clean[0][1], dirty[0][1])
+    assert not dirty[0][0][~away].isfinite().any()
+    away = torch.ones(90, dtype=torch.bool, device=dev)
+    away[30 - W + 1:31] = False
+    assert torch.equal(clean[1][0], dirty[1][0]) and torch.equal(clean[1][1][away], dirty[1][1][away])
+    st = torch.randn(3, W - 1, d, generator=g, device=dev)
+    rows = torch.randn(12, 3, d, generator=g, device=dev)
+    rows[0, 1] = float("inf")
+    ys = [sed_amd.causal_conv_step(st, t, w) for t in rows]
+    assert all(t.isfinite().all() for t in ys[W:]) and st.isfinite().all()
+
+
 def test_conv_rows_behind_are_neither_read_nor_kept():
     import sed_amd
     dev = _dev()
