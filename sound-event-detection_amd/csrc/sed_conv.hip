@@ -105,11 +105,11 @@ __device__ __forceinline__ Vec<T, V> row_at(const sed_conv_args& a, const Run& r
   if (!p) return Vec<T, V>{};
   return *reinterpret_cast<const Vec<T, V>*>(reinterpret_cast<const char*>(p) + (uint32_t)r.d * (uint32_t)sizeof(T));
 }
-// Row i >= 0 of the walk out of the rows `p` of a clip, the last own one in place of those behind it: loads without a condition, which
-// the caller's arithmetic leaves out.
+// Row i >= 0 of the walk out of the rows `p` of a clip that has some, the last own one in place of those behind it: a load without a
+// condition, whose value the caller leaves out there.
 template <class T, int V>
 __device__ __forceinline__ Vec<T, V> row_in(const sed_conv_args& a, const Run& r, const void* p, int64_t step, int64_t i) {
-  const int64_t row = row_of(a, r.own, std::max<int64_t>(0, std::min(i, r.own - 1)));
+  const int64_t row = row_of(a, r.own, std::min(i, r.own - 1));
   return *reinterpret_cast<const Vec<T, V>*>(static_cast<const char*>(p) + row * step * (int64_t)sizeof(T) + (uint32_t)r.d * (uint32_t)sizeof(T));
 }
 
@@ -173,10 +173,13 @@ __global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
   float w[WM][V], bias[V], win[WM][V], du[WM][V], dw[WM][V], db[V];
   Vec<T, V> nx[WM], ny[WM];
   const T *x = static_cast<const T*>(a.x) + r.b * a.x_b, *g = static_cast<const T*>(a.dy) + r.b * a.dy_b;
+  const int64_t last = std::min(r.i1, r.own);  // the run's own rows end here
+  if (r.i0 < last) {
 #pragma unroll
-  for (int k = 0; k < WM; ++k) {
-    nx[k] = row_in<T, V>(a, r, x, a.x_t, r.i0 + k);
-    ny[k] = row_in<T, V>(a, r, g, a.dy_t, r.i0 + k);
+    for (int k = 0; k < WM; ++k) {
+      nx[k] = row_in<T, V>(a, r, x, a.x_t, r.i0 + k);
+      ny[k] = row_in<T, V>(a, r, g, a.dy_t, r.i0 + k);
+    }
   }
 #pragma unroll
   for (int k = 1; k < WM; ++k) {
@@ -192,9 +195,7 @@ __global__ void __launch_bounds__(64) conv_backward_kernel(const ConvParams p) {
     for (int k = 0; k < WM; ++k) dw[k][c] = du[k][c] = 0.0f;
   }
   const float zero[V] = {};
-  const int64_t none = std::max(r.i0, r.own);  // rows behind the clip's own: zeros
-  for (int64_t i = none; i < r.i1; ++i) put_row<T, V>(a, r, a.dx, i, zero);
-  const int64_t last = std::min(r.i1, r.own);
+  for (int64_t i = std::max(r.i0, r.own); i < r.i1; ++i) put_row<T, V>(a, r, a.dx, i, zero);
   for (int64_t i = r.i0; i < last + WM - 1 && r.i0 < last; i += WM) {
     Vec<T, V> in[WM], dy[WM];
 #pragma unroll
