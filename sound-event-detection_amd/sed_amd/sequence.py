@@ -94,6 +94,11 @@ def _no_grad_only(what, *tensors):
         raise RuntimeError(f"{what} updates the state in place and keeps nothing for a gradient: call it under torch.no_grad()")
 
 
+def _moved_on(state):
+    """state was written in place: a gradient that kept it as an input notices (tensors of inference mode have no such count)."""
+    torch._C._increment_version((state,))
+
+
 def _wants_grad(*tensors):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -137,19 +142,21 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, Cm, D, z, dt_bias, state, softplus, frames, reverse, want_last):
         y, last, saved = _scan_forward(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state, want_last, True)
-        ctx.save_for_backward(x, dt, A, B, Cm, D, z, dt_bias, state, frames, saved)
-        ctx.flags = (softplus, reverse)
+        ctx.save_for_backward(x, dt, A, B, Cm, D, z, dt_bias, frames, saved)
+        # the state in front is part of `saved`: it may move on before the gradient is taken
+        ctx.rest = (softplus, reverse, None if state is None else state.shape)
         ctx.set_materialize_grads(False)
         return (y, last) if want_last else y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast=None):
-        x, dt, A, B, Cm, D, z, dt_bias, state, frames, saved = ctx.saved_tensors
-        softplus, reverse = ctx.flags
+        x, dt, A, B, Cm, D, z, dt_bias, frames, saved = ctx.saved_tensors
+        softplus, reverse, state_shape = ctx.rest
         b, n_frames, d = x.shape
         dev = x.device
-        dx, ddt, dA, dB, dC, dD, dz, dbias, dstate = (_new(t) for t in (x, dt, A, B, Cm, D, z, dt_bias, state))
+        dx, ddt, dA, dB, dC, dD, dz, dbias = (_new(t) for t in (x, dt, A, B, Cm, D, z, dt_bias))
+        dstate = None if state_shape is None else x.new_empty(state_shape, dtype=torch.float32)
         if b == 0 or n_frames == 0:
             for t in (dA, dD, dbias, dstate):
                 if t is not None:
@@ -159,7 +166,7 @@ class _GatedScan(torch.autograd.Function):
             return dx, ddt, dA, dB, dC, dD, dz, dbias, dstate, None, None, None, None
         dy = torch.zeros((b, n_frames, d), dtype=x.dtype, device=dev) if dy is None else _rows(dy)
         dlast = None if dlast is None else dlast.contiguous()
-        a = _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, state)
+        a = _scan_args(x, dt, A, B, Cm, D, z, dt_bias, softplus, frames, reverse, None)
         a.saved = saved.data_ptr()
         a.dy, a.dy_b, a.dy_t, a.dh_last = dy.data_ptr(), dy.stride(0), dy.stride(1), _ptr(dlast)
         a.dx, a.ddt, a.dz, a.dB, a.dC = dx.data_ptr(), ddt.data_ptr(), _ptr(dz), dB.data_ptr(), dC.data_ptr()
@@ -250,6 +257,7 @@ def gated_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplu
                    C.data_ptr(), x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, bs[0], 0, bs[1] if wide else 0, cs[0], 0,
                    cs[1] if wide else 0, A.data_ptr(), _ptr(D), _ptr(dt_bias), None, state.data_ptr(), y.data_ptr())
     _call(L.lib.sed_gated_scan_step, a, x.device, "sed_gated_scan_step")
+    _moved_on(state)
     return y
 
 
@@ -365,6 +373,7 @@ def causal_conv_step(state, x, weight, bias=None, activation=None):
     a = L.ConvArgs(x.shape[0], 1, x.shape[1], weight.shape[1], _DTYPES[x.dtype], _ACTIVATIONS[activation], 0, None, x.data_ptr(), x.stride(0), 0,
                    weight.data_ptr(), _ptr(bias), None, y.data_ptr(), _ptr(state))
     _call(L.lib.sed_causal_conv_step, a, x.device, "sed_causal_conv_step")
+    _moved_on(state)
     return y
 
 

@@ -1,0 +1,65 @@
+"""GPU tests of what the sequence operators promise beside their values on ordinary data: derivatives that would be wrong are refused,
+limits and strides are those the documentation names, extreme parameters and recordings keep their digits."""
+import pytest
+import torch
+
+from test_gpu_sequence import _dev
+
+pytestmark = pytest.mark.gpu
+
+
+def _step_inputs(nb=2, d=16, ns=4, W=4):
+    g = torch.Generator(device=_dev()).manual_seed(1)
+    r = lambda *s: torch.randn(s, generator=g, device=_dev())  # noqa: E731
+    return {"x": r(nb, 9, d), "A": -torch.rand(d, ns, generator=g, device=_dev()), "bc": r(nb, 9, ns), "w": r(d, W), "conv": r(nb, W - 1, d), "scan": r(nb, d, ns)}
+
+
+def test_a_step_on_a_saved_state_is_noticed():
+    """causal_conv's gradient reads the state it was given: a step that moves it on in between is an error, as for torch's own operators."""
+    import sed_amd
+    v = _step_inputs()
+    w = v["w"].clone().requires_grad_(True)
+    for activation in (None, "silu"):
+        state = v["conv"].clone()
+        y = sed_amd.causal_conv(v["x"], w, activation=activation, state=state)
+        with torch.no_grad():
+            sed_amd.causal_conv_step(state, v["x"][:, 0], w, activation=activation)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            torch.autograd.grad(y.sum(), w)
+    # any other operator that keeps the state is told as well
+    for start, step in ((v["conv"], lambda s: sed_amd.causal_conv_step(s, v["x"][:, 0], v["w"])),
+                        (v["scan"], lambda s: sed_amd.gated_scan_step(s, v["x"][:, 0], v["x"][:, 0], v["A"], v["bc"][:, 0], v["bc"][:, 0]))):
+        state, scale = start.clone(), torch.ones((), device=_dev(), requires_grad=True)
+        y = (scale * state).sum()
+        with torch.no_grad():
+            step(state)
+        with pytest.raises(RuntimeError, match="inplace operation"):
+            torch.autograd.grad(y, scale)
+
+
+def test_a_step_behind_gated_scan_leaves_its_gradient():
+    """gated_scan's gradient does not read the state in front: the stream may go on before it is taken."""
+    import sed_amd
+    v = _step_inputs()
+    got = []
+    for go_on in (False, True):
+        x, state = v["x"].clone().requires_grad_(True), v["scan"].clone()
+        y = sed_amd.gated_scan(x, v["x"], v["A"], v["bc"], v["bc"], softplus=True, state=state)
+        if go_on:
+            with torch.no_grad():
+                sed_amd.gated_scan_step(state, v["x"][:, 0], v["x"][:, 0], v["A"], v["bc"][:, 0], v["bc"][:, 0], softplus=True)
+        got.append(torch.autograd.grad(y.sum(), x)[0])
+    assert torch.equal(*got)
+
+
+def test_steps_in_inference_mode():
+    import sed_amd
+    v = _step_inputs()
+    want = [v["conv"].clone(), v["scan"].clone()]
+    step = lambda s: [sed_amd.causal_conv_step(s[0], v["x"][:, 0], v["w"]),  # noqa: E731
+                      sed_amd.gated_scan_step(s[1], v["x"][:, 0], v["x"][:, 0], v["A"], v["bc"][:, 0], v["bc"][:, 0], softplus=True)]
+    ys = step(want)
+    with torch.inference_mode():
+        states = [v["conv"].clone(), v["scan"].clone()]
+        got = step(states)
+    assert all(torch.equal(a, b) for a, b in zip(ys + want, got + states))
