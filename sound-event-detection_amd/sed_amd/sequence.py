@@ -6,11 +6,13 @@ matrix products, with gradients, and in the form a stream calls frame by frame.
 convolution in front of it, `group_norm_act` a group norm with an activation on channels-last feature maps (B, T, F, C) or
 sequences (B, T, C).  All take `frames`, the clips' own row counts, as reshape_wav2img does: rows behind a clip's own are never
 read, and are zero in every output and gradient.  Arithmetic, states and sums are fp32 whatever the element type (fp32, bf16,
-fp16); every output is rounded once.  There is no CPU path.
+fp16); every output is rounded once.  Derivatives are first ones in reverse mode: a tensor with a forward-mode tangent is refused.  There
+is no CPU path.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -89,7 +91,15 @@ def _call(fn, args, dev, what):
             L.check(fn(args, stream), what)
 
 
+def _no_tangent(what, *tensors):
+    """A dual tensor of forward-mode differentiation need not require grad; its tangent would get lost without a word."""
+    if forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled() and any(
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative")
+
+
 def _no_grad_only(what, *tensors):
+    _no_tangent(what, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} updates the state in place and keeps nothing for a gradient: call it under torch.no_grad()")
 
@@ -99,7 +109,8 @@ def _moved_on(state):
     torch._C._increment_version((state,))
 
 
-def _wants_grad(*tensors):
+def _wants_grad(what, *tensors):
+    _no_tangent(what, *tensors)
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
@@ -151,6 +162,7 @@ class _GatedScan(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast=None):
+        _no_tangent("the gradient of gated_scan", dy, dlast)
         x, dt, A, B, Cm, D, z, dt_bias, frames, saved = ctx.saved_tensors
         softplus, reverse, state_shape = ctx.rest
         b, n_frames, d = x.shape
@@ -229,7 +241,7 @@ def gated_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, fra
         B, C = B.unsqueeze(2), C.unsqueeze(2)
     x, dt, z, B, C = (_rows(t) for t in (x, dt, z, B, C))
     A, D, dt_bias = _param(A), _param(D), _param(dt_bias)
-    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, state):
+    if _wants_grad(what, x, dt, A, B, C, D, z, dt_bias, state):
         return _GatedScan.apply(x, dt, A, B, C, D, z, dt_bias, state, bool(softplus), frames, bool(reverse), bool(return_state))
     y, last, _ = _scan_forward(x, dt, A, B, C, D, z, dt_bias, softplus, frames, reverse, state, return_state, False)
     return (y, last) if return_state else y
@@ -297,6 +309,7 @@ class _CausalConv(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dlast=None):
+        _no_tangent("the gradient of causal_conv", dy, dlast)
         x, weight, bias, state, frames = ctx.saved_tensors
         act, reverse = ctx.flags
         b, n_frames, d = x.shape
@@ -350,7 +363,7 @@ def causal_conv(x, weight, bias=None, activation=None, frames=None, reverse=Fals
         _check(what, "state", state, x, (x.shape[0], weight.shape[1] - 1, x.shape[2]))
         state = state.contiguous()
     x, weight, bias, act = _rows(x), _param(weight), _param(bias), _ACTIVATIONS[activation]
-    if _wants_grad(x, weight, bias, state):
+    if _wants_grad(what, x, weight, bias, state):
         return _CausalConv.apply(x, weight, bias, state, act, frames, bool(reverse), bool(return_state))
     y, last = _conv_forward(x, weight, bias, act, frames, reverse, state, return_state)
     return (y, last) if return_state else y
@@ -415,6 +428,7 @@ class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
+        _no_tangent("the gradient of group_norm_act", dy)
         x, weight, bias, frames, stats = ctx.saved_tensors
         shape, groups, eps, act = ctx.rest
         dx, dw, db = (_new(t) for t in (x, weight, bias))
@@ -456,6 +470,6 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation=None,
             _check(what, name, t, x, (c,), "float")
     _check_frames(what, frames, x)
     x, weight, bias, act = x.contiguous(), _param(weight), _param(bias), _ACTIVATIONS[activation]
-    if _wants_grad(x, weight, bias):
+    if _wants_grad(what, x, weight, bias):
         return _GroupNormAct.apply(x, weight, bias, groups, float(eps), act, frames)
     return _norm_forward(x, groups, weight, bias, float(eps), act, frames)[0]

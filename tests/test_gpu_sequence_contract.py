@@ -2,6 +2,7 @@
 limits and strides are those the documentation names, extreme parameters and recordings keep their digits."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from test_gpu_sequence import _dev
 
@@ -63,3 +64,49 @@ def test_steps_in_inference_mode():
         states = [v["conv"].clone(), v["scan"].clone()]
         got = step(states)
     assert all(torch.equal(a, b) for a, b in zip(ys + want, got + states))
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor does not require grad; its tangent must not get lost without a word."""
+    import sed_amd
+    v = _step_inputs()
+    calls = {
+        "gated_scan": (sed_amd.gated_scan, dict(x=v["x"], dt=v["x"], A=v["A"], B=v["bc"], C=v["bc"], D=v["w"][:, 0], z=v["x"], dt_bias=v["w"][:, 1], state=v["scan"])),
+        "gated_scan_step": (sed_amd.gated_scan_step, dict(state=v["scan"], x=v["x"][:, 0], dt=v["x"][:, 0], A=v["A"], B=v["bc"][:, 0], C=v["bc"][:, 0],
+                                                          D=v["w"][:, 0], z=v["x"][:, 0], dt_bias=v["w"][:, 1])),
+        "causal_conv": (sed_amd.causal_conv, dict(x=v["x"], weight=v["w"], bias=v["w"][:, 0], state=v["conv"])),
+        "causal_conv_step": (sed_amd.causal_conv_step, dict(state=v["conv"], x=v["x"][:, 0], weight=v["w"], bias=v["w"][:, 0])),
+        "group_norm_act": (sed_amd.group_norm_act, dict(x=v["x"], weight=v["w"][:, 0], bias=v["w"][:, 1], groups=4)),
+    }
+    for name, (call, kw) in calls.items():
+        for k in (k for k, t in kw.items() if torch.is_tensor(t)):
+            for grad in (False, True):
+                if grad and "step" in name:
+                    continue
+                before = kw[k].clone()
+                with forward_ad.dual_level():
+                    dual = forward_ad.make_dual(kw[k].clone().requires_grad_(grad), torch.ones_like(kw[k]))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(**(kw | {k: dual}))
+                    with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                        call(**(kw | {k: dual}))
+                    assert torch.equal(forward_ad.unpack_dual(dual).primal, before), (name, k)
+        with forward_ad.dual_level():  # without a tangent the call is an ordinary one
+            call(**{k: t.clone() if torch.is_tensor(t) else t for k, t in kw.items()})
+
+
+def test_forward_over_reverse_is_refused():
+    import sed_amd
+    v = _step_inputs()
+    for call in (lambda x: sed_amd.gated_scan(x, v["x"], v["A"], v["bc"], v["bc"], softplus=True), lambda x: sed_amd.causal_conv(x, v["w"]),
+                 lambda x: sed_amd.group_norm_act(x, 4)):
+        x = v["x"].clone().requires_grad_(True)
+        y = call(x)
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(y, x, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    for state, call in ((v["scan"], lambda s: sed_amd.gated_scan(v["x"], v["x"], v["A"], v["bc"], v["bc"], softplus=True, state=s, return_state=True)),
+                        (v["conv"], lambda s: sed_amd.causal_conv(v["x"], v["w"], state=s, return_state=True))):
+        state = state.clone().requires_grad_(True)
+        last = call(state)[1]
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(last, state, forward_ad.make_dual(torch.ones_like(last), torch.ones_like(last)))
