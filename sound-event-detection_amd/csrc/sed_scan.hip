@@ -325,6 +325,20 @@ __device__ __forceinline__ void load_dn(const ScanParams& p, const float* base, 
       h[c][n] = k < N ? v : 0.0f;
     }
 }
+// A in units of exp2.  Its lowest values stay finite, so that a step of zero (a lane without a channel, a frame behind the clip's own, a
+// chunk without frames) keeps its state: 0 times infinity would be a NaN.
+__device__ __forceinline__ float exponent(float A) {
+  const float v = A * kLog2e;
+  return v < -3.4028235e38f ? -3.4028235e38f : v;
+}
+template <int NS>
+__device__ __forceinline__ void load_exponents(const ScanParams& p, const Where& w, float (&A2)[4][NS]) {
+  load_dn<NS>(p, p.a.A, w, A2);
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int n = 0; n < NS; ++n) A2[c][n] = exponent(A2[c][n]);
+}
 template <int NS>
 __device__ __forceinline__ void store_dn(float* base, int N, const Where& w, const float (&h)[4][NS]) {
 #pragma unroll
@@ -453,11 +467,7 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(S
   fetch(w.begin);
 
   float A2[4][NS], h[4][NS], bias[4], skip[4], sum[4] = {0, 0, 0, 0};
-  load_dn<NS>(p, a.A, w, A2);
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int n = 0; n < NS; ++n) A2[c][n] *= kLog2e;
+  load_exponents<NS>(p, w, A2);
   per_channel(a.dt_bias, w, bias);
   per_channel(a.skip, w, skip);
   if (!ENDS && p.K > kOwnJoin) {
@@ -567,7 +577,7 @@ __global__ void __launch_bounds__(1024) chunk_join_kernel(const ScanParams p) {
   if (a.frames) own = std::max(0, std::min((int)a.L, a.frames[b]));
   const int k_own = own > 0 ? p.K : 0;
   const bool real = n < a.N;
-  const float A2 = real ? a.A[d * a.N + n] * kLog2e : 0.0f;
+  const float A2 = real ? exponent(a.A[d * a.N + n]) : 0.0f;
   const float* first = BACK ? a.dh_last : a.h0;
   float* hp = p.chunk_h + (b * p.K * NP + n) * a.D + d;
   const float* sp = p.chunk_s + b * p.K * a.D + d;
@@ -698,14 +708,11 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
   if (tiles) fetch(w.begin + (tiles - 1) * G::TT);
 
   float A2[4][NS], g[4][NS], dA[4][NS], sum[4] = {0, 0, 0, 0}, dskip[4] = {0, 0, 0, 0}, dbias[4] = {0, 0, 0, 0};
-  load_dn<NS>(p, a.A, w, A2);
+  load_exponents<NS>(p, w, A2);
 #pragma unroll
   for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int n = 0; n < NS; ++n) {
-      A2[c][n] *= kLog2e;
-      dA[c][n] = g[c][n] = 0.0f;
-    }
+    for (int n = 0; n < NS; ++n) dA[c][n] = g[c][n] = 0.0f;
   {
     float v[4];
     per_channel(a.dt_bias, w, v);

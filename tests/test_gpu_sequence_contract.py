@@ -1,10 +1,11 @@
 """GPU tests of what the sequence operators promise beside their values on ordinary data: derivatives that would be wrong are refused,
 limits and strides are those the documentation names, extreme parameters and recordings keep their digits."""
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
 
-from test_gpu_sequence import _dev
+from test_gpu_sequence import _dev, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -110,3 +111,27 @@ def test_forward_over_reverse_is_refused():
         last = call(state)[1]
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(last, state, forward_ad.make_dual(torch.ones_like(last), torch.ones_like(last)))
+
+
+@pytest.mark.parametrize("ns", (1, 3, 8, 16, 32))
+@pytest.mark.parametrize("nb,n,d,g,frames", ((2, 21, 5, 1, (21, 10)), (3, 70, 6, 3, None), (2, 900, 12, 1, (3, 900)), (1, 5000, 4, 1, None)))
+def test_scan_forgets_at_once_with_the_lowest_decay(nb, n, d, g, frames, ns):
+    """A of the type's lowest value: every frame starts from zero.  exp(delta A) is exactly zero for A = -10^6 as well (delta >= 0.01), so
+    both give the same bits, in lanes without a channel, in frames behind a clip's own that share its tile, and over chunks without frames."""
+    import sed_amd
+    dev, _, rng = _scan_inputs(nb, n, d, g, ns, torch.float32, ns, softplus=False, frames=frames, state=True)
+    dev["dt"] = dev["dt"].clamp(min=0.01)
+    dy = torch.from_numpy(rng.standard_normal((nb, n, d)).astype(np.float32)).to(_dev())
+    dl = torch.from_numpy(rng.standard_normal((nb, d, ns)).astype(np.float32)).to(_dev())
+    for reverse in (False, True):
+        got = []
+        for low in (-1e6, torch.finfo(torch.float32).min):
+            A = dev["A"].clone()
+            A[1::2] = low
+            A[:, -1] = low
+            leaves = {k: t.detach().clone().requires_grad_(True) for k, t in (dev | {"A": A}).items() if k != "frames"}
+            args = dict(leaves)
+            y, last = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, frames=dev.get("frames"), reverse=reverse, return_state=True)
+            got.append([y, last, *torch.autograd.grad([y, last], list(leaves.values()), [dy, dl])])
+        for name, a, b in zip(["y", "last"] + list(leaves), *got):
+            assert a.isfinite().all() and torch.equal(a, b), (name, reverse)
