@@ -378,6 +378,14 @@ __device__ __forceinline__ void only_own(const Where& w, int i0, int r, float (&
   for (int c = 0; c < 4; ++c) v[c] = in && (VEC ? w.nc > 0 : c < w.nc) ? v[c] : 0.0f;
 }
 
+// 2^z h + e over a chunk, z the sum of its frames' exponents.  The frames one by one would carry a state of zero, or a small one, through
+// growth that is beyond fp32 as a whole (A delta > 0), so there 2^z goes on in two halves, the second to the scaled state.
+__device__ __forceinline__ float over_chunk(float z, float h, float e) {
+  const bool far = z > 126.0f;
+  const float f = exp2_hw(far ? std::min(0.5f * z, 127.0f) : z);
+  return fmaf(f, far ? f * h : h, e);
+}
+
 // The state behind `count` chunks from the state h in front of them (their end states from zero and sums of delta): chunks
 // q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.
 template <class G, int NS, bool VEC>
@@ -401,10 +409,19 @@ __device__ __forceinline__ void pass_chunks(const ScanParams& p, const Where& w,
       for (int n = 0; n < NS; ++n) e1[c][n] = e[c][n];
     }
     if (i + 1 < count) load(i + 1);
+    float most = 0.0f;  // the usual decay takes no more than finding that it is one
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int n = 0; n < NS; ++n) h[c][n] = fmaf(exp2_hw(A2[c][n] * s1[c]), h[c][n], e1[c][n]);
+      for (int n = 0; n < NS; ++n) most = fmaxf(most, A2[c][n] * s1[c]);
+    const bool far = __any(most > 126.0f);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < NS; ++n) {
+        const float z = A2[c][n] * s1[c];
+        h[c][n] = far ? over_chunk(z, h[c][n], e1[c][n]) : fmaf(exp2_hw(z), h[c][n], e1[c][n]);
+      }
   }
 }
 
@@ -589,7 +606,7 @@ __global__ void __launch_bounds__(1024) chunk_join_kernel(const ScanParams p) {
 #pragma unroll 4
     for (int q = q0; q < std::min(q1, k_own - 1); ++q) {
       const float sk = sp[at(q) * a.D];
-      h = fmaf(exp2_hw(A2 * sk), h, hp[at(q) * NP * a.D]);
+      h = over_chunk(A2 * sk, h, hp[at(q) * NP * a.D]);
       s += sk;
     }
     s_h[seg][lane] = h;
@@ -597,13 +614,13 @@ __global__ void __launch_bounds__(1024) chunk_join_kernel(const ScanParams p) {
     __syncthreads();
   }
   float h = first && real && live ? first[(b * a.D + d) * a.N + n] : 0.0f;
-  for (int k = 0; k < seg; ++k) h = fmaf(exp2_hw(A2 * s_s[k][lane]), h, s_h[k][lane]);
+  for (int k = 0; k < seg; ++k) h = over_chunk(A2 * s_s[k][lane], h, s_h[k][lane]);
 #pragma unroll 4
   for (int q = q0; q < q1; ++q) {
     const bool more = q < k_own - 1;
     const float end = more ? hp[at(q) * NP * a.D] : 0.0f, sk = more ? sp[at(q) * a.D] : 0.0f;
     hp[at(q) * NP * a.D] = h;
-    h = fmaf(exp2_hw(A2 * sk), h, end);
+    h = over_chunk(A2 * sk, h, end);
   }
 }
 

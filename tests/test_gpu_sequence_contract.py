@@ -5,7 +5,8 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from test_gpu_sequence import _dev, _scan_inputs
+from oracle import sequence as S
+from test_gpu_sequence import NAMES, U, _close, _dev, _rounded, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +136,61 @@ def test_scan_forgets_at_once_with_the_lowest_decay(nb, n, d, g, frames, ns):
             got.append([y, last, *torch.autograd.grad([y, last], list(leaves.values()), [dy, dl])])
         for name, a, b in zip(["y", "last"] + list(leaves), *got):
             assert a.isfinite().all() and torch.equal(a, b), (name, reverse)
+
+
+@pytest.mark.parametrize("ns", (1, 4, 8, 16, 32))
+@pytest.mark.parametrize("n,d", ((900, 8), (900, 7), (9000, 4)))
+def test_scan_growth_over_a_chunk_meets_a_zero_state(n, d, ns):
+    """exp(delta A) > 1 in every frame, x only in the last one and dy only in the first: nothing is there that could grow, so every
+    output is finite although the product of the growths is not."""
+    import sed_amd
+    dev, ref, rng = _scan_inputs(2, n, d, 1, ns, torch.float32, n + ns, softplus=False, bias=False)
+    dy = np.zeros((2, n, d))
+    dy[:, 0] = rng.standard_normal((2, d))
+    ref["x"][:, :-1] = 0
+    ref["A"] = np.full((d, ns), 8.0)
+    ref["dt"] = np.full((2, n, d), 1.0)  # e^8 a frame: 16 frames pass the range of fp32
+    dev = {k: torch.from_numpy(a.astype(np.float32)).to(_dev()).requires_grad_(True) for k, a in ref.items()}
+    dy, rdy = _rounded(dy, torch.float32)
+    args = dict(dev)
+    y, last = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, return_state=True)
+    grads = dict(zip(dev, torch.autograd.grad(y, list(dev.values()), dy)))
+    # By the definition: only the last frame has a state, delta B x, and only the first one a gradient behind it, C gy.
+    x, B, C, D, z = (ref[k] for k in ("x", "B", "C", "D", "z"))
+    gate = z * S.sigmoid(z)
+    h = x[:, -1, :, None] * B[:, -1, 0][:, None]
+    want = {k: np.zeros_like(ref[k]) for k in ref}
+    wy = np.zeros((2, n, d))
+    pre = (h * C[:, -1, 0][:, None]).sum(-1) + D * x[:, -1]
+    wy[:, -1] = pre * gate[:, -1]
+    gy = (rdy * gate)[:, 0]
+    want["x"][:, 0] = D * gy + (gy[..., None] * C[:, 0, 0][:, None] * B[:, 0, 0][:, None]).sum(-1)
+    size = {k: np.zeros_like(ref[k]) for k in ref}
+    size["x"][:, 0] = np.abs(D * gy) + np.abs(gy[..., None] * C[:, 0, 0][:, None] * B[:, 0, 0][:, None]).sum(-1)
+    sy = np.zeros((2, n, d))
+    sy[:, -1] = ((np.abs(h * C[:, -1, 0][:, None])).sum(-1) + np.abs(D * x[:, -1])) * np.abs(gate[:, -1])
+    # sums of at most 34 terms, the gate's 100 u as in every case
+    _close(y, wy, 200 * U * sy, "y")
+    _close(last, h, 8 * U * np.abs(h), "last")
+    for k in ref:  # h is zero where g is not and the other way round, but for the products above
+        _close(grads[k], want[k], 200 * U * size[k], NAMES[k])
+
+
+def test_scan_growth_over_a_chunk_meets_a_small_state():
+    """A state of 1e-36 that grows by e^160 within 16 frames ends at 3e33: the growth alone, e^160, is beyond fp32."""
+    import sed_amd
+    nb, n, d, ns = 48, 96, 4, 4
+    dev = _dev()
+    dt = torch.zeros(nb, n, d, device=dev)
+    for b in range(nb):  # wherever the chunks' borders are, some clips have the growth inside one
+        dt[b, b:b + 16] = 10.0
+    x, bc = torch.zeros(nb, n, d, device=dev), torch.ones(nb, n, ns, device=dev)
+    state = torch.full((nb, d, ns), 1e-36, device=dev, requires_grad=True)
+    few = lambda t: t.repeat(1, 40, 1)[:, :n * 40]  # noqa: E731
+    for dt_, x_, bc_ in ((dt, x, bc), (torch.cat([dt, few(torch.zeros_like(dt))], 1), torch.cat([x, few(x)], 1), torch.cat([bc, few(bc)], 1))):
+        y, last = sed_amd.gated_scan(x_, dt_, torch.ones(d, ns, device=dev), bc_, bc_, state=state, return_state=True)
+        want = np.full((nb, d, ns), state.detach().flatten()[0].item() * np.exp(160.0))
+        # 16 exponents of 10 (or one of 160), each off by 8 u of itself, and the decays' own rounding
+        _close(last, want, U * (8 * 160 + 8 * 32) * want, "last")
+        (g,) = torch.autograd.grad(last, state, torch.full_like(last, 1e-36))
+        _close(g, want, U * (8 * 160 + 8 * 32) * want, "dstate")
