@@ -234,6 +234,16 @@ __device__ __forceinline__ void put4(const float (&v)[4], float* to) {
   *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
+// The states are there from here on: where a branch left their loads under way, the first tile's frames would wait for them, and with them
+// for the next tile's rows, in every tile (64 clips of up to 1024 x 768 x 16: 177 us, 161 so).
+template <int NS>
+__device__ __forceinline__ void arrived(float (&h)[4][NS]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+#pragma unroll
+    for (int n = 0; n < NS; ++n) asm volatile("" : "+v"(h[c][n]));
+}
+
 // What a frame of a tile needs out of LDS; row, state: the lane's places in the tile's first frame.
 template <int NS>
 struct Step {
@@ -387,10 +397,12 @@ __device__ __forceinline__ float over_chunk(float z, float h, float e) {
 }
 
 // The state behind `count` chunks from the state h in front of them (their end states from zero and sums of delta): chunks
-// q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.
-template <class G, int NS, bool VEC>
-__device__ __forceinline__ void pass_chunks(const ScanParams& p, const Where& w, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
-  if (count <= 0) return;
+// q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.  Returns the largest exponent met:
+// without FAR, for which decays are the usual thing, h is right if it is no larger than 126.
+template <class G, int NS, bool VEC, bool FAR>
+__device__ __forceinline__ float pass_chunks(const ScanParams& p, const Where& w, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
+  float most = 0.0f;
+  if (count <= 0) return most;
   const int64_t D = p.a.D;
   float e[4][NS], s[4];
   const auto load = [&](int i) {
@@ -409,19 +421,31 @@ __device__ __forceinline__ void pass_chunks(const ScanParams& p, const Where& w,
       for (int n = 0; n < NS; ++n) e1[c][n] = e[c][n];
     }
     if (i + 1 < count) load(i + 1);
-    float most = 0.0f;  // the usual decay takes no more than finding that it is one
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int n = 0; n < NS; ++n) most = fmaxf(most, A2[c][n] * s1[c]);
-    const bool far = __any(most > 126.0f);
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
       for (int n = 0; n < NS; ++n) {
         const float z = A2[c][n] * s1[c];
-        h[c][n] = far ? over_chunk(z, h[c][n], e1[c][n]) : fmaf(exp2_hw(z), h[c][n], e1[c][n]);
+        if (!FAR) most = fmaxf(most, z);
+        h[c][n] = FAR ? over_chunk(z, h[c][n], e1[c][n]) : fmaf(exp2_hw(z), h[c][n], e1[c][n]);
       }
+  }
+  return most;
+}
+// The same from `first` ([D][N] of the clip, or NULL: zero).
+template <class G, int NS, bool VEC>
+__device__ __forceinline__ void join_chunks(const ScanParams& p, const Where& w, const float* first, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
+  const auto begin = [&] {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
+    if (first) load_dn<NS>(p, first + (int64_t)w.b * p.a.D * p.a.N, w, h);
+  };
+  begin();
+  if (__any(pass_chunks<G, NS, VEC, false>(p, w, q, step, count, A2, h) > 126.0f)) {
+    begin();
+    pass_chunks<G, NS, VEC, true>(p, w, q, step, count, A2, h);
   }
 }
 
@@ -490,13 +514,9 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(S
   if (!ENDS && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
   } else {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
-    if (!ENDS && a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
-    if (!ENDS) pass_chunks<G, NS, VEC>(p, w, 0, 1, w.chunk, A2, h);
+    join_chunks<G, NS, VEC>(p, w, ENDS ? nullptr : a.h0, 0, 1, ENDS ? 0 : w.chunk, A2, h);
   }
+  arrived<NS>(h);
 
   for (int i0 = w.begin; i0 < w.end; i0 += G::TT) {
     T4<T> xs[G::R], zs[G::R];
@@ -742,9 +762,9 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
   if (!ENDS && w.own > 0 && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
   } else if (!ENDS) {
-    if (a.dh_last) load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
-    if (w.own > 0) pass_chunks<G, NS, VEC>(p, w, p.K - 1, -1, p.K - 1 - w.chunk, A2, g);
+    join_chunks<G, NS, VEC>(p, w, a.dh_last, p.K - 1, -1, w.own > 0 ? p.K - 1 - w.chunk : 0, A2, g);
   }
+  arrived<NS>(g);
 
   // what the lane adds to dB and dC: one of its 2 NS sums, or none
   const int held = sum_index<2 * NS, G::J>(w.j), place = held < 0 ? -1 : held < NS ? w.s * NS + held : G::NP + w.s * NS + held - NS;
