@@ -79,38 +79,64 @@ __global__ void __launch_bounds__(256) norm_stats_kernel(const NormParams p) {
   __shared__ float s_m[256][V + 1], s_v[256][V + 1];
   __shared__ int s_n[256];
   float k[V], s1[V], s2[V];
-  int64_t n = 0;
+  int n = 0;
   if (q.in) {
     const T* x = static_cast<const T*>(a.x) + q.b * p.S * a.C + q.c;
     int64_t r = q.r0 + q.ty;
     if (r < end) {
+      float m2[V];
       load_n<T, V, VEC>(x + r * a.C, V, k);
 #pragma unroll
       for (int c = 0; c < V; ++c) s1[c] = s2[c] = 0.0f;
       n = 1;
       r += q.step;
+      const auto walk = [&](int64_t stop) {
+        int more = 0;
 #pragma unroll 4
-      for (; r < end; r += q.step) {
-        float v[V];
-        load_n<T, V, VEC>(x + r * a.C, V, v);
-        ++n;
+        for (; r < stop; r += q.step) {
+          float v[V];
+          load_n<T, V, VEC>(x + r * a.C, V, v);
+          ++more;
 #pragma unroll
-        for (int c = 0; c < V; ++c) {
-          const float e = v[c] - k[c];
-          s1[c] += e;
-          s2[c] = fmaf(e, e, s2[c]);
+          for (int c = 0; c < V; ++c) {
+            const float e = v[c] - k[c];
+            s1[c] += e;
+            s2[c] = fmaf(e, e, s2[c]);
+          }
         }
-      }
+        return more;
+      };
+      n += walk(std::min(end, r + 15 * q.step));
       const float inv = 1.0f / (float)n;
 #pragma unroll
       for (int c = 0; c < V; ++c) {
         const float m = s1[c] * inv;
-        s_m[threadIdx.x][c] = k[c] + m;
-        s_v[threadIdx.x][c] = fmaf(-m, s1[c], s2[c]);
+        k[c] += m;
+        m2[c] = fmaf(-m, s1[c], s2[c]);
+      }
+      // The first value may lie far from the others (a recording that begins with a click): after 16, 128, 1024 .. rows the next are
+      // summed relative to the mean of those, which is no further off than a fraction of what the sum of squares holds.
+      while (r < end) {
+#pragma unroll
+        for (int c = 0; c < V; ++c) s1[c] = s2[c] = 0.0f;
+        const int more = walk(std::min(end, r + (int64_t)(7 * n) * q.step));
+        const float inv = 1.0f / (float)more, all = 1.0f / (float)(n + more), part = (float)n * all;
+        n += more;
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          const float d = s1[c] * inv;
+          m2[c] += fmaf(d * s1[c], part, fmaf(-d, s1[c], s2[c]));
+          k[c] = fmaf(s1[c], all, k[c]);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        s_m[threadIdx.x][c] = k[c];
+        s_v[threadIdx.x][c] = m2[c];
       }
     }
   }
-  s_n[threadIdx.x] = (int)n;
+  s_n[threadIdx.x] = n;
   // the lanes of a channel in pairs, half as many each time
   for (int half = p.half; half >= 1; half /= 2) {
     __syncthreads();

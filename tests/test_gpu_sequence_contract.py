@@ -194,3 +194,24 @@ def test_scan_growth_over_a_chunk_meets_a_small_state():
         _close(last, want, U * (8 * 160 + 8 * 32) * want, "last")
         (g,) = torch.autograd.grad(last, state, torch.full_like(last, 1e-36))
         _close(g, want, U * (8 * 160 + 8 * 32) * want, "dstate")
+
+
+@pytest.mark.parametrize("c,groups", ((129, 129), (129, 3)))
+def test_norm_of_clips_that_begin_with_a_spike(c, groups):
+    """A first frame a hundred spreads away in clips of which one lane walks 600 rows: the variance keeps its digits (100 u, the bound of
+    every other case).  All clips but two are zeros."""
+    import sed_amd
+    nb, n, pick = 2048, 600, [5, 2047]
+    rng = np.random.default_rng(c + groups)
+    v = rng.standard_normal((2, n, c))
+    v[:, 0] += 100.0
+    x, rx = _rounded(v, torch.float32)
+    dy, rdy = _rounded(rng.standard_normal((2, n, c)), torch.float32)
+    bx, bdy = (torch.zeros(nb, n, c, device=_dev()) for _ in range(2))
+    bx[pick], bdy[pick] = x, dy
+    bx.requires_grad_(True)
+    o, _ = S.group_norm(rx.reshape(2, n, 1, c), groups, None, None, 1e-5, None, None, rdy.reshape(2, n, 1, c))
+    y = sed_amd.group_norm_act(bx, groups)
+    _close(y[pick], o["y"][0].reshape(2, n, c), o["y"][1].reshape(2, n, c), "y")
+    (dx,) = torch.autograd.grad(y, bx, bdy)
+    _close(dx[pick], o["dx"][0].reshape(2, n, c), o["dx"][1].reshape(2, n, c), "dx")
