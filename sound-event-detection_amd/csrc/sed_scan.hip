@@ -1216,7 +1216,7 @@ template <int NS, int SPLIT, class T, bool VEC, bool BACK>
 int launch(const ScanParams& p, hipStream_t stream) {
   using G = Geo<NS, SPLIT>;
   const sed_scan_args& a = p.a;
-  const int64_t waves = a.B * p.K * a.G * p.tiles, joins = a.B * G::NP * a.D / 16;
+  const int64_t waves = a.B * p.K * a.G * p.tiles, joins = p.K > kOwnJoin ? a.B * G::NP * a.D / 16 : 0;
   if (!grid_fits(waves + 4, 64) || !grid_fits(joins + 1, 1024)) return SED_ERR_CAPACITY;
   constexpr int WE = waves_of<T, BACK, true>(), WM = waves_of<T, BACK, false>();  // of the ends, of the main pass
   const unsigned ends = (unsigned)((waves + WE - 1) / WE), main = (unsigned)((waves + WM - 1) / WM);

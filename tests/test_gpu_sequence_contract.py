@@ -6,7 +6,7 @@ import torch
 from torch.autograd import forward_ad
 
 from oracle import sequence as S
-from test_gpu_sequence import NAMES, U, _close, _dev, _rounded, _scan_inputs
+from test_gpu_sequence import NAMES, U, _close, _dev, _rounded, _scan_bound, _scan_inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -215,3 +215,33 @@ def test_norm_of_clips_that_begin_with_a_spike(c, groups):
     _close(y[pick], o["y"][0].reshape(2, n, c), o["y"][1].reshape(2, n, c), "y")
     (dx,) = torch.autograd.grad(y, bx, bdy)
     _close(dx[pick], o["dx"][0].reshape(2, n, c), o["dx"][1].reshape(2, n, c), "dx")
+
+
+def test_scan_batches_of_many_states():
+    """Clips x states x channels past 2^26 in one call: all clips but two are zeros, so that those two are the parameters' gradient."""
+    import sed_amd
+    nb, n, d, ns, pick = 2100, 1, 1024, 32, [7, 2099]
+    small, ref, rng = _scan_inputs(2, n, d, 1, ns, torch.bfloat16, 21)
+    dy, rdy = _rounded(rng.standard_normal((2, n, d)), torch.bfloat16)
+    big = {}
+    for k, t in small.items():
+        if t.shape[0] == 2 and t.dim() >= 3:
+            big[k] = torch.zeros(nb, *t.shape[1:], dtype=t.dtype, device=_dev())
+            big[k][pick] = t
+        else:
+            big[k] = t
+    bdy = torch.zeros(nb, n, d, dtype=torch.bfloat16, device=_dev())
+    bdy[pick] = dy
+    leaves = {k: t.requires_grad_(True) for k, t in big.items()}
+    args = dict(leaves)
+    y, last = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, softplus=True, return_state=True)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), bdy)))
+    o = S.scan(**ref, use_softplus=True, dy=rdy)
+    _close(y[pick], o["y"][0], _scan_bound(o, "y", nb, n, d), "y")
+    _close(last[pick], o["last"][0], _scan_bound(o, "last", nb, n, d), "last")
+    for k, got in grads.items():
+        _close(got[pick] if big[k].shape[0] == nb else got, o[NAMES[k]][0], _scan_bound(o, NAMES[k], nb, n, d), NAMES[k])
+    with torch.no_grad():
+        y20 = sed_amd.gated_scan(*(t.expand(-1, 3, *t.shape[2:]) if t.dim() >= 3 else t for t in (leaves[k] for k in ("x", "dt", "A", "B", "C"))), softplus=True)
+        alone = sed_amd.gated_scan(*(t[pick].expand(-1, 3, *t.shape[2:]) if t.dim() >= 3 else t for t in (leaves[k] for k in ("x", "dt", "A", "B", "C"))), softplus=True)
+    assert torch.allclose(y20[pick].float(), alone.float(), rtol=2.0 ** -7, atol=1e-5)
