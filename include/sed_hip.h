@@ -371,7 +371,7 @@ typedef struct sed_scan_args {
   const int32_t* frames;    /* [B] or NULL                                                         */
   const void *x, *dt, *z;   /* [B][L][D]; z may be NULL (no gate)                                  */
   const void *Bm, *Cm;      /* [B][L][G][N]                                                        */
-  int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, Bm_b, Bm_t, Bm_g, Cm_b, Cm_t, Cm_g; /* rows (.._t) 0..2^26 apart */
+  int64_t x_b, x_t, dt_b, dt_t, z_b, z_t, Bm_b, Bm_t, Bm_g, Cm_b, Cm_t, Cm_g; /* rows (.._t) 0..2^26 apart; not read for L = 1 */
   const float *A, *skip, *dt_bias; /* [D][N], [D] or NULL, [D] or NULL                             */
   const float* h0;          /* [B][D][N] state in front of the first frame, or NULL (zero)         */
   float* h_last;            /* [B][D][N] state behind the last, or NULL; the state of a step       */

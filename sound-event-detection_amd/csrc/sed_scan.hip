@@ -1191,7 +1191,7 @@ int check_args(const sed_scan_args* a) {
   if (a->dtype != SED_F32 && a->dtype != SED_BF16 && a->dtype != SED_F16) return SED_ERR_BAD_ARG;
   if (a->B > 0 && a->L > 0 && (!a->x || !a->dt || !a->A || !a->Bm || !a->Cm)) return SED_ERR_BAD_ARG;
   for (const int64_t t : {a->x_t, a->dt_t, a->z_t, a->dy_t, a->Bm_t, a->Cm_t})
-    if (t < 0 || t > (1 << 26)) return SED_ERR_CAPACITY;
+    if (a->L > 1 && (t < 0 || t > (1 << 26))) return SED_ERR_CAPACITY;
   return SED_OK;
 }
 
@@ -1257,6 +1257,7 @@ int launch_t(const ScanParams& p, bool vec, hipStream_t s) {
 int run(const sed_scan_args* args, bool back, void* stream) {
   ScanParams p{};
   p.a = *args;
+  if (p.a.L == 1) p.a.x_t = p.a.dt_t = p.a.z_t = p.a.dy_t = p.a.Bm_t = p.a.Cm_t = 0;  // of a single row any distance, so none that the kernels could form
   const Layout l = layout_of(p.a, back);
   if (l.total > 0 && (!args->ws || args->ws_bytes < l.total * 4 || !aligned(args->ws, 16))) return SED_ERR_CAPACITY;
   float* ws = static_cast<float*>(args->ws);

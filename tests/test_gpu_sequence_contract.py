@@ -245,3 +245,23 @@ def test_scan_batches_of_many_states():
         y20 = sed_amd.gated_scan(*(t.expand(-1, 3, *t.shape[2:]) if t.dim() >= 3 else t for t in (leaves[k] for k in ("x", "dt", "A", "B", "C"))), softplus=True)
         alone = sed_amd.gated_scan(*(t[pick].expand(-1, 3, *t.shape[2:]) if t.dim() >= 3 else t for t in (leaves[k] for k in ("x", "dt", "A", "B", "C"))), softplus=True)
     assert torch.allclose(y20[pick].float(), alone.float(), rtol=2.0 ** -7, atol=1e-5)
+
+
+@pytest.mark.parametrize("reverse", (False, True))
+@pytest.mark.parametrize("d", (6, 8))
+def test_scan_of_one_frame_has_no_row_distance(d, reverse):
+    """One frame whose frame axis has a stride past 2^26 (a time-major sequence's first frame): never used, so never refused."""
+    import sed_amd
+    dev, _, rng = _scan_inputs(3, 1, d, 1, 4, torch.float32, d, state=True)
+    dy = torch.from_numpy(rng.standard_normal((3, 1, d)).astype(np.float32)).to(_dev())
+    far = lambda t: t.as_strided(t.shape, (t.stride(0), (1 << 26) + 4, *t.stride()[2:]))  # noqa: E731
+    got = []
+    for wide in (lambda t: t, far):
+        leaves = {k: t.detach().clone().requires_grad_(True) for k, t in dev.items()}
+        args = {k: wide(t) if k in ("x", "dt", "B", "C", "z") else t for k, t in leaves.items()}
+        y, last = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, softplus=True, reverse=reverse, return_state=True)
+        got.append([y, last, *torch.autograd.grad(y, list(leaves.values()), wide(dy))])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    x = dev["x"]
+    w = torch.from_numpy(rng.standard_normal((d, 4)).astype(np.float32)).to(_dev())
+    assert torch.equal(sed_amd.causal_conv(far(x), w, reverse=reverse), sed_amd.causal_conv(x, w, reverse=reverse))
