@@ -389,7 +389,8 @@ typedef struct sed_scan_args {
 } sed_scan_args;
 
 int64_t sed_gated_scan_saved_floats(int64_t B, int64_t L, int64_t D, int32_t N);
-/* Bytes of workspace of a call with these sizes (B, L, D, N, G, and whether frames is NULL; nothing is read through pointers). */
+/* Bytes of workspace of a call with these sizes, in any element type (B, L, D, N, G, and whether frames is NULL; nothing is read
+ * through pointers). */
 int64_t sed_gated_scan_workspace(const sed_scan_args* args, int32_t backward);
 int sed_gated_scan_forward(const sed_scan_args* args, void* stream);
 /* Reads the inputs of the forward call and its `saved`. */

@@ -1321,7 +1321,17 @@ extern "C" int64_t sed_gated_scan_saved_floats(int64_t B, int64_t L, int64_t D, 
 
 extern "C" int64_t sed_gated_scan_workspace(const sed_scan_args* a, int32_t backward) {
   if (!a || a->B < 0 || a->L < 0 || a->D < 1 || a->N < 1 || a->N > 32 || a->G < 1 || a->D % a->G) return SED_ERR_BAD_ARG;
-  return sed::layout_of(*a, backward != 0).total * 4;
+  // The gradient's chunks follow from the waves that LDS leaves room for, and so from the element's size where that differs: the larger
+  // of both answers serves every type.
+  sed_scan_args b = *a;
+  b.dtype = SED_F32;
+  int64_t most = sed::layout_of(b, backward != 0).total;
+  const sed::Shape s = sed::shape_of(a->N, false);
+  if (backward && sed::resident(s, true, 4) != sed::resident(s, true, 2)) {
+    b.dtype = SED_BF16;
+    most = std::max(most, sed::layout_of(b, true).total);
+  }
+  return most * 4;
 }
 
 extern "C" int sed_gated_scan_forward(const sed_scan_args* args, void* stream) {
