@@ -265,3 +265,119 @@ def test_scan_of_one_frame_has_no_row_distance(d, reverse):
     x = dev["x"]
     w = torch.from_numpy(rng.standard_normal((d, 4)).astype(np.float32)).to(_dev())
     assert torch.equal(sed_amd.causal_conv(far(x), w, reverse=reverse), sed_amd.causal_conv(x, w, reverse=reverse))
+
+
+@pytest.mark.parametrize("dtype", ("fp32", "bf16"))
+@pytest.mark.parametrize("d,start", ((64, 0), (64, 1), (20, 0), (21, 3)))
+@pytest.mark.parametrize("n,reverse", ((50, False), (300, True)))
+def test_scan_gradients_of_views(n, reverse, d, start, dtype):
+    """x, dt, z, B and C as slices of joint projections, dy with strides of its own: every gradient has the bits of the same call on copies."""
+    import sed_amd
+    t = {"fp32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    g = torch.Generator(device=_dev()).manual_seed(n + d)
+    r = lambda *s: torch.randn(s, generator=g, device=_dev())  # noqa: E731
+    nb, ns = 3, 16
+    rest = 4 * ((start + 3 * d + 2 * ns + 7) // 4)
+    xzt, bc, bc4 = r(nb, n, rest).to(t), r(nb, n, 2 * ns + start).to(t), r(nb, n, 2, 3 * ns).to(t)
+    A, D, bias = -4 * torch.rand(d, ns, generator=g, device=_dev()), r(d), 0.3 * r(d) - 2
+    frames = torch.tensor([n, n // 3, 1], dtype=torch.int32, device=_dev())
+    gaps = r(nb, n, 2 * d + 4 * start).to(t)
+    time_major, wide = r(n, nb, d).to(t), r(nb, n + 5, d + 4).to(t)
+    cases = ((xzt[..., start:start + d], xzt[..., start + d:start + 2 * d], xzt[..., start + 2 * d:start + 3 * d], bc[..., start:start + ns], bc[..., start + ns:], gaps[..., start:start + d]),
+             (time_major.transpose(0, 1), wide[:, 5:, :d], wide[:, :n, 4:], bc[..., :ns], bc[..., ns:2 * ns], r(n, nb, d).to(t).transpose(0, 1)))
+    if d % 2 == 0:
+        cases += ((xzt[..., :d], wide[:, :n, :d], None, bc4[..., :ns], bc4[..., 2 * ns:], wide[:, 5:, 4:]),)
+    for x, dt, z, B, C, dy in cases:
+        got = []
+        for keep in (lambda v: v, lambda v: v.contiguous()):
+            # leaves are the views themselves, so that the call meets their strides
+            data = [None if v is None else keep(v).detach().requires_grad_(True) for v in (x, dt, z, B, C)]
+            lx, ldt, lz, lB, lC = data
+            p = [v.clone().requires_grad_(True) for v in (A, D, bias)]
+            y, last = sed_amd.gated_scan(lx, ldt, p[0], lB, lC, D=p[1], z=lz, dt_bias=p[2], softplus=True, frames=frames, reverse=reverse, return_state=True)
+            leaves = [v for v in data if v is not None] + p
+            got.append([y, last, *torch.autograd.grad(y, leaves, keep(dy))])
+        for k, (a, b) in enumerate(zip(*got)):
+            assert torch.equal(a, b), k
+
+
+@pytest.mark.parametrize("dtype", ("fp32", "bf16"))
+@pytest.mark.parametrize("d,start", ((256, 0), (256, 1), (40, 0), (33, 3)))
+@pytest.mark.parametrize("W", (3, 4, 8))
+def test_conv_gradients_of_views(W, d, start, dtype):
+    import sed_amd
+    t = {"fp32": torch.float32, "bf16": torch.bfloat16}[dtype]
+    g = torch.Generator(device=_dev()).manual_seed(W + d)
+    r = lambda *s: torch.randn(s, generator=g, device=_dev())  # noqa: E731
+    nb, n = 3, 130
+    joint, gaps = r(nb, n, 2 * d + 4 * start).to(t), r(nb, n + 3, d + 4).to(t)
+    w, b = r(d, W), r(d)
+    frames = torch.tensor([n, n // 3, 1], dtype=torch.int32, device=_dev())
+    for x, dy in ((joint[..., start:start + d], gaps[:, 3:, start:start + d]), (r(n, nb, d).to(t).transpose(0, 1), r(n, nb, d).to(t).transpose(0, 1)),
+                  (joint[..., d:2 * d], joint[..., :d]), (r(nb, d, n).to(t).transpose(1, 2), r(nb, d, n).to(t).transpose(1, 2))):
+        for reverse in (False, True):
+            got = []
+            for keep in (lambda v: v, lambda v: v.contiguous()):
+                leaves = [v.detach().requires_grad_(True) for v in (keep(x), w.clone(), b.clone())]
+                y, last = sed_amd.causal_conv(*leaves, activation="silu", frames=frames, reverse=reverse, return_state=True)
+                got.append([y, last, *torch.autograd.grad(y, leaves, keep(dy))])
+            assert all(torch.equal(p, q) for p, q in zip(*got))
+
+
+def test_norm_gradients_of_views():
+    import sed_amd
+    g = torch.Generator(device=_dev()).manual_seed(8)
+    r = lambda *s: torch.randn(s, generator=g, device=_dev())  # noqa: E731
+    for x, dy in ((r(3, 16, 40, 2).permute(0, 2, 3, 1), r(3, 16, 40, 2).permute(0, 2, 3, 1)), (r(3, 40, 2, 40)[..., 1:17], r(40, 3, 2, 16).transpose(0, 1)),
+                  (r(3, 40, 2, 32)[..., ::2], r(1, 1, 1, 16).expand(3, 40, 2, 16))):
+        got = []
+        for keep in (lambda v: v, lambda v: v.contiguous()):
+            leaves = [v.detach().requires_grad_(True) for v in (keep(x), torch.ones(16, device=_dev()), torch.zeros(16, device=_dev()))]
+            y = sed_amd.group_norm_act(leaves[0], 4, leaves[1], leaves[2], activation="silu")
+            got.append([y, *torch.autograd.grad(y, leaves, keep(dy))])
+        assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def _norm_relu(shape, groups, dtype, seed, frames=None):
+    """relu, whose slope jumps where u = 0.  Values of x whose u lies within four errors of the corner move by a tenth of the spread,
+    before anything is run, until none is left (moving one moves its group's statistics, hence a few rounds)."""
+    import sed_amd
+    rng = np.random.default_rng(seed)
+    c = shape[-1]
+    four = (shape[0], shape[1], int(np.prod(shape[2:-1])), c)
+    w, rw = _rounded(1 + 0.3 * rng.standard_normal(c), torch.float32)
+    b, rb = _rounded(0.3 * rng.standard_normal(c), torch.float32)
+    dy, rdy = _rounded(rng.standard_normal(shape), dtype)
+    v = rng.standard_normal(shape)
+    near = 1e-3  # more than four times the error of u at these sizes, as the assertion below checks
+    for _ in range(20):
+        x, rx = _rounded(v, dtype)
+        q = rx.reshape(four)
+        u = np.full(four, np.inf)
+        for k in range(shape[0]):
+            own = shape[1] if frames is None else frames[k]
+            if own:
+                z = q[k, :own].reshape(own * four[2], groups, -1)
+                hat = (z - z.mean((0, 2), keepdims=True)) / np.sqrt(z.var((0, 2), keepdims=True) + 1e-5)
+                u[k, :own] = hat.reshape(own, four[2], c) * rw + rb
+        bad = np.abs(u) < near
+        if not bad.any():
+            break
+        v = v + 0.1 * bad.reshape(shape)
+    o, clear = S.group_norm(rx.reshape(four), groups, rw, rb, 1e-5, "relu", frames, rdy.reshape(four))
+    assert clear > 1
+    fr = None if frames is None else torch.tensor(frames, dtype=torch.int32, device=_dev())
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = sed_amd.group_norm_act(x, groups, w, b, activation="relu", frames=fr)
+    _close(y, o["y"][0].reshape(shape), o["y"][1].reshape(shape), "y")
+    for k, got in zip(("dx", "dw", "db"), torch.autograd.grad(y, leaves, dy)):
+        s = shape if k == "dx" else (c,)
+        _close(got, o[k][0].reshape(s), o[k][1].reshape(s), k)
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("shape,groups,frames", (((3, 9000, 32), 4, (9000, 5, 4501)), ((2, 900, 3, 30), 6, (1, 900)), ((1, 901, 33), 3, None), ((2, 433, 3, 64), 8, None),
+                                                 ((2, 33, 96), 2, (33, 7)), ((3, 7, 24), 1, (7, 0, 2)), ((1, 4, 4096), 1, None), ((600, 3, 16), 2, None), ((1, 2000, 64), 1, None)))
+def test_norm_relu(shape, groups, frames, dtype):
+    """Every kernel with relu: walks with whole vectors and single channels, groups held whole with 4 and 8 channels a lane."""
+    _norm_relu(shape, groups, dtype, sum(shape), frames)
