@@ -421,16 +421,17 @@ int go_w(const ConvParams& p, Kind kind, hipStream_t s) {
 template <class T>
 int go(const ConvParams& p, Kind kind, int V, hipStream_t s) {
   const sed_conv_args& a = p.a;
-  int rc = V == 4 ? go_w<T, 4>(p, kind, s) : go_w<T, 1>(p, kind, s);
-  if (rc != SED_OK || kind == STEP || a.W == 1) return rc;
+  const bool state = a.W > 1 && (kind == FORWARD ? a.state_out != nullptr : kind == BACKWARD && a.dstate);
   const int64_t grid = (a.B * (a.W - 1) * a.D + 255) / 256;
-  if (!grid_fits(grid, 256)) return SED_ERR_CAPACITY;
-  if (kind == FORWARD && a.state_out) conv_state_kernel<T><<<(unsigned)grid, 256, 0, s>>>(a);
-  if (kind == BACKWARD && a.dstate) {
-    if (a.act == SED_ACT_SILU)
-      conv_state_grad_kernel<T, SED_ACT_SILU><<<(unsigned)grid, 256, 0, s>>>(a);
-    else
-      conv_state_grad_kernel<T, SED_ACT_NONE><<<(unsigned)grid, 256, 0, s>>>(a);
+  if (state && !grid_fits(grid, 256)) return SED_ERR_CAPACITY;
+  const int rc = V == 4 ? go_w<T, 4>(p, kind, s) : go_w<T, 1>(p, kind, s);
+  if (rc != SED_OK || !state) return rc;
+  if (kind == FORWARD) {
+    conv_state_kernel<T><<<(unsigned)grid, 256, 0, s>>>(a);
+  } else if (a.act == SED_ACT_SILU) {
+    conv_state_grad_kernel<T, SED_ACT_SILU><<<(unsigned)grid, 256, 0, s>>>(a);
+  } else {
+    conv_state_grad_kernel<T, SED_ACT_NONE><<<(unsigned)grid, 256, 0, s>>>(a);
   }
   return seq_status(hipGetLastError());
 }

@@ -381,3 +381,29 @@ def _norm_relu(shape, groups, dtype, seed, frames=None):
 def test_norm_relu(shape, groups, frames, dtype):
     """Every kernel with relu: walks with whole vectors and single channels, groups held whole with 4 and 8 channels a lane."""
     _norm_relu(shape, groups, dtype, sum(shape), frames)
+
+
+def test_conv_of_many_clips_without_a_state():
+    """Clips x rows of state x channels past 2^32 where no state is given or asked for: nothing of that size is launched."""
+    import sed_amd
+    nb, d, W, pick = 150000, 4096, 8, [0, 77777, 149999]
+    assert nb * (W - 1) * d >= 1 << 32
+    g = torch.Generator(device=_dev()).manual_seed(2)
+    x = torch.zeros(nb, 1, d, dtype=torch.float16, device=_dev())
+    x[pick] = torch.randn(3, 1, d, generator=g, device=_dev()).half()
+    w, b = torch.randn(d, W, generator=g, device=_dev()), torch.randn(d, generator=g, device=_dev())
+    y = sed_amd.causal_conv(x, w, b, activation="silu")
+    assert torch.equal(y[pick], sed_amd.causal_conv(x[pick], w, b, activation="silu"))
+    del y
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dy = torch.zeros(nb, 1, d, dtype=torch.float16, device=_dev())
+    dy[pick] = torch.randn(3, 1, d, generator=g, device=_dev()).half()
+    dx, dw, db = torch.autograd.grad(sed_amd.causal_conv(*leaves, activation="silu"), leaves, dy)
+    alone = []
+    for i in pick:
+        few = [x.detach()[i:i + 1].requires_grad_(True), w, b]
+        alone.append(torch.autograd.grad(sed_amd.causal_conv(*few, activation="silu"), few, dy[i:i + 1]))
+    assert torch.equal(dx[pick], torch.cat([t[0] for t in alone]))
+    for k, got in ((1, dw), (2, db)):  # zeros add nothing; three clips' terms in some order, here and there
+        terms = torch.stack([t[k].double() for t in alone])
+        assert ((got.double() - terms.sum(0)).abs() <= 2 * U * terms.abs().sum(0)).all()
