@@ -812,6 +812,7 @@ int launch(const NormParams& p, bool back, hipStream_t s) {
         if (const int n = whole_threads(p, 4, 4, true)) return launch_whole_grad<T, 4, ACT>(p, n, s);
     }
   }
+  if (!grid_fits(a.B * a.G, 256)) return SED_ERR_CAPACITY;  // of the joins
   const dim3 grid((unsigned)p.blocks, (unsigned)a.B, (unsigned)((p.nv + p.nb - 1) / p.nb)), late((unsigned)p.late, grid.y, grid.z);
   // more blocks and channels a group than a workgroup joins in 8 steps: a launch of its own for the blocks
   const int64_t cg = a.C / a.G;
@@ -861,7 +862,6 @@ int run(const sed_norm_args* args, bool back, void* stream) {
   p.S = a.T * a.F;
   const Layout l = layout_of(a.B, p.S, a.C, a.G);
   if (!a.ws || a.ws_bytes < l.total * 4 || !aligned(a.ws, 16)) return SED_ERR_CAPACITY;
-  if (!grid_fits(a.B * a.G, 256)) return SED_ERR_CAPACITY;
   const int V = a.dtype == SED_F32 ? 4 : 8;
   const bool vec = a.C % V == 0 && aligned(a.x, 16) && aligned(a.y, 16) && aligned(a.dy, 16) && aligned(a.dx, 16);
   p.nv = (int32_t)(vec ? a.C / V : a.C);

@@ -407,3 +407,26 @@ def test_conv_of_many_clips_without_a_state():
     for k, got in ((1, dw), (2, db)):  # zeros add nothing; three clips' terms in some order, here and there
         terms = torch.stack([t[k].double() for t in alone])
         assert ((got.double() - terms.sum(0)).abs() <= 2 * U * terms.abs().sum(0)).all()
+
+
+def test_norm_of_many_groups_held_whole():
+    """Clips x groups past 2^24, each held by one workgroup: the walks' joining launch is not needed, so its grid sets no limit."""
+    import sed_amd
+    nb, groups, cg, pick = 65535, 258, 8, [0, 40001, 65534]
+    c = groups * cg
+    assert nb * groups > 1 << 24
+    rng = np.random.default_rng(6)
+    x, rx = _rounded(rng.standard_normal((3, 1, c)), torch.float32)
+    dy, rdy = _rounded(rng.standard_normal((3, 1, c)), torch.float32)
+    w, rw = _rounded(1 + 0.3 * rng.standard_normal(c), torch.float32)
+    b, rb = _rounded(0.3 * rng.standard_normal(c), torch.float32)
+    bx, bdy = (torch.zeros(nb, 1, c, device=_dev()) for _ in range(2))
+    bx[pick], bdy[pick] = x, dy
+    leaves = [t.requires_grad_(True) for t in (bx, w, b)]
+    y = sed_amd.group_norm_act(bx, groups, w, b, activation="silu")
+    o, _ = S.group_norm(rx.reshape(3, 1, 1, c), groups, rw, rb, 1e-5, "silu", None, rdy.reshape(3, 1, 1, c))
+    _close(y[pick], o["y"][0].reshape(3, 1, c), o["y"][1].reshape(3, 1, c), "y")
+    grads = torch.autograd.grad(y, leaves, bdy)  # clips without a gradient add nothing to w and b
+    _close(grads[0][pick], o["dx"][0].reshape(3, 1, c), o["dx"][1].reshape(3, 1, c), "dx")
+    for k, got in zip(("dw", "db"), grads[1:]):
+        _close(got, o[k][0], o[k][1], k)
