@@ -997,23 +997,24 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
   }
 }
 
-// dB and dC: the waves' sums over their channels, added over a group's channel tiles in order, rounded once.
+// dB and dC: the waves' sums over their channels, added over a group's channel tiles in order, rounded once.  A value a thread, or
+// several where there are more than a grid has threads.
 template <class T>
 __global__ void __launch_bounds__(256) scan_bc_kernel(const ScanParams p, int NP) {
   const sed_scan_args& a = p.a;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t rows = a.B * a.G * a.L;
-  if (i >= rows * 2 * NP) return;
-  const int e = (int)(i % (2 * NP)), n = e % NP;
-  const int64_t r = i / (2 * NP), t = r % a.L, g = r / a.L % a.G, b = r / a.L / a.G;
-  if (n >= a.N) return;
-  const bool in = !a.frames || t < a.frames[b];
-  float v = 0.0f;
-  if (in) {
-    const float* q = p.part_bc + ((b * a.G + g) * p.tiles * a.L + t) * (2 * NP) + e;
-    for (int k = 0; k < p.tiles; ++k) v += q[(int64_t)k * a.L * 2 * NP];
+  const int64_t all = a.B * a.G * a.L * 2 * NP;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int e = (int)(i % (2 * NP)), n = e % NP;
+    const int64_t r = i / (2 * NP), t = r % a.L, g = r / a.L % a.G, b = r / a.L / a.G;
+    if (n >= a.N) continue;
+    const bool in = !a.frames || t < a.frames[b];
+    float v = 0.0f;
+    if (in) {
+      const float* q = p.part_bc + ((b * a.G + g) * p.tiles * a.L + t) * (2 * NP) + e;
+      for (int k = 0; k < p.tiles; ++k) v += q[(int64_t)k * a.L * 2 * NP];
+    }
+    static_cast<T*>(e < NP ? a.dB : a.dC)[((b * a.L + t) * a.G + g) * a.N + n] = (T)v;
   }
-  static_cast<T*>(e < NP ? a.dB : a.dC)[((b * a.L + t) * a.G + g) * a.N + n] = (T)v;
 }
 
 // dA [D][N], d skip and d dt_bias [D]: sums over clips and chunks; dA's partial sums lie [NP][D].
@@ -1227,8 +1228,8 @@ int launch(const ScanParams& p, hipStream_t stream) {
     }
     scan_forward_kernel<NS, SPLIT, T, VEC, false><<<main, 64 * WM, 0, stream>>>(p);
   } else {
-    const int64_t bc = (a.B * a.G * a.L * 2 * G::NP + 255) / 256, pr = ((a.N + 2) * a.D + kColumns - 1) / kColumns;
-    if (!grid_fits(bc, 256) || !grid_fits(pr, 1024)) return SED_ERR_CAPACITY;
+    const int64_t bc = std::min<int64_t>((a.B * a.G * a.L * 2 * G::NP + 255) / 256, 1 << 23), pr = ((a.N + 2) * a.D + kColumns - 1) / kColumns;
+    if (!grid_fits(pr, 1024)) return SED_ERR_CAPACITY;
     if (p.K > 1) {
       scan_backward_kernel<NS, SPLIT, T, VEC, true><<<ends, 64 * WE, 0, stream>>>(p);
       launch_join<G, true>(p, stream);

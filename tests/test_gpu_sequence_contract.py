@@ -430,3 +430,30 @@ def test_norm_of_many_groups_held_whole():
     _close(grads[0][pick], o["dx"][0].reshape(3, 1, c), o["dx"][1].reshape(3, 1, c), "dx")
     for k, got in zip(("dw", "db"), grads[1:]):
         _close(got, o[k][0], o[k][1], k)
+
+
+def test_scan_gradient_of_more_rows_than_a_grid_has_threads():
+    """dB and dC of clips x frames x states past 2^32 values together: all clips but three are zeros."""
+    import sed_amd
+    nb, n, ns, pick = (1 << 18) + 8, 256, 32, [3, 1 << 17, (1 << 18) + 7]
+    assert nb * n * 2 * ns >= 1 << 32
+    small, ref, rng = _scan_inputs(3, n, 1, 1, ns, torch.bfloat16, 31, gate=False)
+    dy, rdy = _rounded(rng.standard_normal((3, n, 1)), torch.bfloat16)
+    big = dict(small)
+    for k in ("x", "dt", "B", "C"):
+        big[k] = torch.zeros(nb, *small[k].shape[1:], dtype=torch.bfloat16, device=_dev())
+        big[k][pick] = small[k]
+    bdy = torch.zeros(nb, n, 1, dtype=torch.bfloat16, device=_dev())
+    bdy[pick] = dy
+    leaves = {k: t.requires_grad_(True) for k, t in big.items()}
+    args = dict(leaves)
+    y = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, softplus=True)
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), bdy)))
+    o = S.scan(**ref, use_softplus=True, dy=rdy)
+    _close(y[pick], o["y"][0], _scan_bound(o, "y", 3, n, 1), "y")
+    for k in ("x", "dt", "B", "C"):
+        _close(grads[k][pick], o[NAMES[k]][0], _scan_bound(o, NAMES[k], 3, n, 1), NAMES[k])
+    for k in ("A", "D", "dt_bias"):  # zeros add nothing to a sum
+        _close(grads[k], o[NAMES[k]][0], _scan_bound(o, NAMES[k], 3, n, 1), NAMES[k])
+    rest = grads["B"][(1 << 18) - 100000:(1 << 18)]
+    assert (rest == 0).all()
