@@ -27,6 +27,7 @@
 #include "seq_core.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace sed {
 namespace {
@@ -388,10 +389,12 @@ __device__ __forceinline__ void only_own(const Where& w, int i0, int r, float (&
   for (int c = 0; c < 4; ++c) v[c] = in && (VEC ? w.nc > 0 : c < w.nc) ? v[c] : 0.0f;
 }
 
-// 2^z h + e over a chunk, z the sum of its frames' exponents.  The frames one by one would carry a state of zero, or a small one, through
-// growth that is beyond fp32 as a whole (A delta > 0), so there 2^z goes on in two halves, the second to the scaled state.
-__device__ __forceinline__ float over_chunk(float z, float h, float e) {
-  const bool far = z > 126.0f;
+// 2^z h + e over a chunk, z the sum of its frames' exponents.  FAR: the frames one by one carry a state of zero, or a small one, through
+// growth that is beyond fp32 as a whole (A delta > 0), so there 2^z goes on in two halves, the second to the scaled state.  The usual
+// decay (z <= 126) takes the short form, whose bits are the same.
+template <bool FAR>
+__device__ __forceinline__ float pass_chunk(float z, float h, float e) {
+  const bool far = FAR && z > 126.0f;
   const float f = exp2_hw(far ? std::min(0.5f * z, 127.0f) : z);
   return fmaf(f, far ? f * h : h, e);
 }
@@ -427,7 +430,7 @@ __device__ __forceinline__ float pass_chunks(const ScanParams& p, const Where& w
       for (int n = 0; n < NS; ++n) {
         const float z = A2[c][n] * s1[c];
         if (!FAR) most = fmaxf(most, z);
-        h[c][n] = FAR ? over_chunk(z, h[c][n], e1[c][n]) : fmaf(exp2_hw(z), h[c][n], e1[c][n]);
+        h[c][n] = pass_chunk<FAR>(z, h[c][n], e1[c][n]);
       }
   }
   return most;
@@ -621,26 +624,37 @@ __global__ void __launch_bounds__(1024) chunk_join_kernel(const ScanParams p) {
   const int per = (k_own + SEG - 1) / SEG, q0 = seg * per, q1 = live ? std::min(q0 + per, k_own) : 0;
   const auto at = [&](int q) { return (int64_t)(BACK ? k_own - 1 - q : q); };
   // the last chunk of the walk hands nothing on
-  {
-    float h = 0.0f, s = 0.0f;
+  const auto ends = [&](auto far) {
+    float h = 0.0f, s = 0.0f, most = 0.0f;
 #pragma unroll 4
     for (int q = q0; q < std::min(q1, k_own - 1); ++q) {
-      const float sk = sp[at(q) * a.D];
-      h = over_chunk(A2 * sk, h, hp[at(q) * NP * a.D]);
+      const float sk = sp[at(q) * a.D], z = A2 * sk;
+      h = pass_chunk<decltype(far)::value>(z, h, hp[at(q) * NP * a.D]);
       s += sk;
+      most = fmaxf(most, z);
     }
     s_h[seg][lane] = h;
     s_s[seg][lane] = s;
-    __syncthreads();
-  }
-  float h = first && real && live ? first[(b * a.D + d) * a.N + n] : 0.0f;
-  for (int k = 0; k < seg; ++k) h = over_chunk(A2 * s_s[k][lane], h, s_h[k][lane]);
+    return fmaxf(most, A2 * s);
+  };
+  const auto starts = [&](auto far) {
+    constexpr bool FAR = decltype(far)::value;
+    float h = first && real && live ? first[(b * a.D + d) * a.N + n] : 0.0f;
+    for (int k = 0; k < seg; ++k) h = pass_chunk<FAR>(A2 * s_s[k][lane], h, s_h[k][lane]);
 #pragma unroll 4
-  for (int q = q0; q < q1; ++q) {
-    const bool more = q < k_own - 1;
-    const float end = more ? hp[at(q) * NP * a.D] : 0.0f, sk = more ? sp[at(q) * a.D] : 0.0f;
-    hp[at(q) * NP * a.D] = h;
-    h = over_chunk(A2 * sk, h, end);
+    for (int q = q0; q < q1; ++q) {
+      const bool more = q < k_own - 1;
+      const float end = more ? hp[at(q) * NP * a.D] : 0.0f, sk = more ? sp[at(q) * a.D] : 0.0f;
+      hp[at(q) * NP * a.D] = h;
+      h = pass_chunk<FAR>(A2 * sk, h, end);
+    }
+  };
+  if (__syncthreads_or(ends(std::false_type{}) > 126.0f)) {
+    ends(std::true_type{});
+    __syncthreads();
+    starts(std::true_type{});
+  } else {
+    starts(std::false_type{});
   }
 }
 
