@@ -27,7 +27,6 @@
 #include "seq_core.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace sed {
 namespace {
@@ -39,7 +38,7 @@ struct ScanParams {
   int32_t K;        // chunks of a clip
   int32_t tiles;    // channel tiles of a group
   float* chunk_h;   // [B][K][NP][D]  end states from zero, then the states in front of the chunks
-  float* chunk_s;   // [B][K][D]      sums of delta
+  float* chunk_s;   // [B][K][D]      half the sums of delta
   float* part_bc;   // [B][G * tiles][L][2 * NP]  dB, dC of one wave's channels
   float* part_a;    // [B * K][D * NP] dA  [NP][D] per row
   float* part_d;    // [B * K][2][D]  d skip, d dt_bias
@@ -340,7 +339,7 @@ __device__ __forceinline__ void load_dn(const ScanParams& p, const float* base, 
 // chunk without frames) keeps its state: 0 times infinity would be a NaN.
 __device__ __forceinline__ float exponent(float A) {
   const float v = A * kLog2e;
-  return v < -3.4028235e38f ? -3.4028235e38f : v;
+  return __builtin_amdgcn_classf(v, 4) ? -3.4028235e38f : v;  // -infinity
 }
 template <int NS>
 __device__ __forceinline__ void load_exponents(const ScanParams& p, const Where& w, float (&A2)[4][NS]) {
@@ -389,23 +388,19 @@ __device__ __forceinline__ void only_own(const Where& w, int i0, int r, float (&
   for (int c = 0; c < 4; ++c) v[c] = in && (VEC ? w.nc > 0 : c < w.nc) ? v[c] : 0.0f;
 }
 
-// 2^z h + e over a chunk, z the sum of its frames' exponents.  FAR: the frames one by one carry a state of zero, or a small one, through
-// growth that is beyond fp32 as a whole (A delta > 0), so there 2^z goes on in two halves, the second to the scaled state.  The usual
-// decay (z <= 126) takes the short form, whose bits are the same.
-template <bool FAR>
+// 4^z h + e over a chunk, z half the sum of its frames' exponents.  In two steps, the second to the scaled state: the frames one by one
+// carry a state of zero, or a small one, through growth that is beyond fp32 as a whole (A delta > 0), and so does this (0 times
+// infinity would be a NaN).  A NaN in z is in e as well.
 __device__ __forceinline__ float pass_chunk(float z, float h, float e) {
-  const bool far = FAR && z > 126.0f;
-  const float f = exp2_hw(far ? std::min(0.5f * z, 127.0f) : z);
-  return fmaf(f, far ? f * h : h, e);
+  const float f = exp2_hw(fminf(z, 127.0f));
+  return fmaf(f, f * h, e);
 }
 
-// The state behind `count` chunks from the state h in front of them (their end states from zero and sums of delta): chunks
-// q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.  Returns the largest exponent met:
-// without FAR, for which decays are the usual thing, h is right if it is no larger than 126.
-template <class G, int NS, bool VEC, bool FAR>
-__device__ __forceinline__ float pass_chunks(const ScanParams& p, const Where& w, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
-  float most = 0.0f;
-  if (count <= 0) return most;
+// The state behind `count` chunks from the state h in front of them (their end states from zero and sums of delta, halved): chunks
+// q, q + step, ..  A chunk's values are on their way while the one in front of it is worked on.
+template <class G, int NS, bool VEC>
+__device__ __forceinline__ void pass_chunks(const ScanParams& p, const Where& w, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
+  if (count <= 0) return;
   const int64_t D = p.a.D;
   float e[4][NS], s[4];
   const auto load = [&](int i) {
@@ -425,30 +420,11 @@ __device__ __forceinline__ float pass_chunks(const ScanParams& p, const Where& w
     }
     if (i + 1 < count) load(i + 1);
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < 4; ++c) {
 #pragma unroll
-      for (int n = 0; n < NS; ++n) {
-        const float z = A2[c][n] * s1[c];
-        if (!FAR) most = fmaxf(most, z);
-        h[c][n] = pass_chunk<FAR>(z, h[c][n], e1[c][n]);
-      }
-  }
-  return most;
-}
-// The same from `first` ([D][N] of the clip, or NULL: zero).
-template <class G, int NS, bool VEC>
-__device__ __forceinline__ void join_chunks(const ScanParams& p, const Where& w, const float* first, int q, int step, int count, const float (&A2)[4][NS], float (&h)[4][NS]) {
-  const auto begin = [&] {
-#pragma unroll
-    for (int c = 0; c < 4; ++c)
-#pragma unroll
-      for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
-    if (first) load_dn<NS>(p, first + (int64_t)w.b * p.a.D * p.a.N, w, h);
-  };
-  begin();
-  if (__any(pass_chunks<G, NS, VEC, false>(p, w, q, step, count, A2, h) > 126.0f)) {
-    begin();
-    pass_chunks<G, NS, VEC, true>(p, w, q, step, count, A2, h);
+      for (int n = 0; n < NS; ++n) h[c][n] = pass_chunk(A2[c][n] * s1[c], h[c][n], e1[c][n]);
+      __builtin_amdgcn_sched_barrier(0);  // all at once they would take the registers of the rows on their way
+    }
   }
 }
 
@@ -517,7 +493,12 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(S
   if (!ENDS && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, h);
   } else {
-    join_chunks<G, NS, VEC>(p, w, ENDS ? nullptr : a.h0, 0, 1, ENDS ? 0 : w.chunk, A2, h);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < NS; ++n) h[c][n] = 0.0f;
+    if (!ENDS && a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
+    if (!ENDS) pass_chunks<G, NS, VEC>(p, w, 0, 1, w.chunk, A2, h);
   }
   arrived<NS>(h);
 
@@ -592,6 +573,8 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(S
     if (w.s == 0) {
       float v[4];
       get4(&s_dl[0][4 * w.j], v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] *= 0.5f;
       store_n<float, 4, VEC>(p.chunk_s + ((int64_t)w.b * p.K + w.chunk) * a.D + w.c0, w.nc, v);
     }
   } else if (a.h_last && w.chunk == p.K - 1) {
@@ -624,37 +607,26 @@ __global__ void __launch_bounds__(1024) chunk_join_kernel(const ScanParams p) {
   const int per = (k_own + SEG - 1) / SEG, q0 = seg * per, q1 = live ? std::min(q0 + per, k_own) : 0;
   const auto at = [&](int q) { return (int64_t)(BACK ? k_own - 1 - q : q); };
   // the last chunk of the walk hands nothing on
-  const auto ends = [&](auto far) {
-    float h = 0.0f, s = 0.0f, most = 0.0f;
+  {
+    float h = 0.0f, s = 0.0f;
 #pragma unroll 4
     for (int q = q0; q < std::min(q1, k_own - 1); ++q) {
-      const float sk = sp[at(q) * a.D], z = A2 * sk;
-      h = pass_chunk<decltype(far)::value>(z, h, hp[at(q) * NP * a.D]);
+      const float sk = sp[at(q) * a.D];
+      h = pass_chunk(A2 * sk, h, hp[at(q) * NP * a.D]);
       s += sk;
-      most = fmaxf(most, z);
     }
     s_h[seg][lane] = h;
     s_s[seg][lane] = s;
-    return fmaxf(most, A2 * s);
-  };
-  const auto starts = [&](auto far) {
-    constexpr bool FAR = decltype(far)::value;
-    float h = first && real && live ? first[(b * a.D + d) * a.N + n] : 0.0f;
-    for (int k = 0; k < seg; ++k) h = pass_chunk<FAR>(A2 * s_s[k][lane], h, s_h[k][lane]);
-#pragma unroll 4
-    for (int q = q0; q < q1; ++q) {
-      const bool more = q < k_own - 1;
-      const float end = more ? hp[at(q) * NP * a.D] : 0.0f, sk = more ? sp[at(q) * a.D] : 0.0f;
-      hp[at(q) * NP * a.D] = h;
-      h = pass_chunk<FAR>(A2 * sk, h, end);
-    }
-  };
-  if (__syncthreads_or(ends(std::false_type{}) > 126.0f)) {
-    ends(std::true_type{});
     __syncthreads();
-    starts(std::true_type{});
-  } else {
-    starts(std::false_type{});
+  }
+  float h = first && real && live ? first[(b * a.D + d) * a.N + n] : 0.0f;
+  for (int k = 0; k < seg; ++k) h = pass_chunk(A2 * s_s[k][lane], h, s_h[k][lane]);
+#pragma unroll 4
+  for (int q = q0; q < q1; ++q) {
+    const bool more = q < k_own - 1;
+    const float end = more ? hp[at(q) * NP * a.D] : 0.0f, sk = more ? sp[at(q) * a.D] : 0.0f;
+    hp[at(q) * NP * a.D] = h;
+    h = pass_chunk(A2 * sk, h, end);
   }
 }
 
@@ -776,7 +748,8 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
   if (!ENDS && w.own > 0 && p.K > kOwnJoin) {
     load_plane<NS, VEC>(p.chunk_h + ((int64_t)w.b * p.K + w.chunk) * G::NP * a.D, a.D, w, g);
   } else if (!ENDS) {
-    join_chunks<G, NS, VEC>(p, w, a.dh_last, p.K - 1, -1, w.own > 0 ? p.K - 1 - w.chunk : 0, A2, g);
+    if (a.dh_last) load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
+    if (w.own > 0) pass_chunks<G, NS, VEC>(p, w, p.K - 1, -1, p.K - 1 - w.chunk, A2, g);
   }
   arrived<NS>(g);
 
@@ -992,6 +965,8 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
     if (w.s == 0) {
       float v[4];
       get4(&s_dl[0][4 * w.j], v);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] *= 0.5f;
       store_n<float, 4, VEC>(p.chunk_s + ((int64_t)w.b * p.K + w.chunk) * a.D + w.c0, w.nc, v);
     }
     return;
