@@ -234,16 +234,6 @@ __device__ __forceinline__ void put4(const float (&v)[4], float* to) {
   *reinterpret_cast<f32x4*>(to) = f32x4{v[0], v[1], v[2], v[3]};
 }
 
-// The states are there from here on: where a branch left their loads under way, the first tile's frames would wait for them, and with them
-// for the next tile's rows, in every tile (64 clips of up to 1024 x 768 x 16: 177 us, 161 so).
-template <int NS>
-__device__ __forceinline__ void arrived(float (&h)[4][NS]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-#pragma unroll
-    for (int n = 0; n < NS; ++n) asm volatile("" : "+v"(h[c][n]));
-}
-
 // What a frame of a tile needs out of LDS; row, state: the lane's places in the tile's first frame.
 template <int NS>
 struct Step {
@@ -500,7 +490,6 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(S
     if (!ENDS && a.h0) load_dn<NS>(p, a.h0 + (int64_t)w.b * a.D * a.N, w, h);
     if (!ENDS) pass_chunks<G, NS, VEC>(p, w, 0, 1, w.chunk, A2, h);
   }
-  arrived<NS>(h);
 
   for (int i0 = w.begin; i0 < w.end; i0 += G::TT) {
     T4<T> xs[G::R], zs[G::R];
@@ -751,7 +740,6 @@ __global__ void __launch_bounds__((64 * waves_of<T, true, ENDS>()), (ENDS ? 4 : 
     if (a.dh_last) load_dn<NS>(p, a.dh_last + (int64_t)w.b * a.D * a.N, w, g);
     if (w.own > 0) pass_chunks<G, NS, VEC>(p, w, p.K - 1, -1, p.K - 1 - w.chunk, A2, g);
   }
-  arrived<NS>(g);
 
   // what the lane adds to dB and dC: one of its 2 NS sums, or none
   const int held = sum_index<2 * NS, G::J>(w.j), place = held < 0 ? -1 : held < NS ? w.s * NS + held : G::NP + w.s * NS + held - NS;
@@ -1094,7 +1082,7 @@ Shape shape_of(int N, bool thin) {
 
 struct Layout {
   bool thin;
-  int32_t K, tiles, nt, ns;
+  int32_t K, tiles, ns;
   int64_t h, s, bc, pa, pd, total;  // float offsets into the workspace
 };
 
@@ -1155,7 +1143,7 @@ Layout layout_of(const sed_scan_args& a, bool back) {
     const int32_t tiles = (int32_t)((cg + c.CW - 1) / c.CW), nt = (int32_t)((a.L + c.TT - 1) / c.TT);
     double t;
     const int64_t K = chunks_of(a, c, a.B * a.G * tiles, nt, back, t);
-    if (best == 0.0 || t < best) best = t, s = c, l.thin = thin, l.tiles = tiles, l.nt = nt, l.K = (int32_t)K;
+    if (best == 0.0 || t < best) best = t, s = c, l.thin = thin, l.tiles = tiles, l.K = (int32_t)K;
   }
   l.ns = (int32_t)((a.L + s.TS - 1) / s.TS);
   const int64_t K = l.K;
