@@ -356,6 +356,9 @@ int sed_resampler_forward(const sed_resampler* r, const void* pcm, int32_t pcm_k
  * The caller gives the workspace the matching sed_*_workspace function asks for (bytes, 16-byte aligned); its contents need not
  * live past the call's work on `stream`.  Results do not depend on timing: no sum is formed with atomics.  The entry points only
  * launch kernels, so they can be captured into a HIP graph; two graphs that may run at the same time need workspaces of their own.
+ * A call that would need a launch of 2^32 threads or more is refused with SED_ERR_CAPACITY and launches nothing.  Far from that: a scan or
+ * a convolution takes a wave of 64 threads for a run of frames of 16 to 256 neighbouring channels of a clip, a norm 64 to 1024 threads for
+ * a clip's group.
  * All pointers belong to the current device. */
 enum { SED_F32 = 0, SED_BF16 = 1, SED_F16 = 2 };
 enum { SED_ACT_NONE = 0, SED_ACT_SILU = 1, SED_ACT_RELU = 2, SED_ACT_GELU = 3 };
@@ -400,7 +403,7 @@ int sed_gated_scan_step(const sed_scan_args* args, void* stream);
 
 /* y_t[d] = act(bias[d] + sum_k weight[d,k] x_{t-W+1+k}[d]), x in front of the first frame = state or zero. */
 typedef struct sed_conv_args {
-  int64_t B, L, D;
+  int64_t B, L, D;          /* D <= 2^24                                                           */
   int32_t W;                /* taps, 1..8                                                          */
   int32_t dtype;            /* x, y, state and their gradients                                     */
   int32_t act;              /* SED_ACT_NONE or SED_ACT_SILU                                        */

@@ -734,7 +734,8 @@ struct Layout {
   int32_t blocks, late;
 };
 // Blocks of a clip: 2048 over the batch, eight for each compute unit (4096 cost the joining kernels more than they gave the others);
-// a block walks 32 places and 4096 values at least, so that its sums cost little beside its rows.  The second walk leaves no sums:
+// no more than one for every 32 places and 4096 values of the padded length (rounded up), so that its sums cost little beside its rows.  A
+// clip's own places are divided evenly among them: a short clip's blocks may have one place or none.  The second walk leaves no sums:
 // 8192 blocks, which end closer together (32 x 1001 x 64 x 64 forward and gradient: 435 us with 2048, 429 with 4096, 423 with 8192,
 // 450 with 16384; fewer than 32 places each: 64 clips of up to 862 x 768 in 72 us, 57 with 32).
 Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
@@ -754,9 +755,11 @@ Layout layout_of(int64_t B, int64_t S, int64_t C, int64_t G) {
 
 // Threads of norm_whole_kernel (BACK: of norm_whole_grad_kernel) for lanes of V channels and `held` rows, or 0 where it does not fit
 // or is slower: 8 rows a lane (more registers, more code) beyond a workgroup a compute unit (64 x 862 x 768 bf16: 71 us, the walks 68;
-// 16 x 101 x 64 x 32 fp32 15 us, 17); pieces of lines under 32 bytes where more than 96 MB are read (4 channels a group of 256 x 101 x
-// 32 x 32: fp32 62 us, the walks 57, bf16 gradient 106, 73; but 64 x 125 x 16 x 64 fp32 23, 28 and gradient 37, 44).  Many groups: as
-// few threads as hold one, so that a compute unit has several; else all, for the shortest way through.
+// 16 x 101 x 64 x 32 fp32 15 us, 17); pieces of lines under 32 bytes where more than 96 MiB are read (4 channels a group of 256 x 101 x
+// 32 x 32: fp32 62 us, the walks 57, bf16 gradient 106, 73; but 64 x 125 x 16 x 64 fp32 23, 28 and gradient 37, 44).  The border lies
+// right under what was measured slower (98 MiB and more; up to 73 MiB was faster), too high for bf16 gradients: 1960 x 200 x 64 in 8
+// groups takes 183 us forward and gradient, 2000 clips of it by the walks 144.  Many groups: as few threads as hold one, so that a
+// compute unit has several; else all, for the shortest way through.
 int whole_threads(const NormParams& p, int V, int held, bool back) {
   const sed_norm_args& a = p.a;
   const int64_t cg = a.C / a.G, nv = cg / V, items = a.B * a.G;

@@ -20,9 +20,10 @@
 // tile's frames, was slower for the registers it took (two waves a unit need 256 at most).
 // States, decays and sums are fp32; x, dt, z, B, C, y and their gradients are fp32, bf16 or fp16, rounded once at the store.
 //
-// Measured (MI355X, bf16, N = 16): 16 x 513 x 1536 forward 111 us in one pass of thin waves (134 in chunks of wide ones), 1.8e12
-// states of a frame a second; its gradient 202 us and 54 us for the chunks' ends: 26.5 vector instructions a state and
-// frame, of which 16 are the formulas', the vector units issuing 76 % of the time.  64 clips of up to 1024 x 768: 167 us.
+// Measured (MI355X, bf16, N = 16): 16 x 513 x 1536 forward 107 us in one pass of thin waves (46 + 67 in chunks of wide ones), 1.9e12
+// states of a frame a second; its gradient 190 .. 203 us and 50 .. 53 us for the chunks' ends: 26.5 vector instructions a state and
+// frame, of which 16 are the formulas', the vector units issuing 76 % of the time.  64 clips of up to 1024 x 768, 31759 frames
+// together: 169 us.
 // 512 streams x 1536 x 16, one frame: 25 us for 107 MB (4.2 TB/s; a 1 GiB copy reaches 5.1).
 #include "seq_core.h"
 
@@ -103,8 +104,8 @@ __device__ __forceinline__ int chunk_begin(const ScanParams& p, int own, int k) 
 }
 
 // The clip that place q of the batch stands for.  Clips of other lengths are started by 64, the longest ones first, so that the last
-// waves to end are short ones: 64 clips of up to 1024 x 768 x 16 forward take 186 us, 228 in the batch's own order, their gradient
-// 566 us, 620 (other batches 5 .. 25 % less).  A wave ranks its 64 clips by itself, 5 instructions each.
+// waves to end are short ones: 64 clips of up to 1024 x 768 x 16 (31759 frames together, the longest 1009) forward take 169 us, 223 in the
+// batch's own order; both passes of another batch's gradient 563 us, 634.  A wave ranks its 64 clips by itself, 5 instructions each.
 __device__ __forceinline__ int by_length(const sed_scan_args& a, int q) {
   const int lane = threadIdx.x % 64, first = q & ~63, n = (int)std::min<int64_t>(64, a.B - first);
   const int mine = lane < n ? std::max(0, std::min((int)a.L, a.frames[first + lane])) : -1;
@@ -513,7 +514,7 @@ __global__ void __launch_bounds__((64 * waves_of<T, false, ENDS>()), (per_unit(S
     if (!ENDS) put_states<G, T>(p, w, i0, cv, &s_C[0][0]);
     if (i0 + G::TT < w.end) fetch(i0 + G::TT);
     wave_sync();
-// a frame's values are read while the frame in front of it is worked on
+    // a frame's values are read while the frame in front of it is worked on
     const int row = 4 * w.j, state = w.s * NS;
     Step<NS> f[2];
     f[0].template get<G, true, false, !ENDS>(row, state, 0, s_dl[0], s_dx[0], nullptr, s_B[0], s_C[0]);

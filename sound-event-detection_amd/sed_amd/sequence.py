@@ -250,7 +250,7 @@ def gated_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False, fra
 def gated_scan_step(state, x, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=False):
     """One frame of gated_scan for a batch of streams: state (streams, channels, states) fp32, contiguous, is updated in place;
     x, dt, z (streams, channels), B, C (streams, states) or (streams, groups, states).  Returns y (streams, channels).  For
-    inference: it has no gradient."""
+    inference: it has no gradient, and a gradient that kept this state as an input raises afterwards."""
     what = "gated_scan_step"
     _check_x(what, x, 2)
     g, n = _scan_checks(what, x, dt, A, B, C, D, z, dt_bias, 1)
@@ -371,7 +371,8 @@ def causal_conv(x, weight, bias=None, activation=None, frames=None, reverse=Fals
 
 def causal_conv_step(state, x, weight, bias=None, activation=None):
     """One frame of causal_conv for a batch of streams: state (streams, W - 1, channels) of x's type, contiguous, moves up by the
-    new row in place; x (streams, channels).  Returns y (streams, channels).  For inference: it has no gradient."""
+    new row in place; x (streams, channels).  Returns y (streams, channels).  For inference: it has no gradient, and a gradient that
+    kept this state as an input (causal_conv's does) raises afterwards."""
     what = "causal_conv_step"
     _check_x(what, x, 2)
     weight = _conv_checks(what, x, weight, bias, activation)
@@ -451,7 +452,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, activation=None,
     x (clips, frames, ..., channels) fp32, bf16 or fp16: mean and (biased) variance are taken per clip and group of
     channels // groups neighbouring channels over the clip's own frames and all axes in between.  weight, bias (channels,), any
     floating type, or None; activation None, "silu", "relu" or "gelu" (the exact one).  frames (clips,) int32 on the device:
-    rows behind a clip's own give zero and are not read."""
+    rows behind a clip's own give zero and are not read.  At most 65535 clips and 2^19 channels."""
     what = "group_norm_act"
     if not torch.is_tensor(x) or x.dim() < 3:
         raise ValueError(f"{what}: x: (clips, frames, ..., channels)")
