@@ -457,3 +457,55 @@ def test_scan_gradient_of_more_rows_than_a_grid_has_threads():
         _close(grads[k], o[NAMES[k]][0], _scan_bound(o, NAMES[k], 3, n, 1), NAMES[k])
     rest = grads["B"][(1 << 18) - 100000:(1 << 18)]
     assert (rest == 0).all()
+
+
+@pytest.mark.parametrize("dtype", (torch.float32, torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("n,ns,d", ((40, 16, 7), (600, 16, 64), (50, 4, 12), (3000, 8, 5)))
+def test_scan_steps_masked_by_the_lowest_value(n, ns, d, dtype):
+    """dt of the type's lowest value behind a softplus is no step at all, z of it a closed gate: the state passes, every output is finite."""
+    import sed_amd
+    dev, ref, rng = _scan_inputs(2, n, d, 1, ns, dtype, n + d, state=True)
+    low = torch.finfo(dtype).min
+    hit = rng.random((2, n, d)) < 0.3
+    for k, where in (("dt", hit), ("z", np.roll(hit, 1, 1))):
+        dev[k][torch.from_numpy(where).to(_dev())] = low
+        ref[k][where] = low
+    dy, rdy = _rounded(rng.standard_normal((2, n, d)), dtype)
+    dl, rdl = _rounded(rng.standard_normal((2, d, ns)), torch.float32)
+    leaves = {k: t.requires_grad_(True) for k, t in dev.items()}
+    args = dict(leaves)
+    y, last = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, softplus=True, return_state=True)
+    with np.errstate(over="ignore"):
+        o = S.scan(**ref, use_softplus=True, dy=rdy, dlast=rdl)
+    _close(y, o["y"][0], _scan_bound(o, "y", 2, n, d), "y")
+    _close(last, o["last"][0], _scan_bound(o, "last", 2, n, d), "last")
+    for (k, t), got in zip(leaves.items(), torch.autograd.grad([y, last], list(leaves.values()), [dy, dl])):
+        _close(got, o[NAMES[k]][0], _scan_bound(o, NAMES[k], 2, n, d), NAMES[k])
+
+
+@pytest.mark.parametrize("reverse", (False, True))
+@pytest.mark.parametrize("n,d,ns", ((40, 6, 16), (700, 64, 16), (50, 12, 4), (3000, 5, 8), (90, 9, 1), (200, 20, 32)))
+def test_scan_infinities_reach_later_frames_of_their_channel_only(n, d, ns, reverse):
+    """A value of x that is no number: other channels and clips, the frames walked before it and the gradient of x, which does not read x,
+    keep their bits; dB and dC do in the frames walked before."""
+    import sed_amd
+    dev, _, rng = _scan_inputs(2, n, d, 1, ns, torch.float32, n, gate=False, state=True)
+    dy = torch.from_numpy(rng.standard_normal((2, n, d)).astype(np.float32)).to(_dev())
+    t0, c0, got = n // 3, d // 2, []
+    for bad in (None, float("nan"), float("inf")):
+        leaves = {k: t.clone() for k, t in dev.items()}
+        if bad is not None:
+            leaves["x"][0, t0, c0] = bad
+        for t in leaves.values():
+            t.requires_grad_(True)
+        args = dict(leaves)
+        y = sed_amd.gated_scan(*[args.pop(k) for k in ("x", "dt", "A", "B", "C")], **args, softplus=True, reverse=reverse)
+        got.append((y, *torch.autograd.grad(y, [leaves["x"], leaves["B"], leaves["C"]], dy)))
+    before = torch.arange(n, device=_dev()) > t0 if reverse else torch.arange(n, device=_dev()) < t0
+    rest = torch.arange(d, device=_dev()) != c0
+    y, dx, dB, dC = got[0]
+    for by, bdx, bdB, bdC in got[1:]:
+        assert torch.equal(by[1], y[1]) and torch.equal(by[0][:, rest], y[0][:, rest]) and torch.equal(by[0][before], y[0][before])
+        assert not by[0, t0, c0].isfinite()
+        assert torch.equal(bdx, dx)
+        assert torch.equal(bdB[1], dB[1]) and torch.equal(bdC[1], dC[1]) and torch.equal(bdB[0][before], dB[0][before]) and torch.equal(bdC[0][before], dC[0][before])
